@@ -449,6 +449,166 @@ megacu_status megacu_b200_events_status(void *events, void *stream,
 megacu_status megacu_b200_events_counters(void *events, void *stream,
                                           uint64_t counters[8]);
 
+/* ---- routing of tokens to experts (new, no counterpart in megacu) --------- */
+
+/*
+ * A batch of `tokens` tokens, each with `topk` expert ids, on a PE that holds
+ * experts [first_expert, first_expert + experts). Slot s = token * topk +
+ * choice. In the sorted order every expert has a contiguous range of rows
+ * that starts at a multiple of `align`; slots whose id lies elsewhere have no
+ * row (-1). Two choices of one token may name the same expert.
+ */
+typedef struct megacu_moe_problem {
+  int64_t tokens;       /* 0 is an empty batch; tokens * topk <= 2^30 */
+  int64_t hidden;       /* elements of a row; not read by the sort */
+  int32_t topk;         /* 1..32 */
+  int32_t experts;      /* experts held here, 1..1024 */
+  int32_t first_expert; /* id of the first of them */
+  int32_t align;        /* 1..1024; 128 for products by expert */
+  int32_t dtype;        /* of the rows: f16, bf16 or f32 (enum megacu_dtype) */
+  int32_t id_bytes;     /* 4 (or 0): int32 ids, 8: int64 */
+  int64_t token_stride; /* elements between rows of x, y, dy; 0 = hidden */
+  int64_t row_stride;   /* elements between rows of rows, drows; 0 = hidden */
+} megacu_moe_problem;
+
+/* sizes[0] rows the sorted order can need (entries of slot_of_row, rows of
+ * `rows`), sizes[1] bytes of the sort's workspace (0: none). */
+megacu_status megacu_b200_moe_sizes(const megacu_moe_problem *problem, int64_t sizes[2]);
+
+/*
+ * Stable counting sort of the slots by expert. expert_ids: [tokens, topk].
+ * Writes int32 counts [experts], offsets [experts + 1] (offsets[e] the first
+ * row of expert e, offsets[experts] the rows in use, padding included),
+ * row_of_slot [tokens, topk] (-1: not here) and slot_of_row [sizes[0]] (-1:
+ * padding and rows behind the last). Rows of an expert are in slot order.
+ * workspace: sizes[1] bytes, need not be initialised, nothing is kept in it
+ * between calls; one per concurrent call.
+ */
+megacu_status megacu_cuda_moe_sort(megacu_driver_view driver, const void *expert_ids,
+                                   void *counts, void *offsets, void *row_of_slot,
+                                   void *slot_of_row, void *workspace,
+                                   const megacu_moe_problem *problem);
+
+/* rows[row_of_slot[t, j]] = x[t]; other rows are left as they were. Its
+ * gradient is megacu_cuda_moe_combine of the rows' gradient without weights. */
+megacu_status megacu_cuda_moe_dispatch(megacu_driver_view driver, const void *x,
+                                       const void *row_of_slot, void *rows,
+                                       const megacu_moe_problem *problem);
+
+/* y[t] = sum_j weights[t, j] * rows[row_of_slot[t, j]] over the slots that
+ * have a row (0 when none has), summed in fp32 in the order of j and rounded
+ * once. weights: fp32 [tokens, topk], NULL = 1. */
+megacu_status megacu_cuda_moe_combine(megacu_driver_view driver, const void *rows,
+                                      const void *weights, const void *row_of_slot, void *y,
+                                      const megacu_moe_problem *problem);
+
+/* The weighted combine's gradient: drows[row_of_slot[t, j]] = weights[t, j] *
+ * dy[t] (other rows are left as they were) and dweights[t, j] = <dy[t],
+ * rows[row_of_slot[t, j]]> in fp32, 0 for a slot without a row. drows may be
+ * `rows`. */
+megacu_status megacu_cuda_moe_combine_grad(megacu_driver_view driver, const void *dy,
+                                           const void *rows, const void *weights,
+                                           const void *row_of_slot, void *drows,
+                                           void *dweights,
+                                           const megacu_moe_problem *problem);
+
+/* ---- 4-bit block formats and their products (new, no counterpart in megacu) */
+
+/*
+ * Elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two per byte, the
+ * lower nibble first; each block of a row has one scale byte. A quantised
+ * matrix [rows, cols] is `data` [rows, cols / 2] bytes, row-major, and
+ * `scales`: tiles of 128 rows x 4 blocks, tile (row tile, block / 4) at 512 *
+ * (row tile * tiles per row + block / 4), in it row r, block b at byte
+ * (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4.
+ */
+enum megacu_fp4_format {
+  MEGACU_FP4_MX = 0, /* blocks of 32, scale byte 2^(byte - 127), 255 = NaN */
+  MEGACU_FP4_NV = 1  /* blocks of 16, scale byte e4m3, 127 = NaN */
+};
+
+typedef struct megacu_fp4_matrix {
+  int64_t rows;      /* rows of the quantised matrix; 0 is empty */
+  int64_t cols;      /* its columns (a product's k); multiple of 32 */
+  int64_t stride;    /* elements between rows of the plain matrix as stored; 0 = dense */
+  int32_t format;    /* enum megacu_fp4_format */
+  int32_t dtype;     /* of the plain matrix: f16, bf16 or f32 */
+  int32_t transpose; /* 1: the plain matrix is stored [cols, rows] */
+  int32_t topk;      /* > 0: row r is the plain matrix's row slot_of_row[r] / topk */
+  float scale;       /* g, a power of two from 2^-60 to 2^60; 1 = none */
+} megacu_fp4_matrix;
+
+/* sizes[0] bytes of data, sizes[1] bytes of scales. */
+megacu_status megacu_b200_fp4_sizes(const megacu_fp4_matrix *matrix, int64_t sizes[2]);
+
+/*
+ * With z = g * x and amax the largest |z| of a block:
+ *   MX scale = 2^e, e = floor(log2(amax)) - 2 within [-127, 127]
+ *   NV scale = e4m3 nearest to min(amax / 6, 448), ties to even
+ *   element  = e2m1 nearest to z / scale, ties to even, at most 6 in magnitude
+ * decided on the exact quotients. A block with an infinity or NaN gets a NaN
+ * scale; an NV block whose scale rounds to 0 holds zeros. Scale bytes behind
+ * the last row or column of a tile are 0. With slot_of_row (int32 [rows], as
+ * megacu_cuda_moe_sort writes it) rows whose entry is negative are left as
+ * they were, scales included, and x is gathered when topk > 0; NULL: every row.
+ */
+megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, const void *x,
+                                       const void *slot_of_row, void *data, void *scales,
+                                       const megacu_fp4_matrix *matrix);
+
+/* out[r, c] = element * scale / g, rounded once to matrix->dtype; transpose
+ * and topk must be 0, stride is out's. */
+megacu_status megacu_cuda_fp4_dequantize(megacu_driver_view driver, const void *data,
+                                         const void *scales, void *out,
+                                         const megacu_fp4_matrix *matrix);
+
+typedef struct megacu_fp4_gemm_problem {
+  int64_t m;           /* rows of A; by expert: its capacity, a multiple of 128 */
+  int64_t n;           /* rows of B (of each expert's B) = columns of out */
+  int64_t k;           /* multiple of 32 */
+  int64_t out_stride;  /* elements between rows of out; 0 = n */
+  int32_t format;      /* enum megacu_fp4_format, of both operands */
+  int32_t out_dtype;   /* f16, bf16 or f32 */
+  int32_t experts;     /* 0: one B; else B is [experts, n, k], at most 1024 */
+  int32_t tile_n;      /* 0 = auto; else 128 or 256 accumulator columns per tile */
+  int32_t split;       /* 0 = auto; else 1, 2, 4 or 8 CTAs share a tile's K */
+  float alpha;         /* 1 / (g_a * g_b) undoes the operands' scales */
+  uint64_t timeout_ns; /* bound of every wait inside the launch; 0 = 4 s */
+} megacu_fp4_gemm_problem;
+
+/* Bytes of `events` of the products: zero-filled once, then reused; it holds
+ * only the error word that megacu_b200_events_status reads and clears
+ * (detail 41; info[0] = tile, info[2] = which wait: 51 producer's free stage,
+ * 52 MMA's free accumulator, 53 MMA's full stage, 54 epilogue's accumulator). */
+megacu_status megacu_b200_fp4_events_bytes(int64_t *bytes);
+
+/*
+ * out[i, j] = alpha * sum_k A[i, k] * B[j, k] of two quantised matrices (both
+ * K-major, as megacu_cuda_fp4_quantize writes them), fp32 accumulation, one
+ * rounding. By expert (experts > 0): rows [offsets[e], offsets[e] + counts[e])
+ * of A are multiplied with B's expert e (its data at e * n rows, its scales at
+ * e times the scale bytes of an [n, k] matrix) and alpha * alphas[e] (fp32
+ * [experts], NULL = 1); offsets and counts are device int32 as
+ * megacu_cuda_moe_sort writes them with align 128, and other rows of out are
+ * left as they were. offsets, counts, alphas: NULL when experts is 0.
+ */
+megacu_status megacu_cuda_fp4_gemm(megacu_driver_view driver, const void *a,
+                                   const void *a_scales, const void *b, const void *b_scales,
+                                   const void *offsets, const void *counts,
+                                   const void *alphas, void *out, void *events,
+                                   const megacu_fp4_gemm_problem *problem);
+
+/* act[i, j] = silu(G[i, j]) * U[i, j] with G and U the two products as above
+ * (alpha and alphas scale both); tile_n must be 0 or 256 (128 gate and 128 up
+ * columns). */
+megacu_status megacu_cuda_fp4_gemm_swiglu(megacu_driver_view driver, const void *a,
+                                          const void *a_scales, const void *gate,
+                                          const void *gate_scales, const void *up,
+                                          const void *up_scales, const void *offsets,
+                                          const void *counts, const void *alphas, void *act,
+                                          void *events,
+                                          const megacu_fp4_gemm_problem *problem);
+
 /* ---- team: symmetric heap over NVLink peer mappings ---------------------- */
 
 /* Size of the opaque handle a PE exports for its heap. */

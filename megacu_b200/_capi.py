@@ -25,7 +25,8 @@ STATUS_NAMES = ["ok", "invalid_argument", "unsupported", "backend_error", "launc
 MODE_ALLREDUCE, MODE_REDUCE_SCATTER, MODE_ALLGATHER = 0, 1, 2
 ALGO_AUTO, ALGO_ONE_SHOT, ALGO_TWO_SHOT = 0, 1, 2
 CTA_PAIRS_AUTO, CTA_PAIRS_OFF, CTA_PAIRS_ON = 0, 1, 2
-DTYPE_BF16 = 2
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 1, 2, 3
+FP4_MX, FP4_NV = 0, 1
 
 
 class Status(ctypes.Structure):
@@ -68,6 +69,26 @@ class MlpChainProblem(ctypes.Structure):
     _fields_ = [("tokens", c_int64), ("hidden", c_int64), ("inter", c_int64),
                 ("layers", c_int32), ("algo", c_int32), ("deterministic", c_int32),
                 ("num_ctas", c_int32), ("cta_pairs", c_int32), ("single_launch", c_int32),
+                ("timeout_ns", c_uint64)]
+
+
+class MoeProblem(ctypes.Structure):
+    _fields_ = [("tokens", c_int64), ("hidden", c_int64), ("topk", c_int32),
+                ("experts", c_int32), ("first_expert", c_int32), ("align", c_int32),
+                ("dtype", c_int32), ("id_bytes", c_int32), ("token_stride", c_int64),
+                ("row_stride", c_int64)]
+
+
+class Fp4Matrix(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("cols", c_int64), ("stride", c_int64), ("format", c_int32),
+                ("dtype", c_int32), ("transpose", c_int32), ("topk", c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class Fp4GemmProblem(ctypes.Structure):
+    _fields_ = [("m", c_int64), ("n", c_int64), ("k", c_int64), ("out_stride", c_int64),
+                ("format", c_int32), ("out_dtype", c_int32), ("experts", c_int32),
+                ("tile_n", c_int32), ("split", c_int32), ("alpha", ctypes.c_float),
                 ("timeout_ns", c_uint64)]
 
 
@@ -115,6 +136,18 @@ _PROTOTYPES = {
         (Status, [GemmArProblemV2, c_int32, c_int32, ctypes.POINTER(c_int32)]),
     "megacu_b200_events_status": (Status, [c_void_p, c_void_p, ctypes.POINTER(c_int64)]),
     "megacu_b200_events_counters": (Status, [c_void_p, c_void_p, ctypes.POINTER(c_uint64)]),
+    # The last argument of these is a pointer to MoeProblem / Fp4Matrix / Fp4GemmProblem.
+    "megacu_b200_moe_sizes": (Status, [c_void_p, ctypes.POINTER(c_int64)]),
+    "megacu_cuda_moe_sort": (Status, [DriverView, *[c_void_p] * 7]),
+    "megacu_cuda_moe_dispatch": (Status, [DriverView, *[c_void_p] * 4]),
+    "megacu_cuda_moe_combine": (Status, [DriverView, *[c_void_p] * 5]),
+    "megacu_cuda_moe_combine_grad": (Status, [DriverView, *[c_void_p] * 7]),
+    "megacu_b200_fp4_sizes": (Status, [c_void_p, ctypes.POINTER(c_int64)]),
+    "megacu_cuda_fp4_quantize": (Status, [DriverView, *[c_void_p] * 5]),
+    "megacu_cuda_fp4_dequantize": (Status, [DriverView, *[c_void_p] * 4]),
+    "megacu_b200_fp4_events_bytes": (Status, [ctypes.POINTER(c_int64)]),
+    "megacu_cuda_fp4_gemm": (Status, [DriverView, *[c_void_p] * 10]),
+    "megacu_cuda_fp4_gemm_swiglu": (Status, [DriverView, *[c_void_p] * 12]),
     "megacu_b200_team_create":
         (Status, [c_int32, c_int32, c_int32, c_int64, ctypes.POINTER(c_void_p)]),
     "megacu_b200_team_export": (Status, [c_void_p, c_void_p]),

@@ -488,6 +488,309 @@ def mlp_chain(x, w_gate, w_up, w_down, out, *, act, workspace, x_work, events_sw
                                            problem.to_c()))
 
 
+# ---- routing of tokens to experts, 4-bit products ---------------------------------------
+
+class _CProblem:
+    """Base of the problem dataclasses passed by pointer: the C struct is built
+    once and reused until a field changes."""
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        self.__dict__.pop("_c", None)
+
+    def to_c(self):
+        c = self.__dict__.get("_c")
+        if c is None:
+            c = self.__dict__["_c"] = self._build()
+        return c
+
+
+_TORCH_NAMES = {_capi.DTYPE_F16: "torch.float16", _capi.DTYPE_BF16: "torch.bfloat16",
+                _capi.DTYPE_F32: "torch.float32"}
+
+
+def _buffer(x, name: str, elements: int, size: int, device: int, dtype: int = 0) -> Optional[int]:
+    """The address of ``x``; a tensor must be contiguous, on ``device``, with
+    elements of ``size`` bytes (of ``dtype`` when given) and at least
+    ``elements`` of them. Raw addresses (int) are taken as they are."""
+    if x is None or isinstance(x, int):
+        return x
+    if x.device.type == "cuda" and x.device.index != device:
+        raise ValueError(f"{name} is on {x.device}, the call on device {device}")
+    if x.element_size() != size or (dtype and str(x.dtype) != _TORCH_NAMES[dtype]):
+        raise ValueError(f"{name} has dtype {x.dtype}")
+    if x.numel() < elements or not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with at least {elements} elements")
+    return x.data_ptr()
+
+
+def _matrix(x, name: str, rows: int, cols: int, stride: int, dtype: int,
+            device: int) -> Optional[int]:
+    """The address of the row-major matrix ``x``, whose rows are ``stride``
+    elements apart (0: dense)."""
+    if x is None or isinstance(x, int):
+        return x
+    if stride == 0 or stride == cols:
+        return _buffer(x, name, rows * cols, 2 if dtype != _capi.DTYPE_F32 else 4, device, dtype)
+    if x.device.type == "cuda" and x.device.index != device:
+        raise ValueError(f"{name} is on {x.device}, the call on device {device}")
+    if str(x.dtype) != _TORCH_NAMES[dtype]:
+        raise ValueError(f"{name} has dtype {x.dtype}")
+    if (x.dim() != 2 or x.shape[0] < rows or x.shape[1] < cols or x.stride(1) != 1
+            or (rows > 1 and x.stride(0) != stride)):
+        raise ValueError(f"{name} must be [{rows}, {cols}] with rows {stride} elements apart")
+    return x.data_ptr()
+
+
+@dataclass
+class MoeProblem(_CProblem):
+    """megacu_moe_problem: ``tokens`` tokens with ``topk`` expert ids each, on a
+    PE that holds experts [first_expert, first_expert + experts). Strides are
+    in elements, 0 = hidden."""
+    tokens: int
+    topk: int
+    experts: int
+    hidden: int = 0
+    first_expert: int = 0
+    align: int = 1       # 128 for products by expert
+    dtype: int = _capi.DTYPE_BF16
+    token_stride: int = 0
+    row_stride: int = 0
+
+    def _build(self, id_bytes: int = 0):
+        return _capi.MoeProblem(tokens=self.tokens, hidden=self.hidden, topk=self.topk,
+                                experts=self.experts, first_expert=self.first_expert,
+                                align=self.align, dtype=self.dtype, id_bytes=id_bytes,
+                                token_stride=self.token_stride, row_stride=self.row_stride)
+
+
+def _moe_sizes(problem: MoeProblem) -> tuple[int, int]:
+    c = problem.to_c()
+    sizes = problem.__dict__.get("_sizes")
+    if sizes is None or sizes[0] is not c:
+        out = (ctypes.c_int64 * 2)()
+        check(lib().megacu_b200_moe_sizes(ctypes.byref(c), out))
+        sizes = problem.__dict__["_sizes"] = (c, out[0], out[1])
+    return sizes[1], sizes[2]
+
+
+def moe_rows(problem: MoeProblem) -> int:
+    """Rows the sorted order can need: entries of ``slot_of_row``, rows of ``rows``."""
+    return _moe_sizes(problem)[0]
+
+
+def moe_workspace_bytes(problem: MoeProblem) -> int:
+    return _moe_sizes(problem)[1]
+
+
+def moe_sort(expert_ids, *, counts, offsets, row_of_slot, slot_of_row, problem: MoeProblem,
+             workspace=None, stream=None, device: int = 0) -> None:
+    """Sorts the (token, choice) slots by expert, stably (async).
+    ``expert_ids`` [tokens, topk] int32 or int64; writes int32 ``counts``
+    [experts], ``offsets`` [experts + 1], ``row_of_slot`` [tokens, topk] and
+    ``slot_of_row`` [moe_rows(problem)]; -1 marks slots whose expert is
+    elsewhere and rows without a slot. ``workspace``: moe_workspace_bytes()."""
+    rows, need = _moe_sizes(problem)
+    slots, experts = problem.tokens * problem.topk, problem.experts
+    size = 4 if expert_ids is None or isinstance(expert_ids, int) else expert_ids.element_size()
+    c = problem.to_c() if size == 4 else problem._build(size)
+    check(lib().megacu_cuda_moe_sort(
+        _launch_view(stream, device, None), _buffer(expert_ids, "expert_ids", slots, size, device),
+        _buffer(counts, "counts", experts, 4, device),
+        _buffer(offsets, "offsets", experts + 1, 4, device),
+        _buffer(row_of_slot, "row_of_slot", slots, 4, device),
+        _buffer(slot_of_row, "slot_of_row", rows, 4, device),
+        _buffer(workspace, "workspace", need, 1, device) if need else None, ctypes.byref(c)))
+
+
+def _token_rows(x, name: str, p: MoeProblem, device: int) -> Optional[int]:
+    return _matrix(x, name, p.tokens, p.hidden, p.token_stride, p.dtype, device)
+
+
+def _expert_rows(x, name: str, p: MoeProblem, device: int) -> Optional[int]:
+    return _matrix(x, name, moe_rows(p), p.hidden, p.row_stride, p.dtype, device)
+
+
+def moe_dispatch(x, rows, *, row_of_slot, problem: MoeProblem, stream=None,
+                 device: int = 0) -> None:
+    """rows[row_of_slot[t, j]] = x[t] (async); other rows are left as they
+    were. The gradient is :func:`moe_combine` of the rows' gradient without
+    weights."""
+    p = problem
+    check(lib().megacu_cuda_moe_dispatch(
+        _launch_view(stream, device, None), _token_rows(x, "x", p, device),
+        _buffer(row_of_slot, "row_of_slot", p.tokens * p.topk, 4, device),
+        _expert_rows(rows, "rows", p, device), ctypes.byref(p.to_c())))
+
+
+def moe_combine(rows, y, *, row_of_slot, problem: MoeProblem, weights=None, stream=None,
+                device: int = 0) -> None:
+    """y[t] = sum over j of weights[t, j] * rows[row_of_slot[t, j]] (async), fp32
+    sums in the order of j, one rounding; ``weights`` fp32, None = 1."""
+    p, slots = problem, problem.tokens * problem.topk
+    check(lib().megacu_cuda_moe_combine(
+        _launch_view(stream, device, None), _expert_rows(rows, "rows", p, device),
+        _buffer(weights, "weights", slots, 4, device, _capi.DTYPE_F32),
+        _buffer(row_of_slot, "row_of_slot", slots, 4, device), _token_rows(y, "y", p, device),
+        ctypes.byref(p.to_c())))
+
+
+def moe_combine_grad(dy, rows, drows, dweights, *, weights, row_of_slot, problem: MoeProblem,
+                     stream=None, device: int = 0) -> None:
+    """Gradient of the weighted :func:`moe_combine` (async): drows = weights *
+    dy at the rows of each token (other rows are left as they were), dweights
+    [tokens, topk] fp32 = <dy[t], rows[...]>, 0 for a slot without a row."""
+    p, slots = problem, problem.tokens * problem.topk
+    check(lib().megacu_cuda_moe_combine_grad(
+        _launch_view(stream, device, None), _token_rows(dy, "dy", p, device),
+        _expert_rows(rows, "rows", p, device),
+        _buffer(weights, "weights", slots, 4, device, _capi.DTYPE_F32),
+        _buffer(row_of_slot, "row_of_slot", slots, 4, device),
+        _expert_rows(drows, "drows", p, device),
+        _buffer(dweights, "dweights", slots, 4, device, _capi.DTYPE_F32),
+        ctypes.byref(p.to_c())))
+
+
+@dataclass
+class Fp4Matrix(_CProblem):
+    """megacu_fp4_matrix: a quantised matrix [rows, cols] of FP4_MX or FP4_NV
+    blocks along its rows, and the plain matrix of ``dtype`` it comes from
+    (stored [cols, rows] with ``transpose``). ``scale``: a power of two that
+    multiplies the values before they are quantised."""
+    rows: int
+    cols: int
+    format: int = _capi.FP4_MX
+    dtype: int = _capi.DTYPE_BF16
+    transpose: bool = False
+    scale: float = 1.0
+    stride: int = 0
+
+    def _build(self, topk: int = 0):
+        return _capi.Fp4Matrix(rows=self.rows, cols=self.cols, stride=self.stride,
+                               format=self.format, dtype=self.dtype,
+                               transpose=1 if self.transpose else 0, topk=topk,
+                               scale=self.scale)
+
+
+def fp4_sizes(problem: Fp4Matrix) -> tuple[int, int]:
+    """Bytes of the data and of the scales of a quantised matrix."""
+    c = problem.to_c()
+    sizes = problem.__dict__.get("_sizes")
+    if sizes is None or sizes[0] is not c:
+        out = (ctypes.c_int64 * 2)()
+        check(lib().megacu_b200_fp4_sizes(ctypes.byref(c), out))
+        sizes = problem.__dict__["_sizes"] = (c, out[0], out[1])
+    return sizes[1], sizes[2]
+
+
+def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, topk: int = 0,
+                 stream=None, device: int = 0) -> None:
+    """Quantises ``x`` into ``data`` and ``scales`` (async). With
+    ``slot_of_row`` (of :func:`moe_sort`, int32 [rows]) rows whose entry is
+    negative are left as they were; with ``topk`` too, row r is taken from
+    x[slot_of_row[r] // topk]."""
+    p = problem
+    nbytes, sbytes = fp4_sizes(p)
+    if topk:  # the gathered rows' number is the batch's, known to the caller alone
+        x_ptr = _matrix(x, "x", 0, p.cols, p.stride, p.dtype, device)
+    elif p.transpose:
+        x_ptr = _matrix(x, "x", p.cols, p.rows, p.stride, p.dtype, device)
+    else:
+        x_ptr = _matrix(x, "x", p.rows, p.cols, p.stride, p.dtype, device)
+    c = p._build(topk) if topk else p.to_c()
+    check(lib().megacu_cuda_fp4_quantize(
+        _launch_view(stream, device, None), x_ptr,
+        _buffer(slot_of_row, "slot_of_row", p.rows, 4, device),
+        _buffer(data, "data", nbytes, 1, device), _buffer(scales, "scales", sbytes, 1, device),
+        ctypes.byref(c)))
+
+
+def fp4_dequantize(data, scales, out, *, problem: Fp4Matrix, stream=None,
+                   device: int = 0) -> None:
+    """The values of a quantised matrix (async): out [rows, cols] = element *
+    scale / problem.scale, rounded once to problem.dtype."""
+    p = problem
+    nbytes, sbytes = fp4_sizes(p)
+    check(lib().megacu_cuda_fp4_dequantize(
+        _launch_view(stream, device, None), _buffer(data, "data", nbytes, 1, device),
+        _buffer(scales, "scales", sbytes, 1, device),
+        _matrix(out, "out", p.rows, p.cols, p.stride, p.dtype, device), ctypes.byref(p.to_c())))
+
+
+@dataclass
+class Fp4Gemm(_CProblem):
+    """megacu_fp4_gemm_problem: out [m, n] = alpha * A [m, k] @ B [n, k]^T of
+    quantised matrices; ``experts`` > 0: B is [experts, n, k] and A's rows are
+    sorted by expert."""
+    m: int
+    n: int
+    k: int
+    format: int = _capi.FP4_MX
+    out_dtype: int = _capi.DTYPE_BF16
+    experts: int = 0
+    alpha: float = 1.0
+    out_stride: int = 0
+    tile_n: int = 0
+    split: int = 0
+    timeout_ns: int = 0
+
+    def _build(self):
+        return _capi.Fp4GemmProblem(m=self.m, n=self.n, k=self.k, out_stride=self.out_stride,
+                                    format=self.format, out_dtype=self.out_dtype,
+                                    experts=self.experts, tile_n=self.tile_n, split=self.split,
+                                    alpha=self.alpha, timeout_ns=self.timeout_ns)
+
+
+def fp4_events_bytes() -> int:
+    """Bytes of the products' ``events`` (zero-filled once, then reused)."""
+    out = ctypes.c_int64()
+    check(lib().megacu_b200_fp4_events_bytes(ctypes.byref(out)))
+    return out.value
+
+
+def _operand(data, scales, name: str, matrices: int, rows: int, p: Fp4Gemm, device: int):
+    """Addresses of a quantised operand of ``matrices`` matrices [rows, k]."""
+    tiles = -(-p.k // (128 if p.format == _capi.FP4_MX else 64))
+    return (_buffer(data, name, matrices * rows * (p.k // 2), 1, device),
+            _buffer(scales, name + "_scales", matrices * -(-rows // 128) * tiles * 512, 1, device))
+
+
+def _product(fn, weights, a, a_scales, out, offsets, counts, alphas, events, p: Fp4Gemm, stream,
+             device: int) -> None:
+    experts = max(p.experts, 1)
+    args = [*_operand(a, a_scales, "a", 1, p.m, p, device)]
+    for name, data, scales in weights:
+        args += _operand(data, scales, name, experts, p.n, p, device)
+    check(fn(_launch_view(stream, device, None), *args,
+             _buffer(offsets, "offsets", p.experts + 1, 4, device),
+             _buffer(counts, "counts", p.experts, 4, device),
+             _buffer(alphas, "alphas", p.experts, 4, device, _capi.DTYPE_F32),
+             _matrix(out, "out", p.m, p.n, p.out_stride, p.out_dtype, device),
+             _buffer(events, "events", 256 // events.element_size(), events.element_size(), device)
+             if events is not None and not isinstance(events, int) else events,
+             ctypes.byref(p.to_c())))
+
+
+def fp4_gemm(a, a_scales, b, b_scales, out, *, events, problem: Fp4Gemm, offsets=None,
+             counts=None, alphas=None, stream=None, device: int = 0) -> None:
+    """out = alpha * A @ B^T of two quantised matrices (async), fp32
+    accumulation and one rounding. By expert: ``offsets`` and ``counts`` of
+    :func:`moe_sort` (align 128), ``alphas`` fp32 [experts] factors; rows
+    without a slot are left as they were."""
+    _product(lib().megacu_cuda_fp4_gemm, [("b", b, b_scales)], a, a_scales, out, offsets, counts,
+             alphas, events, problem, stream, device)
+
+
+def fp4_gemm_swiglu(a, a_scales, gate, gate_scales, up, up_scales, act, *, events,
+                    problem: Fp4Gemm, offsets=None, counts=None, alphas=None, stream=None,
+                    device: int = 0) -> None:
+    """act = silu(alpha * A @ gate^T) * (alpha * A @ up^T) of quantised
+    matrices (async); ``problem.n`` = act columns. By expert as
+    :func:`fp4_gemm`."""
+    _product(lib().megacu_cuda_fp4_gemm_swiglu, [("gate", gate, gate_scales), ("up", up, up_scales)],
+             a, a_scales, act, offsets, counts, alphas, events, problem, stream, device)
+
+
 def events_status(events, stream=None) -> list[int]:
     """Synchronises ``stream`` and raises MegacuError if a device wait failed."""
     info = (ctypes.c_int64 * 4)()

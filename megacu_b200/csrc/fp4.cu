@@ -1,0 +1,424 @@
+// 4-bit block formats (no counterpart in megacu): quantisation, the values
+// back, and the products of quantised matrices, dense or by expert.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+
+#include <megacu_b200.h>
+
+#include "kernels/fp4_gemm_kernel.cuh"
+#include "kernels/fp4_quant_kernel.cuh"
+#include "status.h"
+#include "tma_map.h"
+
+namespace {
+
+using namespace megacu_b200;
+
+constexpr int kMaxDevices = 64;
+constexpr std::int64_t kMaxDim = 1ll << 30;
+constexpr std::int32_t kMaxExperts = 1024;
+constexpr int kMaxLog2Scale = 60;
+
+bool known_format(std::int32_t f) { return f == MEGACU_FP4_MX || f == MEGACU_FP4_NV; }
+bool known_dtype(std::int32_t t) {
+  return t == MEGACU_DTYPE_F16 || t == MEGACU_DTYPE_BF16 || t == MEGACU_DTYPE_F32;
+}
+int element_size(std::int32_t dtype) { return dtype == MEGACU_DTYPE_F32 ? 4 : 2; }
+
+std::int64_t ceil_div(std::int64_t a, std::int64_t b) { return (a + b - 1) / b; }
+
+std::int64_t scale_tiles(std::int64_t cols, bool nv) { return ceil_div(cols, fp4_tile_cols(nv)); }
+
+megacu_status check_matrix(megacu_fp4_matrix const *m, int &log2_scale) {
+  if (m == nullptr) return fail(MEGACU_INVALID_ARGUMENT, 2, "missing matrix");
+  if (m->rows < 0 || m->cols < 1 || m->stride < 0 || m->topk < 0) {
+    return fail(MEGACU_INVALID_ARGUMENT, 1, "invalid matrix");
+  }
+  if (!known_format(m->format)) return fail(MEGACU_INVALID_ARGUMENT, 1, "unknown format");
+  if (!known_dtype(m->dtype)) return fail(MEGACU_UNSUPPORTED, 20, "dtype must be f16, bf16 or f32");
+  if (m->cols % 32 != 0) {
+    return fail(MEGACU_INVALID_ARGUMENT, 21, "cols must be a multiple of 32 (16-byte rows)");
+  }
+  if (m->rows > kMaxDim || m->cols > kMaxDim ||
+      ceil_div(m->rows, kScaleTileRows) * ceil_div(m->cols, kQuantCols) > 0x7fffffffll) {
+    return fail(MEGACU_UNSUPPORTED, 22, "dimension too large");
+  }
+  int e = 0;
+  if (!(std::frexp(m->scale, &e) == 0.5f) || e - 1 > kMaxLog2Scale || e - 1 < -kMaxLog2Scale) {
+    return fail(MEGACU_INVALID_ARGUMENT, 1, "scale must be a power of two, 2^-60 to 2^60");
+  }
+  log2_scale = e - 1;
+  return ok_status();
+}
+
+fp4_matrix_params matrix_params(megacu_fp4_matrix const &m, int log2_scale, void *data,
+                                void *scales, bool transpose) {
+  fp4_matrix_params p{};
+  p.rows = m.rows;
+  p.cols = static_cast<std::int32_t>(m.cols);
+  p.stride = m.stride != 0 ? m.stride : transpose ? m.rows : m.cols;
+  p.log2_scale = log2_scale;
+  p.tiles = static_cast<std::int32_t>(scale_tiles(m.cols, m.format == MEGACU_FP4_NV));
+  p.col_tiles = static_cast<std::uint32_t>(ceil_div(m.cols, kQuantCols));
+  p.topk = m.topk;
+  p.data = static_cast<std::uint8_t *>(data);
+  p.scales = static_cast<std::uint8_t *>(scales);
+  return p;
+}
+
+// Calls f with the element type (a value of it) and the format as constants.
+template <class F>
+void by_type(std::int32_t dtype, std::int32_t format, F f) {
+  auto with = [&](auto value) {
+    if (format == MEGACU_FP4_NV) {
+      f(value, std::true_type{});
+    } else {
+      f(value, std::false_type{});
+    }
+  };
+  if (dtype == MEGACU_DTYPE_F16) {
+    with(__half{});
+  } else if (dtype == MEGACU_DTYPE_BF16) {
+    with(__nv_bfloat16{});
+  } else {
+    with(float{});
+  }
+}
+
+// ---- product ---------------------------------------------------------------------
+
+// Bytes [rows, k / 2] in boxes of box_rows x 128 bytes, 128-byte swizzle.
+bool encode_fp4_map(CUtensorMap *map, void const *base, std::int64_t rows, std::int64_t k,
+                    std::uint32_t box_rows) {
+  auto const encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  cuuint64_t const dims[2] = {static_cast<cuuint64_t>(k / 2), static_cast<cuuint64_t>(rows)};
+  cuuint64_t const strides[1] = {static_cast<cuuint64_t>(k / 2)};
+  cuuint32_t const box[2] = {128, box_rows};
+  cuuint32_t const elem[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides,
+                box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct fp4_plan {
+  int tile_n = 256;  // accumulator columns of a tile
+  int split = 1;
+  std::int64_t m_tiles = 0, n_tiles = 0;
+};
+
+// Tile width and K split with the least work on the busiest SM, in units of
+// one 128 x 128 x 256 block of MMAs, which costs about as much as its loads;
+// a tile adds about 3 units of start-up and epilogue, a split 4 more for the
+// exchange.
+megacu_status make_plan(megacu_fp4_gemm_problem const &p, bool swiglu, int sms, fp4_plan &out) {
+  std::int64_t const k_blocks = ceil_div(p.k, kFp4BlockK);
+  std::int64_t best = -1;
+  for (int tile_n : {256, 128}) {
+    if ((swiglu && tile_n != 256) || (p.tile_n != 0 && p.tile_n != tile_n)) continue;
+    for (int split : {1, 2, 4, 8}) {
+      if (split > k_blocks || (p.split != 0 && p.split != split)) continue;
+      std::int64_t const m_tiles = ceil_div(p.m, kFp4BlockM);
+      std::int64_t const n_tiles = ceil_div(p.n, swiglu ? tile_n / 2 : tile_n);
+      std::int64_t const waves = ceil_div(m_tiles * n_tiles * split, sms);
+      std::int64_t const per_tile =
+          ceil_div(k_blocks, split) * (tile_n / 128) + 3 + (split > 1 ? 4 : 0);
+      std::int64_t const cost = waves * per_tile;
+      if (best < 0 || cost < best) {
+        best = cost;
+        out = {tile_n, split, m_tiles, n_tiles};
+      }
+    }
+  }
+  if (best < 0) return fail(MEGACU_UNSUPPORTED, 22, "tile_n or split not possible");
+  if (out.m_tiles * out.n_tiles * out.split > (1 << 28)) {
+    return fail(MEGACU_UNSUPPORTED, 22, "too many tiles");
+  }
+  return ok_status();
+}
+
+struct fp4_operands {
+  void const *a, *a_scales, *b, *b_scales, *b2, *b2_scales;
+};
+
+template <bool kNv, bool kSwiglu, int BN>
+cudaError_t launch_gemm(int device, int grid, cudaStream_t stream, CUtensorMap const (&maps)[4],
+                        fp4_gemm_params const &prm) {
+  constexpr auto kKernel = &fp4_gemm_kernel<kNv, kSwiglu, BN>;
+  constexpr int kSmem = fp4_config<kNv, BN>::smem_bytes;
+  static std::atomic<bool> configured[kMaxDevices] = {};
+  bool const known = device >= 0 && device < kMaxDevices;
+  if (!known || !configured[device].load(std::memory_order_acquire)) {
+    cudaError_t const e =
+        cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    if (known) configured[device].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(prm.split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kFp4Threads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = prm.split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kKernel, maps[0], maps[1], maps[2], maps[3], prm);
+}
+
+megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &op,
+                          void const *offsets, void const *counts, void const *alphas, void *out,
+                          void *events, megacu_fp4_gemm_problem const *problem, bool swiglu) {
+  if (problem == nullptr) return fail(MEGACU_INVALID_ARGUMENT, 2, "missing problem");
+  megacu_fp4_gemm_problem const &p = *problem;
+  if (p.m < 0 || p.n < 1 || p.k < 1 || p.experts < 0 || p.out_stride < 0) {
+    return fail(MEGACU_INVALID_ARGUMENT, 1, "invalid problem");
+  }
+  if (!known_format(p.format)) return fail(MEGACU_INVALID_ARGUMENT, 1, "unknown format");
+  if (!known_dtype(p.out_dtype)) {
+    return fail(MEGACU_UNSUPPORTED, 20, "out_dtype must be f16, bf16 or f32");
+  }
+  if (p.k % 32 != 0) {
+    return fail(MEGACU_INVALID_ARGUMENT, 21, "k must be a multiple of 32 (16-byte rows)");
+  }
+  if (p.out_stride != 0 && p.out_stride < p.n) {
+    return fail(MEGACU_INVALID_ARGUMENT, 1, "out_stride is smaller than n");
+  }
+  if (p.m > kMaxDim || p.n > kMaxDim || p.k > kMaxDim || p.experts > kMaxExperts ||
+      std::max(p.experts, 1) * p.n > kMaxDim) {
+    return fail(MEGACU_UNSUPPORTED, 22, "dimension or number of experts too large");
+  }
+  if (p.experts > 0 && p.m % kFp4BlockM != 0) {
+    return fail(MEGACU_UNSUPPORTED, 22, "rows by expert come in tiles of 128");
+  }
+  fp4_plan plan;
+  megacu_status const st = make_plan(p, swiglu, 148, plan);
+  if (st.code != MEGACU_OK) return st;
+  if (p.m == 0) return ok_status();
+  void const *const needed[] = {op.a, op.a_scales, op.b, op.b_scales, out, events};
+  for (void const *ptr : needed) {
+    if (ptr == nullptr) return fail(MEGACU_INVALID_ARGUMENT, 2, "missing storage");
+  }
+  if ((swiglu && (op.b2 == nullptr || op.b2_scales == nullptr)) ||
+      (p.experts > 0 && (offsets == nullptr || counts == nullptr))) {
+    return fail(MEGACU_INVALID_ARGUMENT, 2, "missing storage");
+  }
+  void const *const operands[] = {op.a, op.a_scales, op.b, op.b_scales, op.b2, op.b2_scales, events};
+  for (void const *ptr : operands) {
+    if (!aligned_to(ptr, 16)) {
+      return fail(MEGACU_INVALID_ARGUMENT, 21, "operands and events must be 16-byte aligned");
+    }
+  }
+  if (!aligned_to(out, element_size(p.out_dtype)) || !aligned_to(offsets, 4) ||
+      !aligned_to(counts, 4) || !aligned_to(alphas, 4)) {
+    return fail(MEGACU_INVALID_ARGUMENT, 21, "out and indices must be aligned to their element");
+  }
+  if (driver.launch.stream == nullptr) return ok_status();
+  int const device = driver.launch.device_ordinal;
+  device_guard const guard(device);
+  if (guard.status() != cudaSuccess) return cuda_fail(guard.status(), 10);
+  int sms = 0;
+  cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (e != cudaSuccess) return cuda_fail(e, 10);
+
+  bool const nv = p.format == MEGACU_FP4_NV;
+  std::int64_t const b_rows = std::max(p.experts, 1) * p.n;
+  std::uint32_t const b_box = swiglu ? 128 : static_cast<std::uint32_t>(plan.tile_n);
+  CUtensorMap maps[4];
+  if (!encode_fp4_map(&maps[0], op.a, p.m, p.k, kFp4BlockM) ||
+      !encode_fp4_map(&maps[1], op.a, p.m, p.k, kFp4SmallRows) ||
+      !encode_fp4_map(&maps[2], op.b, b_rows, p.k, b_box) ||
+      !encode_fp4_map(&maps[3], swiglu ? op.b2 : op.b, b_rows, p.k, b_box)) {
+    return fail(MEGACU_BACKEND_ERROR, 30, "cuTensorMapEncodeTiled failed");
+  }
+  fp4_gemm_params prm{};
+  prm.n = static_cast<std::int32_t>(p.n);
+  prm.k = static_cast<std::int32_t>(p.k);
+  prm.m_tiles = static_cast<std::int32_t>(plan.m_tiles);
+  prm.n_tiles = static_cast<std::int32_t>(plan.n_tiles);
+  prm.n_row_tiles = static_cast<std::int32_t>(ceil_div(p.n, kScaleTileRows));
+  prm.rows = static_cast<std::int32_t>(p.m);
+  prm.group_m = 16;
+  prm.experts = p.experts;
+  prm.split = plan.split;
+  prm.scale_tiles = static_cast<std::int32_t>(scale_tiles(p.k, nv));
+  prm.out_dtype = p.out_dtype;
+  prm.out_stride = p.out_stride != 0 ? p.out_stride : p.n;
+  prm.vec_store = aligned_to(out, 16) && prm.out_stride * element_size(p.out_dtype) % 16 == 0;
+  prm.alpha = p.alpha;
+  prm.alphas = static_cast<float const *>(alphas);
+  prm.offsets = static_cast<std::int32_t const *>(offsets);
+  prm.counts = static_cast<std::int32_t const *>(counts);
+  prm.a_scales = static_cast<std::uint8_t const *>(op.a_scales);
+  prm.b_scales = static_cast<std::uint8_t const *>(op.b_scales);
+  prm.b2_scales = static_cast<std::uint8_t const *>(op.b2_scales);
+  prm.out = out;
+  prm.events = static_cast<std::uint32_t *>(events);
+  prm.timeout_ns = p.timeout_ns != 0 ? p.timeout_ns : 4000000000ull;
+  std::int64_t const tiles = plan.m_tiles * plan.n_tiles;
+  int const grid = static_cast<int>(plan.split > 1 ? tiles * plan.split
+                                                   : std::min<std::int64_t>(tiles, sms));
+  auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
+  if (swiglu) {
+    e = nv ? launch_gemm<true, true, 256>(device, grid, stream, maps, prm)
+           : launch_gemm<false, true, 256>(device, grid, stream, maps, prm);
+  } else if (plan.tile_n == 256) {
+    e = nv ? launch_gemm<true, false, 256>(device, grid, stream, maps, prm)
+           : launch_gemm<false, false, 256>(device, grid, stream, maps, prm);
+  } else {
+    e = nv ? launch_gemm<true, false, 128>(device, grid, stream, maps, prm)
+           : launch_gemm<false, false, 128>(device, grid, stream, maps, prm);
+  }
+  return e == cudaSuccess ? ok_status() : cuda_fail(e, 14);
+}
+
+}  // namespace
+
+extern "C" megacu_status megacu_b200_fp4_sizes(megacu_fp4_matrix const *matrix,
+                                               std::int64_t sizes[2]) {
+  int log2_scale = 0;
+  megacu_status const st = check_matrix(matrix, log2_scale);
+  if (st.code != MEGACU_OK) return st;
+  if (sizes == nullptr) return fail(MEGACU_INVALID_ARGUMENT, 2, "missing output");
+  sizes[0] = matrix->rows * (matrix->cols / 2);
+  sizes[1] = ceil_div(matrix->rows, kScaleTileRows) *
+             scale_tiles(matrix->cols, matrix->format == MEGACU_FP4_NV) * kScaleTileBytes;
+  return ok_status();
+}
+
+extern "C" megacu_status megacu_b200_fp4_events_bytes(std::int64_t *bytes) {
+  if (bytes == nullptr) return fail(MEGACU_INVALID_ARGUMENT, 2, "missing output");
+  *bytes = kControlBytes;
+  return ok_status();
+}
+
+extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, void const *x,
+                                                  void const *slot_of_row, void *data,
+                                                  void *scales,
+                                                  megacu_fp4_matrix const *matrix) {
+  int log2_scale = 0;
+  megacu_status const st = check_matrix(matrix, log2_scale);
+  if (st.code != MEGACU_OK) return st;
+  megacu_fp4_matrix const &m = *matrix;
+  bool const transpose = m.transpose != 0;
+  if (m.stride != 0 && m.stride < (transpose ? m.rows : m.cols)) {
+    return fail(MEGACU_INVALID_ARGUMENT, 1, "stride is smaller than a row");
+  }
+  if (transpose && (slot_of_row != nullptr || m.topk > 0)) {
+    return fail(MEGACU_UNSUPPORTED, 22, "a transposed matrix is quantised whole");
+  }
+  if (m.topk > 0 && slot_of_row == nullptr) {
+    return fail(MEGACU_INVALID_ARGUMENT, 2, "gathered rows need slot_of_row");
+  }
+  if (m.rows == 0) return ok_status();
+  if (x == nullptr || data == nullptr || scales == nullptr) {
+    return fail(MEGACU_INVALID_ARGUMENT, 2, "missing storage");
+  }
+  int const size = element_size(m.dtype);
+  if (!aligned_to(data, 16) || !aligned_to(scales, 16) || !aligned_to(x, size) ||
+      !aligned_to(slot_of_row, 4)) {
+    return fail(MEGACU_INVALID_ARGUMENT, 21,
+                "data and scales must be 16-byte aligned, x to its element");
+  }
+  if (driver.launch.stream == nullptr) return ok_status();
+  device_guard const guard(driver.launch.device_ordinal);
+  if (guard.status() != cudaSuccess) return cuda_fail(guard.status(), 10);
+  fp4_matrix_params prm = matrix_params(m, log2_scale, data, scales, transpose);
+  prm.slot_of_row = static_cast<std::int32_t const *>(slot_of_row);
+  auto const grid =
+      static_cast<unsigned>(ceil_div(m.rows, kScaleTileRows) * prm.col_tiles);
+  auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
+  by_type(m.dtype, m.format, [&](auto value, auto nv) {
+    using T = decltype(value);
+    auto const *src = static_cast<T const *>(x);
+    constexpr bool kNv = decltype(nv)::value;
+    if (transpose) {
+      // Pairs of columns are read together when every row starts on a pair.
+      if (m.rows % 2 == 0 && prm.stride % 2 == 0 && aligned_to(x, 2 * size)) {
+        fp4_quantize_t_kernel<T, kNv, true><<<grid, kQuantTThreads, 0, stream>>>(prm, src);
+      } else {
+        fp4_quantize_t_kernel<T, kNv, false><<<grid, kQuantTThreads, 0, stream>>>(prm, src);
+      }
+    } else if (prm.stride * size % 16 == 0 && aligned_to(x, 16)) {
+      fp4_quantize_kernel<T, kNv, true><<<grid, kQuantThreads, 0, stream>>>(prm, src);
+    } else {
+      fp4_quantize_kernel<T, kNv, false><<<grid, kQuantThreads, 0, stream>>>(prm, src);
+    }
+  });
+  cudaError_t const e = cudaGetLastError();
+  return e == cudaSuccess ? ok_status() : cuda_fail(e, 14);
+}
+
+extern "C" megacu_status megacu_cuda_fp4_dequantize(megacu_driver_view driver, void const *data,
+                                                    void const *scales, void *out,
+                                                    megacu_fp4_matrix const *matrix) {
+  int log2_scale = 0;
+  megacu_status const st = check_matrix(matrix, log2_scale);
+  if (st.code != MEGACU_OK) return st;
+  megacu_fp4_matrix const &m = *matrix;
+  if (m.transpose != 0 || m.topk != 0) {
+    return fail(MEGACU_UNSUPPORTED, 22, "values come back row by row as quantised");
+  }
+  if (m.stride != 0 && m.stride < m.cols) {
+    return fail(MEGACU_INVALID_ARGUMENT, 1, "stride is smaller than a row");
+  }
+  if (m.rows == 0) return ok_status();
+  if (data == nullptr || scales == nullptr || out == nullptr) {
+    return fail(MEGACU_INVALID_ARGUMENT, 2, "missing storage");
+  }
+  int const size = element_size(m.dtype);
+  if (!aligned_to(data, 16) || !aligned_to(scales, 16) || !aligned_to(out, size)) {
+    return fail(MEGACU_INVALID_ARGUMENT, 21,
+                "data and scales must be 16-byte aligned, out to its element");
+  }
+  if (driver.launch.stream == nullptr) return ok_status();
+  device_guard const guard(driver.launch.device_ordinal);
+  if (guard.status() != cudaSuccess) return cuda_fail(guard.status(), 10);
+  fp4_matrix_params const prm =
+      matrix_params(m, log2_scale, const_cast<void *>(data), const_cast<void *>(scales), false);
+  auto const grid = static_cast<unsigned>(
+      std::min<std::int64_t>(ceil_div(m.rows * (m.cols / 16), kQuantThreads), 1 << 20));
+  auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
+  bool const vec = prm.stride * size % 16 == 0 && aligned_to(out, 16);
+  by_type(m.dtype, m.format, [&](auto value, auto nv) {
+    using T = decltype(value);
+    constexpr bool kNv = decltype(nv)::value;
+    if (vec) {
+      fp4_dequantize_kernel<T, kNv, true><<<grid, kQuantThreads, 0, stream>>>(
+          prm, static_cast<T *>(out));
+    } else {
+      fp4_dequantize_kernel<T, kNv, false><<<grid, kQuantThreads, 0, stream>>>(
+          prm, static_cast<T *>(out));
+    }
+  });
+  cudaError_t const e = cudaGetLastError();
+  return e == cudaSuccess ? ok_status() : cuda_fail(e, 14);
+}
+
+extern "C" megacu_status megacu_cuda_fp4_gemm(megacu_driver_view driver, void const *a,
+                                              void const *a_scales, void const *b,
+                                              void const *b_scales, void const *offsets,
+                                              void const *counts, void const *alphas, void *out,
+                                              void *events,
+                                              megacu_fp4_gemm_problem const *problem) {
+  return run_product(driver, {a, a_scales, b, b_scales, nullptr, nullptr}, offsets, counts, alphas,
+                     out, events, problem, false);
+}
+
+extern "C" megacu_status megacu_cuda_fp4_gemm_swiglu(
+    megacu_driver_view driver, void const *a, void const *a_scales, void const *gate,
+    void const *gate_scales, void const *up, void const *up_scales, void const *offsets,
+    void const *counts, void const *alphas, void *act, void *events,
+    megacu_fp4_gemm_problem const *problem) {
+  return run_product(driver, {a, a_scales, gate, gate_scales, up, up_scales}, offsets, counts,
+                     alphas, act, events, problem, true);
+}

@@ -1,0 +1,298 @@
+// Routing of tokens to experts: a stable counting sort of the (token, choice)
+// slots by expert, and the rows' way to the experts and back.
+//
+//   sort      row_of_slot[s] = offsets[e(s)] + #{s' < s : e(s') = e(s)}
+//   dispatch  rows[row_of_slot[t, j]] = x[t]
+//   combine   y[t] = sum_j w[t, j] rows[row_of_slot[t, j]]
+//   gradient  drows[row_of_slot[t, j]] = w[t, j] dy[t],
+//             dw[t, j] = <dy[t], rows[row_of_slot[t, j]]>
+// The gradient of dispatch is combine without weights.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "vec.cuh"
+
+namespace megacu_b200 {
+
+inline constexpr int kMoeMaxExperts = 1024;
+inline constexpr int kMoeMaxTopk = 32;
+inline constexpr int kMoeSortThreads = 1024;
+inline constexpr int kMoeSortWarps = kMoeSortThreads / 32;
+
+struct moe_sort_params {
+  void const *ids;
+  std::int64_t slots;
+  std::int64_t rows;       // capacity of slot_of_row
+  std::int32_t chunk;      // slots per CTA
+  std::int32_t experts;
+  std::int32_t first;
+  std::int32_t align;
+  std::int32_t *histogram;  // [CTAs][experts], unused with one CTA
+  std::int32_t *counts;
+  std::int32_t *offsets;
+  std::int32_t *row_of_slot;
+  std::int32_t *slot_of_row;
+};
+
+// The slot's expert here, or -1.
+template <class Id>
+__device__ __forceinline__ std::int32_t local_expert(moe_sort_params const &p, std::int64_t slot) {
+  std::int64_t const e = static_cast<std::int64_t>(static_cast<Id const *>(p.ids)[slot]) - p.first;
+  return e >= 0 && e < p.experts ? static_cast<std::int32_t>(e) : -1;
+}
+
+// Histogram of one chunk of slots per CTA.
+template <class Id>
+__global__ void __launch_bounds__(kMoeSortThreads) moe_count_kernel(moe_sort_params p) {
+  extern __shared__ std::int32_t moe_smem[];
+  asm volatile("griddepcontrol.launch_dependents;");
+  for (int e = threadIdx.x; e < p.experts; e += kMoeSortThreads) moe_smem[e] = 0;
+  __syncthreads();
+  std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
+  std::int64_t const end = min(begin + p.chunk, p.slots);
+  for (std::int64_t s = begin + threadIdx.x; s < end; s += kMoeSortThreads) {
+    std::int32_t const e = local_expert<Id>(p, s);
+    if (e >= 0) atomicAdd(&moe_smem[e], 1);
+  }
+  __syncthreads();
+  std::int32_t *const mine = p.histogram + static_cast<std::int64_t>(blockIdx.x) * p.experts;
+  for (int e = threadIdx.x; e < p.experts; e += kMoeSortThreads) mine[e] = moe_smem[e];
+}
+
+// Places one chunk of slots per CTA. Every warp owns a contiguous part of the
+// chunk, so that the order within an expert is the slots' order: the warp's
+// first row of each expert is the expert's start, plus what earlier chunks
+// and earlier warps hold of it; within 32 slots, lanes of one expert rank
+// themselves by a warp match. No counter is kept between calls and nothing
+// depends on the order of atomics.
+template <class Id>
+__global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_params p) {
+  extern __shared__ std::int32_t moe_smem[];
+  __shared__ std::int32_t warp_sums[kMoeSortWarps];
+  int const experts = p.experts;
+  std::int32_t *const cursor = moe_smem;                           // [warps][experts]
+  std::int32_t *const total = moe_smem + kMoeSortWarps * experts;  // [experts]
+  std::int32_t *const start = total + experts;                     // [experts]
+  int const tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+
+  for (int i = tid; i < (kMoeSortWarps + 2) * experts; i += kMoeSortThreads) moe_smem[i] = 0;
+  __syncthreads();
+  std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
+  std::int64_t const end = min(begin + p.chunk, p.slots);
+  std::int32_t const part = (p.chunk + kMoeSortThreads - 1) / kMoeSortThreads * 32;
+  std::int64_t const w0 = min(begin + static_cast<std::int64_t>(warp) * part, end);
+  std::int64_t const w1 = min(w0 + part, end);
+  std::int32_t *const mine = cursor + warp * experts;
+  for (std::int64_t s = w0 + lane; s < w1; s += 32) {
+    std::int32_t const e = local_expert<Id>(p, s);
+    if (e >= 0) atomicAdd(&mine[e], 1);
+  }
+  // The histograms of every chunk are complete past this point.
+  if (gridDim.x > 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+  __syncthreads();
+
+  // total[e] = slots of e anywhere, start[e] = slots of e in earlier chunks.
+  if (gridDim.x > 1) {
+    int const lanes = kMoeSortThreads / experts;  // threads that share an expert's column
+    if (tid < lanes * experts) {
+      int const e = tid % experts, first = tid / experts;
+      std::int32_t all = 0, before = 0;
+      for (int c = first; c < static_cast<int>(gridDim.x); c += lanes) {
+        std::int32_t const n = p.histogram[static_cast<std::int64_t>(c) * experts + e];
+        all += n;
+        before += c < static_cast<int>(blockIdx.x) ? n : 0;
+      }
+      if (all) atomicAdd(&total[e], all);
+      if (before) atomicAdd(&start[e], before);
+    }
+  } else {
+    for (int e = tid; e < experts; e += kMoeSortThreads) {
+      std::int32_t all = 0;
+#pragma unroll 8
+      for (int w = 0; w < kMoeSortWarps; ++w) all += cursor[w * experts + e];
+      total[e] = all;
+    }
+  }
+  __syncthreads();
+
+  // Exclusive scan of the padded counts (one thread per expert).
+  std::int32_t const count = tid < experts ? total[tid] : 0;
+  std::int32_t const before = tid < experts ? start[tid] : 0;
+  std::int32_t const padded = (count + p.align - 1) / p.align * p.align;
+  std::int32_t sum = padded;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    std::int32_t const up = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += up;
+  }
+  if (lane == 31) warp_sums[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    std::int32_t v = warp_sums[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      std::int32_t const up = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += up;
+    }
+    warp_sums[lane] = v;
+  }
+  __syncthreads();
+  std::int32_t const offset = sum - padded + (warp > 0 ? warp_sums[warp - 1] : 0);
+  std::int32_t const used = warp_sums[kMoeSortWarps - 1];
+  if (tid < experts) {
+    std::int32_t next = offset + before;
+#pragma unroll 8
+    for (int w = 0; w < kMoeSortWarps; ++w) {
+      std::int32_t const n = cursor[w * experts + tid];
+      cursor[w * experts + tid] = next;
+      next += n;
+    }
+    if (blockIdx.x == 0) {
+      p.counts[tid] = count;
+      p.offsets[tid] = offset;
+      if (tid == experts - 1) p.offsets[experts] = used;
+    }
+    // Padding rows of the experts of this CTA's share.
+    if (tid % gridDim.x == blockIdx.x) {
+      for (std::int32_t r = offset + count; r < offset + padded; ++r) p.slot_of_row[r] = -1;
+    }
+  }
+  for (std::int64_t r = used + static_cast<std::int64_t>(blockIdx.x) * kMoeSortThreads + tid;
+       r < p.rows; r += static_cast<std::int64_t>(gridDim.x) * kMoeSortThreads) {
+    p.slot_of_row[r] = -1;
+  }
+  __syncthreads();
+
+  for (std::int64_t s0 = w0; s0 < w1; s0 += 32) {
+    std::int64_t const s = s0 + lane;
+    bool const in = s < w1;
+    std::int32_t const e = in ? local_expert<Id>(p, s) : -1;
+    std::uint32_t const same = __match_any_sync(0xffffffffu, e);
+    std::int32_t row = -1;
+    if (e >= 0) row = mine[e] + __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+    if (in) p.row_of_slot[s] = row;
+    if (row >= 0) p.slot_of_row[row] = static_cast<std::int32_t>(s);
+  }
+}
+
+struct moe_rows_params {
+  std::int64_t tokens;
+  std::int32_t hidden;
+  std::int32_t topk;
+  std::int64_t token_stride;  // elements between rows of x, y and dy
+  std::int64_t row_stride;    // elements between rows of rows and drows
+  std::int32_t const *row_of_slot;
+};
+
+inline constexpr int kMoeGroup = 8;  // choices whose rows are in flight together
+
+// One CTA per token reads its row once and writes it once per choice.
+template <class T, int N>
+__global__ void moe_dispatch_kernel(moe_rows_params p, T const *x, T *rows) {
+  std::int64_t const t = blockIdx.x;
+  std::int32_t const *const at = p.row_of_slot + t * p.topk;
+  T const *const src = x + t * p.token_stride;
+  for (int c = threadIdx.x * N; c < p.hidden; c += blockDim.x * N) {
+    vec<T, N> const v = load_vec<T, N>(src + c);
+    for (int j = 0; j < p.topk; ++j) {
+      std::int32_t const r = at[j];
+      if (r >= 0) store_vec<T, N>(rows + r * p.row_stride + c, v);
+    }
+  }
+}
+
+// One CTA per token; sums in 32 bits in the order of the choices, one
+// rounding. kMoeGroup rows' loads are in flight per thread.
+template <class T, int N>
+__global__ void moe_combine_kernel(moe_rows_params p, T const *rows, float const *weights, T *y) {
+  std::int64_t const t = blockIdx.x;
+  std::int32_t const *const at = p.row_of_slot + t * p.topk;
+  float const *const w = weights == nullptr ? nullptr : weights + t * p.topk;
+  for (int c = threadIdx.x * N; c < p.hidden; c += blockDim.x * N) {
+    float acc[N] = {};
+    for (int j0 = 0; j0 < p.topk; j0 += kMoeGroup) {
+      vec<T, N> v[kMoeGroup];
+      std::int32_t r[kMoeGroup];
+#pragma unroll
+      for (int j = 0; j < kMoeGroup; ++j) {
+        r[j] = j0 + j < p.topk ? at[j0 + j] : -1;
+        if (r[j] >= 0) v[j] = load_vec<T, N>(rows + r[j] * p.row_stride + c);
+      }
+#pragma unroll
+      for (int j = 0; j < kMoeGroup; ++j) {
+        if (r[j] < 0) continue;
+        float const f = w == nullptr ? 1.0f : w[j0 + j];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(f, v[j].f32(i), acc[i]);
+      }
+    }
+    vec<T, N> out;
+#pragma unroll
+    for (int i = 0; i < N; ++i) out.v[i] = from_f32<T>(acc[i]);
+    store_vec<T, N>(y + t * p.token_stride + c, out);
+  }
+}
+
+// One CTA per token: dy is read once per kMoeGroup choices (from L1 after the
+// first), each choice's row once; the dot products are summed in 32 bits per
+// thread, then over the warp, then over the warps in order.
+template <class T, int N>
+__global__ void moe_combine_grad_kernel(moe_rows_params p, T const *dy, T const *rows,
+                                        float const *weights, T *drows, float *dweights) {
+  __shared__ float partial[32][kMoeGroup];
+  std::int64_t const t = blockIdx.x;
+  std::int32_t const *const at = p.row_of_slot + t * p.topk;
+  float const *const w = weights + t * p.topk;
+  T const *const g = dy + t * p.token_stride;
+  int const warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int j0 = 0; j0 < p.topk; j0 += kMoeGroup) {
+    std::int32_t r[kMoeGroup];
+    float f[kMoeGroup], dot[kMoeGroup];
+#pragma unroll
+    for (int j = 0; j < kMoeGroup; ++j) {
+      r[j] = j0 + j < p.topk ? at[j0 + j] : -1;
+      f[j] = r[j] >= 0 ? w[j0 + j] : 0.0f;
+      dot[j] = 0.0f;
+    }
+    for (int c = threadIdx.x * N; c < p.hidden; c += blockDim.x * N) {
+      vec<T, N> const d = *reinterpret_cast<vec<T, N> const *>(g + c);
+      vec<T, N> v[kMoeGroup];
+#pragma unroll
+      for (int j = 0; j < kMoeGroup; ++j) {
+        if (r[j] >= 0) v[j] = load_vec<T, N>(rows + r[j] * p.row_stride + c);
+      }
+#pragma unroll
+      for (int j = 0; j < kMoeGroup; ++j) {
+        if (r[j] < 0) continue;
+        vec<T, N> out;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          dot[j] = fmaf(d.f32(i), v[j].f32(i), dot[j]);
+          out.v[i] = from_f32<T>(f[j] * d.f32(i));
+        }
+        store_vec<T, N>(drows + r[j] * p.row_stride + c, out);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kMoeGroup; ++j) {
+#pragma unroll
+      for (int m = 16; m > 0; m /= 2) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], m);
+      if (lane == 0) partial[warp][j] = dot[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < kMoeGroup && j0 + static_cast<int>(threadIdx.x) < p.topk) {
+      float sum = 0.0f;
+      for (int i = 0; i < static_cast<int>(blockDim.x) / 32; ++i) sum += partial[i][threadIdx.x];
+      dweights[t * p.topk + j0 + threadIdx.x] = sum;
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace megacu_b200
