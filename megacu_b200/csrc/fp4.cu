@@ -107,9 +107,24 @@ bool encode_fp4_map(CUtensorMap *map, void const *base, std::int64_t rows, std::
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Scale tiles, 512 bytes each, in boxes of `box` consecutive ones.
+bool encode_scale_map(CUtensorMap *map, void const *base, std::int64_t tiles, std::uint32_t box) {
+  auto const encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  cuuint64_t const dims[2] = {kScaleTileBytes / 4, static_cast<cuuint64_t>(tiles)};
+  cuuint64_t const strides[1] = {kScaleTileBytes};
+  cuuint32_t const boxes[2] = {kScaleTileBytes / 4, box};
+  cuuint32_t const elem[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides,
+                boxes, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct fp4_plan {
   int tile_n = 256;  // accumulator columns of a tile
   int split = 1;
+  bool pair = false;
   std::int64_t m_tiles = 0, n_tiles = 0;
 };
 
@@ -132,10 +147,11 @@ megacu_status make_plan(megacu_fp4_gemm_problem const &p, bool swiglu, int sms, 
       std::int64_t const cost = waves * per_tile;
       if (best < 0 || cost < best) {
         best = cost;
-        out = {tile_n, split, m_tiles, n_tiles};
+        out = {tile_n, split, false, m_tiles, n_tiles};
       }
     }
   }
+  out.pair = p.experts == 0 && out.tile_n == 256 && out.split == 1 && out.m_tiles > 1;
   if (best < 0) return fail(MEGACU_UNSUPPORTED, 22, "tile_n or split not possible");
   if (out.m_tiles * out.n_tiles * out.split > (1 << 28)) {
     return fail(MEGACU_UNSUPPORTED, 22, "too many tiles");
@@ -147,11 +163,11 @@ struct fp4_operands {
   void const *a, *a_scales, *b, *b_scales, *b2, *b2_scales;
 };
 
-template <bool kNv, bool kSwiglu, int BN>
-cudaError_t launch_gemm(int device, int grid, cudaStream_t stream, CUtensorMap const (&maps)[4],
+template <bool kNv, bool kSwiglu, int BN, bool kPair>
+cudaError_t launch_gemm(int device, int grid, cudaStream_t stream, fp4_maps const &maps,
                         fp4_gemm_params const &prm) {
-  constexpr auto kKernel = &fp4_gemm_kernel<kNv, kSwiglu, BN>;
-  constexpr int kSmem = fp4_config<kNv, BN>::smem_bytes;
+  constexpr auto kKernel = &fp4_gemm_kernel<kNv, kSwiglu, BN, kPair>;
+  constexpr int kSmem = fp4_config<kNv, BN, kPair>::smem_bytes;
   static std::atomic<bool> configured[kMaxDevices] = {};
   bool const known = device >= 0 && device < kMaxDevices;
   if (!known || !configured[device].load(std::memory_order_acquire)) {
@@ -162,17 +178,45 @@ cudaError_t launch_gemm(int device, int grid, cudaStream_t stream, CUtensorMap c
   }
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
+  static std::atomic<int> max_pairs[kMaxDevices] = {};
+  int const cluster = kPair ? 2 : prm.split;
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(prm.split);
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kFp4Threads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = prm.split > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kKernel, maps[0], maps[1], maps[2], maps[3], prm);
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  if constexpr (kPair) {
+    // As many clusters as the device holds at once, each for several tiles.
+    int pairs = known ? max_pairs[device].load(std::memory_order_acquire) : 0;
+    if (pairs == 0) {
+      cfg.gridDim = dim3(2);
+      cudaError_t const e = cudaOccupancyMaxActiveClusters(&pairs, kKernel, &cfg);
+      if (e != cudaSuccess) return e;
+      if (pairs < 1) return cudaErrorInvalidConfiguration;
+      if (known) max_pairs[device].store(pairs, std::memory_order_release);
+    }
+    grid = std::min(grid, 2 * pairs);
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  return cudaLaunchKernelEx(&cfg, kKernel, maps, prm);
+}
+
+template <bool kNv>
+cudaError_t launch_plan(fp4_plan const &plan, bool swiglu, int device, int grid,
+                        cudaStream_t stream, fp4_maps const &maps, fp4_gemm_params const &prm) {
+  if (swiglu) {
+    return plan.pair ? launch_gemm<kNv, true, 256, true>(device, grid, stream, maps, prm)
+                     : launch_gemm<kNv, true, 256, false>(device, grid, stream, maps, prm);
+  }
+  if (plan.tile_n == 256) {
+    return plan.pair ? launch_gemm<kNv, false, 256, true>(device, grid, stream, maps, prm)
+                     : launch_gemm<kNv, false, 256, false>(device, grid, stream, maps, prm);
+  }
+  return launch_gemm<kNv, false, 128, false>(device, grid, stream, maps, prm);
 }
 
 megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &op,
@@ -232,12 +276,24 @@ megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &
 
   bool const nv = p.format == MEGACU_FP4_NV;
   std::int64_t const b_rows = std::max(p.experts, 1) * p.n;
-  std::uint32_t const b_box = swiglu ? 128 : static_cast<std::uint32_t>(plan.tile_n);
-  CUtensorMap maps[4];
-  if (!encode_fp4_map(&maps[0], op.a, p.m, p.k, kFp4BlockM) ||
-      !encode_fp4_map(&maps[1], op.a, p.m, p.k, kFp4SmallRows) ||
-      !encode_fp4_map(&maps[2], op.b, b_rows, p.k, b_box) ||
-      !encode_fp4_map(&maps[3], swiglu ? op.b2 : op.b, b_rows, p.k, b_box)) {
+  std::uint32_t const b_box = swiglu || plan.pair ? 128 : static_cast<std::uint32_t>(plan.tile_n);
+  std::int64_t const tiles_k = scale_tiles(p.k, nv);
+  std::int64_t const a_tiles = plan.m_tiles * tiles_k;
+  std::int64_t const b_tiles =
+      std::max(p.experts, 1) * ceil_div(p.n, kScaleTileRows) * tiles_k;
+  if (a_tiles > 0x7fffffffll || b_tiles > 0x7fffffffll) {
+    return fail(MEGACU_UNSUPPORTED, 22, "operand too large");
+  }
+  std::uint32_t const scale_box = kFp4BlockK / fp4_tile_cols(nv);
+  fp4_maps maps;
+  if (!encode_fp4_map(&maps.a, op.a, p.m, p.k, kFp4BlockM) ||
+      !encode_fp4_map(&maps.a_small, op.a, p.m, p.k, kFp4SmallRows) ||
+      !encode_fp4_map(&maps.b, op.b, b_rows, p.k, b_box) ||
+      !encode_fp4_map(&maps.b2, swiglu ? op.b2 : op.b, b_rows, p.k, b_box) ||
+      !encode_scale_map(&maps.a_scales, op.a_scales, a_tiles, scale_box) ||
+      !encode_scale_map(&maps.b_scales, op.b_scales, b_tiles, scale_box) ||
+      !encode_scale_map(&maps.b2_scales, swiglu ? op.b2_scales : op.b_scales, b_tiles,
+                        scale_box)) {
     return fail(MEGACU_BACKEND_ERROR, 30, "cuTensorMapEncodeTiled failed");
   }
   fp4_gemm_params prm{};
@@ -258,26 +314,18 @@ megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &
   prm.alphas = static_cast<float const *>(alphas);
   prm.offsets = static_cast<std::int32_t const *>(offsets);
   prm.counts = static_cast<std::int32_t const *>(counts);
-  prm.a_scales = static_cast<std::uint8_t const *>(op.a_scales);
-  prm.b_scales = static_cast<std::uint8_t const *>(op.b_scales);
-  prm.b2_scales = static_cast<std::uint8_t const *>(op.b2_scales);
   prm.out = out;
   prm.events = static_cast<std::uint32_t *>(events);
   prm.timeout_ns = p.timeout_ns != 0 ? p.timeout_ns : 4000000000ull;
+  // Persistent, one CTA per SM; a split's cluster computes one tile.
   std::int64_t const tiles = plan.m_tiles * plan.n_tiles;
-  int const grid = static_cast<int>(plan.split > 1 ? tiles * plan.split
-                                                   : std::min<std::int64_t>(tiles, sms));
+  std::int64_t const pairs = (plan.m_tiles + 1) / 2 * plan.n_tiles;
+  std::int64_t const grid = plan.pair        ? 2 * std::min<std::int64_t>(pairs, sms / 2)
+                            : plan.split > 1 ? tiles * plan.split
+                                             : std::min<std::int64_t>(tiles, sms);
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
-  if (swiglu) {
-    e = nv ? launch_gemm<true, true, 256>(device, grid, stream, maps, prm)
-           : launch_gemm<false, true, 256>(device, grid, stream, maps, prm);
-  } else if (plan.tile_n == 256) {
-    e = nv ? launch_gemm<true, false, 256>(device, grid, stream, maps, prm)
-           : launch_gemm<false, false, 256>(device, grid, stream, maps, prm);
-  } else {
-    e = nv ? launch_gemm<true, false, 128>(device, grid, stream, maps, prm)
-           : launch_gemm<false, false, 128>(device, grid, stream, maps, prm);
-  }
+  e = nv ? launch_plan<true>(plan, swiglu, device, static_cast<int>(grid), stream, maps, prm)
+         : launch_plan<false>(plan, swiglu, device, static_cast<int>(grid), stream, maps, prm);
   return e == cudaSuccess ? ok_status() : cuda_fail(e, 14);
 }
 

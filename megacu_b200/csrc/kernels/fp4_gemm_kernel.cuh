@@ -4,18 +4,26 @@
 // also by expert (each 128-row tile of A against its expert's B).
 //
 // tcgen05.mma block-scaled kinds: mxf4 (blocks of 32, ue8m0) and mxf4nvf4
-// (blocks of 16, e4m3), K = 64 per instruction, fp32 accumulators in TMEM. One
-// MMA covers 128 rows of A and BN rows of B.
+// (blocks of 16, e4m3), K = 64 per instruction, fp32 accumulators in TMEM.
 //
-//   warp 0     TMA producer: 128 rows x 256 elements of A, BN rows of B
-//              (128-byte swizzle) and their scale tiles per stage
+//   warp 0     TMA producer: 128 rows x 256 elements of A, the tile's rows of B
+//              (128-byte swizzle) and their scale tiles per stage; the first
+//              tile's first stages are issued before the CTA's set-up ends
 //   warp 1     TMEM allocation, scale copies shared -> TMEM, MMA issue
-//   warps 2-5  epilogue: accumulators -> alpha / SwiGLU -> out type -> memory
+//   warps 2-9  epilogue: accumulators -> alpha / SwiGLU -> out type -> memory;
+//              two warps per 32 rows take alternate chunks of 32 columns
 //
 // TMEM holds two accumulators and the scales of a stage. With BN = 256 the two
 // accumulators share 64 columns (0..255 and 192..447, scales from 448): the
 // epilogue drains the shared columns first and then lets the next tile's MMAs
 // start, so a tile's epilogue overlaps the next tile's MMAs.
+//
+// kPair: a 2-CTA cluster computes 256 x 256 tiles with cta_group::2 MMAs. Each
+// CTA stages its own 128 rows of A and half of B (SwiGLU: gate and up), so an
+// SM moves 35 KB per 256 of K instead of 51, and holds its rows' accumulators
+// and every B row's scales. One CTA alone is bound by shared memory: its loads
+// and its MMAs' operand reads together exceed what the SM moves in the time of
+// the MMAs.
 //
 // A few rows (decode): bound by the weights' stream, so the tile's K is split
 // over the CTAs of a cluster (params.split) to occupy every SM; each CTA then
@@ -30,6 +38,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "fp4_format.cuh"
 #include "layout.h"
@@ -38,11 +47,18 @@
 
 namespace megacu_b200 {
 
-inline constexpr int kFp4Threads = 192;
+inline constexpr int kFp4EpilogueWarps = 8;
+inline constexpr int kFp4Threads = 64 + 32 * kFp4EpilogueWarps;
 inline constexpr int kFp4BlockM = 128;
 inline constexpr int kFp4BlockK = 256;  // elements per stage: one 128-byte swizzled row
 inline constexpr int kFp4SmallRows = 32;  // rows of the smaller A box
-inline constexpr int kFp4MaxSplit = 8;
+// Bound of the waits that only let copies and MMAs in flight end after an error.
+inline constexpr unsigned long long kFp4DrainNs = 10000000ull;
+
+// b2, b2_scales: SwiGLU's up; a_small: A in boxes of kFp4SmallRows rows.
+struct fp4_maps {
+  CUtensorMap a, a_small, b, b2, a_scales, b_scales, b2_scales;
+};
 
 struct fp4_gemm_params {
   std::int32_t n, k;
@@ -61,72 +77,98 @@ struct fp4_gemm_params {
   float const *alphas;            // per expert, or nullptr
   std::int32_t const *offsets;    // [experts + 1], multiples of 128
   std::int32_t const *counts;     // [experts]
-  std::uint8_t const *a_scales;
-  std::uint8_t const *b_scales;
-  std::uint8_t const *b2_scales;  // SwiGLU: up
   void *out;
   std::uint32_t *events;
   unsigned long long timeout_ns;
 };
 
-template <bool kNv, int BN>
+template <bool kNv, int BN, bool kPair>
 struct fp4_config {
   static constexpr int scale_tiles = kFp4BlockK / fp4_tile_cols(kNv);  // per row tile and stage
+  static constexpr int b_tiles = BN / 128;  // row tiles of B whose scales a CTA holds
   static constexpr int a_bytes = kFp4BlockM * 128;
-  static constexpr int b_bytes = BN * 128;
+  static constexpr int b_bytes = BN * 128 / (kPair ? 2 : 1);
   static constexpr int sfa_bytes = scale_tiles * kScaleTileBytes;
-  static constexpr int sfb_bytes = BN / 128 * sfa_bytes;
+  static constexpr int sfb_bytes = b_tiles * sfa_bytes;
   static constexpr int stage_bytes = a_bytes + b_bytes + sfa_bytes + sfb_bytes;
-  static constexpr int stages = BN == 256 ? 4 : 6;
+  static constexpr int staging_bytes = kFp4EpilogueWarps * 1024;
+  static constexpr int overhead = 1024 + staging_bytes + 256;
+  static constexpr int stages = (232448 - overhead) / stage_bytes;
   static constexpr int ring_bytes = stages * stage_bytes;
-  static constexpr int staging_bytes = 4 * 2048;  // 2 KB per epilogue warp
-  static constexpr int smem_bytes = 1024 + ring_bytes + staging_bytes + 256;
+  static constexpr int smem_bytes = overhead + ring_bytes;
   static constexpr int acc1 = BN == 256 ? 192 : BN;  // columns of the second accumulator
   static constexpr int sf_column = acc1 + BN;
   static constexpr int tmem_columns = 512;
-  static_assert(smem_bytes <= 232448, "dynamic shared memory per CTA");
-  static_assert(sf_column + scale_tiles * 4 * (1 + BN / 128) <= tmem_columns, "TMEM");
+  static_assert(stages >= 4 && stages <= 8, "stage ring");
+  static_assert(sf_column + scale_tiles * 4 * (1 + b_tiles) <= tmem_columns, "TMEM");
   static_assert(BN * 128 * 4 <= ring_bytes, "the split's exchange fits the ring");
 };
 
 namespace ptx {
 
+// One lane of a converged warp. The tensor core's instructions take uniform
+// registers; in a branch on this predicate the compiler knows that one lane
+// runs and keeps the operands there. In a branch on `lane == 0` it moves each
+// into place first: 170 cycles per MMA and 62 per scale copy at issue, against
+// MMAs of 128 cycles (measured; 4096 x 8192 x 8192 MX: 156 -> 105 us).
+__device__ __forceinline__ bool elect_one() {
+  std::uint32_t elected;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
+               "selp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(elected));
+  return elected != 0;
+}
+
 // D (+)= A * B with block scales from TMEM.
-template <bool kNv>
+template <bool kNv, bool kPair>
 __device__ __forceinline__ void umma_fp4(std::uint32_t d, std::uint64_t a, std::uint64_t b,
                                          std::uint32_t idesc, std::uint32_t sfa,
                                          std::uint32_t sfb, std::uint32_t accumulate) {
-  if constexpr (kNv) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X "
-        "[%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
+#define MEGACU_FP4_MMA(group, kind)                                              \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                  \
+               "tcgen05.mma.cta_group::" group ".kind::" kind                    \
+               " [%0], %1, %2, %3, [%4], [%5], p;\n\t}"                          \
+               :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) \
+               : "memory")
+  if constexpr (kNv && kPair) {
+    MEGACU_FP4_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+  } else if constexpr (kNv) {
+    MEGACU_FP4_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  } else if constexpr (kPair) {
+    MEGACU_FP4_MMA("2", "mxf4.block_scale.scale_vec::2X");
   } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X "
-        "[%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
+    MEGACU_FP4_MMA("1", "mxf4.block_scale.scale_vec::2X");
   }
+#undef MEGACU_FP4_MMA
 }
 
 // One scale tile (32 rows of 16 bytes in shared memory) into four TMEM
-// columns, repeated for the four groups of 32 lanes.
+// columns, repeated for the four groups of 32 lanes; with kPair in both CTAs,
+// each from its own shared memory.
+template <bool kPair>
 __device__ __forceinline__ void copy_scale_tile(std::uint32_t tmem, std::uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(desc)
-               : "memory");
+  if constexpr (kPair) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(desc)
+                 : "memory");
+  } else {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(desc)
+                 : "memory");
+  }
 }
 
-// Contiguous copy global -> shared; addresses and size multiples of 16.
-__device__ __forceinline__ void bulk_load(void *dst, void const *src, std::uint32_t bytes,
-                                          std::uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-      :: "r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar))
-      : "memory");
+// Arrives on `bar` (with kPair: on both CTAs' barrier at that place) when
+// every earlier copy and MMA of this thread has completed.
+template <bool kPair>
+__device__ __forceinline__ void commit_fp4(std::uint64_t *bar) {
+  if constexpr (kPair) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;"
+        :: "r"(smem_addr(bar)), "h"(static_cast<std::uint16_t>(3))
+        : "memory");
+  } else {
+    umma_commit(bar);
+  }
 }
 
 // Descriptor of a scale tile: no swizzle, 8-row groups 128 bytes apart.
@@ -215,60 +257,62 @@ __device__ __forceinline__ std::uint32_t pack16(std::int32_t dtype, float lo, fl
   return ptx::pack_bf16x2(lo, hi);
 }
 
-// Stores NC (16 or 32) consecutive columns from `col` of a warp's 32 rows:
-// lane = row on entry; through `stage` (2 KB) so that each row leaves as 16-byte
-// vectors of neighbouring lanes. `rows` rows exist.
-template <int NC>
+// Where a warp's 32 rows of a tile go.
+struct fp4_rows_out {
+  std::uint8_t *base;        // row 0, column 0
+  std::int64_t stride;       // bytes between rows
+  std::int32_t rows;         // rows that exist
+};
+
+// Stores kCount consecutive columns from `col` of a warp's 32 rows (lane = row
+// on entry), 32 bytes of each row at a time: turned through `stage` (1 KB, no
+// bank conflicts) so that two neighbouring lanes write a row's 32 bytes, or,
+// where the rows do not allow 16-byte stores, neighbouring lanes neighbouring
+// elements.
+template <bool kWide, int kCount>
 __device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uint8_t *stage,
-                                              float const (&v)[NC], std::int64_t row0,
-                                              std::int32_t rows, std::int32_t col) {
+                                              float const (&v)[kCount], fp4_rows_out const &out,
+                                              std::int32_t col) {
+  using element = std::conditional_t<kWide, std::uint32_t, std::uint16_t>;
+  constexpr int kSize = sizeof(element);
+  constexpr int kCols = 32 / kSize;
   std::uint32_t const lane = ptx::lane_id();
-  bool const wide = p.out_dtype == 3;
-  std::uint32_t const size = wide ? 4 : 2;
-  std::uint32_t const passes = wide && NC == 32 ? 2 : 1;
-  std::uint32_t const chunks = wide ? 4 : NC / 8;    // 16-byte vectors per row and pass
-  std::uint32_t const per_pass = chunks * 16 / size;  // columns per pass
+  auto slot = [stage](std::uint32_t r, std::uint32_t c) {
+    return stage + r * 32 + ((c ^ (r >> 2)) & 1u) * 16;
+  };
 #pragma unroll
-  for (std::uint32_t pass = 0; pass < 2; ++pass) {
-    if (pass >= passes) break;
+  for (int u = 0; u < kCount / kCols; ++u) {
+    std::int32_t const first = col + u * kCols;
+    if (first >= p.n) break;
 #pragma unroll
-    for (std::uint32_t c = 0; c < 4; ++c) {
-      if (c >= chunks) break;
+    for (int c = 0; c < 2; ++c) {
       uint4 q;
-      if (wide) {
-        std::uint32_t const i = (pass * 16 + c * 4) % NC;
-        q = make_uint4(__float_as_uint(v[i]), __float_as_uint(v[i + 1]),
-                       __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3]));
-      } else {
-        std::uint32_t const i = c * 8 % NC;
-        q = make_uint4(pack16(p.out_dtype, v[i], v[i + 1]), pack16(p.out_dtype, v[i + 2], v[i + 3]),
-                       pack16(p.out_dtype, v[i + 4], v[i + 5]),
-                       pack16(p.out_dtype, v[i + 6], v[i + 7]));
+      std::uint32_t *const w = &q.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int const e = u * kCols + c * (16 / kSize);
+        w[i] = kWide ? __float_as_uint(v[(e + i) % kCount])
+                     : pack16(p.out_dtype, v[(e + 2 * i) % kCount], v[(e + 2 * i + 1) % kCount]);
       }
-      *reinterpret_cast<uint4 *>(stage + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16) = q;
+      *reinterpret_cast<uint4 *>(slot(lane, c)) = q;
     }
     __syncwarp();
-    for (std::uint32_t i = lane; i < 32 * chunks; i += 32) {
-      std::uint32_t const r = i / chunks, c = i % chunks;
-      std::int32_t const first = col + static_cast<std::int32_t>(pass * per_pass + c * 16 / size);
-      if (static_cast<std::int32_t>(r) < rows && first < p.n) {
-        uint4 const q = *reinterpret_cast<uint4 const *>(stage + r * 64 + ((c ^ (r >> 1)) & 3) * 16);
-        std::uint8_t *const dst = static_cast<std::uint8_t *>(p.out) +
-                                  ((row0 + r) * p.out_stride + first) * size;
-        std::int32_t const left = p.n - first;
-        if (p.vec_store && left >= static_cast<std::int32_t>(16 / size)) {
-          *reinterpret_cast<uint4 *>(dst) = q;
-        } else {
-          std::uint32_t const w[4] = {q.x, q.y, q.z, q.w};
+    std::uint8_t *const dst = out.base + static_cast<std::int64_t>(first) * kSize;
+    if (p.vec_store && first + kCols <= p.n) {
 #pragma unroll
-          for (std::int32_t e = 0; e < 8; ++e) {
-            if (wide) {
-              if (e < 4 && e < left) reinterpret_cast<std::uint32_t *>(dst)[e] = w[e % 4];
-            } else if (e < left) {
-              reinterpret_cast<std::uint16_t *>(dst)[e] =
-                  static_cast<std::uint16_t>(w[e / 2] >> (16 * (e % 2)));
-            }
-          }
+      for (std::uint32_t r = lane / 2, h = 0; h < 2; ++h, r += 16) {
+        if (static_cast<std::int32_t>(r) < out.rows) {
+          *reinterpret_cast<uint4 *>(dst + r * out.stride + lane % 2 * 16) =
+              *reinterpret_cast<uint4 const *>(slot(r, lane % 2));
+        }
+      }
+    } else {
+      std::uint32_t const e = lane % kCols;
+      for (std::uint32_t r = lane / kCols; static_cast<std::int32_t>(r) < min(out.rows, 32);
+           r += 32 / kCols) {
+        if (first + static_cast<std::int32_t>(e) < p.n) {
+          *reinterpret_cast<element *>(dst + r * out.stride + e * kSize) =
+              *reinterpret_cast<element const *>(slot(r, e * kSize / 16) + e * kSize % 16);
         }
       }
     }
@@ -276,22 +320,37 @@ __device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uin
   }
 }
 
+template <int kCount>
+__device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uint8_t *stage,
+                                              float const (&v)[kCount], fp4_rows_out const &out,
+                                              std::int32_t col) {
+  if (p.out_dtype == 3) {
+    store_columns<true, kCount>(p, stage, v, out, col);
+  } else {
+    store_columns<false, kCount>(p, stage, v, out, col);
+  }
+}
+
+__device__ __forceinline__ fp4_rows_out rows_out(fp4_gemm_params const &p, std::int64_t row,
+                                                 std::int32_t rows) {
+  std::int64_t const stride = p.out_stride * (p.out_dtype == 3 ? 4 : 2);
+  return {static_cast<std::uint8_t *>(p.out) + row * stride, stride, rows};
+}
+
 __device__ __forceinline__ float swiglu(float g, float u) {
-  return g / (1.0f + __expf(-g)) * u;
+  return __fdividef(g, 1.0f + __expf(-g)) * u;
 }
 
 }  // namespace detail
 
-template <bool kNv, bool kSwiglu, int BN>
+template <bool kNv, bool kSwiglu, int BN, bool kPair>
 __global__ void __launch_bounds__(kFp4Threads, 1)
-    fp4_gemm_kernel(__grid_constant__ CUtensorMap const map_a,
-                    __grid_constant__ CUtensorMap const map_a_small,
-                    __grid_constant__ CUtensorMap const map_b,
-                    __grid_constant__ CUtensorMap const map_b2,
+    fp4_gemm_kernel(__grid_constant__ fp4_maps const maps,
                     __grid_constant__ fp4_gemm_params const p) {
-  using cfg = fp4_config<kNv, BN>;
+  using cfg = fp4_config<kNv, BN, kPair>;
   static_assert(!kSwiglu || BN == 256, "128 gate and 128 up columns");
-  constexpr int kStages = cfg::stages;
+  static_assert(!kPair || BN == 256, "pairs compute 256 x 256 tiles");
+  constexpr std::uint32_t kStages = cfg::stages;
   constexpr int kActCols = kSwiglu ? BN / 2 : BN;
   extern __shared__ std::uint8_t raw_smem[];
   std::uint8_t *const smem = reinterpret_cast<std::uint8_t *>(
@@ -307,103 +366,148 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   auto *const tmem_slot = reinterpret_cast<std::uint32_t *>(acc_free + 1);
   std::uint32_t *const abort_word = &reinterpret_cast<control_block *>(p.events)->error_code;
 
-  std::int32_t const warp = static_cast<std::int32_t>(threadIdx.x) / 32;
+  std::int32_t const warp =
+      __shfl_sync(0xffffffffu, static_cast<std::int32_t>(threadIdx.x) / 32, 0);
   std::uint32_t const lane = ptx::lane_id();
-  std::int32_t const split = p.split;
-  std::int32_t const rank = split > 1 ? static_cast<std::int32_t>(ptx::cluster_ctarank()) : 0;
-  std::int32_t const unit0 = static_cast<std::int32_t>(blockIdx.x) / split;
-  std::int32_t const units = static_cast<std::int32_t>(gridDim.x) / split;
+  // A cluster is a pair, or the CTAs that share a tile's K, or one CTA.
+  std::int32_t const split = kPair ? 1 : p.split;
+  std::int32_t const cluster = kPair ? 2 : split;
+  std::int32_t const rank =
+      cluster > 1 ? static_cast<std::int32_t>(ptx::cluster_ctarank()) : 0;
+  std::int32_t const unit0 = static_cast<std::int32_t>(blockIdx.x) / cluster;
+  std::int32_t const units = static_cast<std::int32_t>(gridDim.x) / cluster;
   std::int32_t const k_blocks = (p.k + kFp4BlockK - 1) / kFp4BlockK;
-  std::int32_t const kb0 = rank * k_blocks / split;
-  std::int32_t const kb1 = (rank + 1) * k_blocks / split;
+  std::int32_t const kb0 = kPair ? 0 : rank * k_blocks / split;
+  std::int32_t const kb1 = kPair ? k_blocks : (rank + 1) * k_blocks / split;
   std::int32_t const m_tiles =
       p.experts > 0 ? min(p.offsets[p.experts] / kFp4BlockM, p.m_tiles) : p.m_tiles;
-  std::int32_t const tiles = m_tiles * p.n_tiles;
+  // Rows of tiles as the raster counts them: pairs of 128-row tiles, or tiles.
+  std::int32_t const unit_rows = kPair ? (m_tiles + 1) / 2 : m_tiles;
+  std::int32_t const tiles = unit_rows * p.n_tiles;
+  bool const leader = !kPair || rank == 0;
+  // The 128-row tile of this CTA and the column tile of unit t.
+  auto locate = [&](std::int32_t t) {
+    fp4_tile c = fp4_locate(t, unit_rows, p.n_tiles, p.group_m);
+    if constexpr (kPair) c.row = 2 * c.row + rank;
+    return c;
+  };
 
-  if (threadIdx.x == 0) {
-    ptx::prefetch_tensor_map(&map_a);
-    ptx::prefetch_tensor_map(&map_a_small);
-    ptx::prefetch_tensor_map(&map_b);
-    if constexpr (kSwiglu) ptx::prefetch_tensor_map(&map_b2);
-    for (int s = 0; s < kStages; ++s) {
+  // Loads of the k-block `kb` of a tile into `stage` (one lane).
+  struct load_place {
+    std::int32_t row, a_tile, b_row, b_tile, boxes;
+  };
+  auto place = [&](std::int32_t t) {  // whole warp
+    fp4_tile const c = locate(t);
+    load_place l;
+    l.row = c.row * kFp4BlockM;
+    detail::fp4_rows const rows = detail::locate_rows(p, l.row);
+    l.boxes = min(max((rows.valid + kFp4SmallRows - 1) / kFp4SmallRows, 1), 4);
+    if constexpr (kPair) l.boxes = 4;  // both CTAs' bytes are counted by the leader
+    l.a_tile = min(c.row, m_tiles - 1) * p.scale_tiles;  // a pair's second tile may not exist
+    l.b_row = rows.expert * p.n + c.col * kActCols;
+    l.b_tile = (rows.expert * p.n_row_tiles + c.col * (kActCols / 128)) * p.scale_tiles;
+    return l;
+  };
+  auto load = [&](load_place const &l, std::int32_t kb, std::uint32_t stage) {
+    std::int32_t const st = kb * cfg::scale_tiles;
+    std::uint8_t *const sa = smem + stage * (cfg::a_bytes + cfg::b_bytes);
+    std::uint8_t *const sb = sa + cfg::a_bytes;
+    std::uint8_t *const sfa = scales + stage * (cfg::sfa_bytes + cfg::sfb_bytes);
+    std::uint8_t *const sfb = sfa + cfg::sfa_bytes;
+    std::uint32_t const bar = kPair ? ptx::map_to_rank(&full[stage], 0) : 0;
+    auto tma = [&](CUtensorMap const &map, void *dst, std::int32_t x, std::int32_t y) {
+      if constexpr (kPair) {
+        ptx::tma_load_2d_pair(&map, bar, dst, x, y);
+      } else {
+        ptx::tma_load_2d(&map, &full[stage], dst, x, y);
+      }
+    };
+    if (leader) {
+      std::uint32_t const mine = static_cast<std::uint32_t>(l.boxes) * kFp4SmallRows * 128 +
+                                 cfg::b_bytes + cfg::sfa_bytes + cfg::sfb_bytes;
+      ptx::mbar_arrive_expect_tx(&full[stage], mine * (kPair ? 2 : 1));
+    }
+    std::int32_t const x = kb * 128;
+    if (l.boxes == 4) {
+      tma(maps.a, sa, x, l.row);
+    } else {
+      for (std::int32_t i = 0; i < l.boxes; ++i) {
+        tma(maps.a_small, sa + i * kFp4SmallRows * 128, x, l.row + i * kFp4SmallRows);
+      }
+    }
+    if constexpr (kSwiglu) {
+      if constexpr (kPair) {  // the leader stages gate, the other CTA up
+        tma(leader ? maps.b : maps.b2, sb, x, l.b_row);
+      } else {
+        tma(maps.b, sb, x, l.b_row);
+        tma(maps.b2, sb + cfg::b_bytes / 2, x, l.b_row);
+      }
+    } else {
+      tma(maps.b, sb, x, l.b_row + (kPair ? rank * (BN / 2) : 0));
+    }
+    // Scale tiles: a box of a stage's tiles; past a row tile's last one it
+    // holds other tiles or zeros, which no MMA reads.
+    tma(maps.a_scales, sfa, 0, l.a_tile + st);
+    tma(maps.b_scales, sfb, 0, l.b_tile + st);
+    if constexpr (kSwiglu) {
+      tma(maps.b2_scales, sfb + cfg::sfa_bytes, 0, l.b_tile + st);
+    } else if constexpr (BN == 256) {
+      tma(maps.b_scales, sfb + cfg::sfa_bytes, 0, l.b_tile + p.scale_tiles + st);
+    }
+  };
+
+  std::uint32_t issued = 0;  // by the producer, in all
+  auto set_up_barriers = [&] {
+    for (std::uint32_t s = 0; s < kStages; ++s) {
       ptx::mbar_init(&full[s], 1);
       ptx::mbar_init(&empty[s], 1);
     }
     ptx::mbar_init(acc_full, 1);
-    ptx::mbar_init(acc_free, 4);
+    ptx::mbar_init(acc_free, kFp4EpilogueWarps * (kPair ? 2 : 1));
     ptx::fence_barrier_init();
     ptx::fence_proxy_async_shared();
-  }
-  if (warp == 1) {
-    ptx::tmem_alloc(tmem_slot, cfg::tmem_columns);
-    ptx::tmem_relinquish();
+  };
+  if (warp == 0) {
+    if (lane == 0) set_up_barriers();
+    __syncwarp();
+    if (!kPair && unit0 < tiles) {
+      load_place const l = place(unit0);
+      issued = static_cast<std::uint32_t>(min(kb1 - kb0, static_cast<std::int32_t>(kStages)));
+      if (lane == 0) {
+        for (std::uint32_t s = 0; s < issued; ++s) load(l, kb0 + static_cast<std::int32_t>(s), s);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1) {
+    if constexpr (kPair) {
+      ptx::tmem_alloc_pair(tmem_slot, cfg::tmem_columns);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, cfg::tmem_columns);
+      ptx::tmem_relinquish();
+    }
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
+  if constexpr (kPair) ptx::cluster_sync();  // both CTAs' barriers exist
   ptx::tc_fence_after_sync();
   std::uint32_t const tmem = *tmem_slot;
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    std::uint32_t stage = 0, phase = 0, issued = 0;
+    std::uint32_t stage = issued % kStages, phase = issued / kStages & 1u;
+    std::int32_t skip = static_cast<std::int32_t>(issued);  // loaded during the set-up
     bool ok = true;
     for (std::int32_t t = unit0; ok && t < tiles; t += units) {
-      fp4_tile const c = fp4_locate(t, m_tiles, p.n_tiles, p.group_m);
-      std::int32_t const row = c.row * kFp4BlockM;
-      detail::fp4_rows const rows = detail::locate_rows(p, row);
-      std::int32_t const boxes =
-          min(max((rows.valid + kFp4SmallRows - 1) / kFp4SmallRows, 1), 4);
-      std::int32_t const b_row = rows.expert * p.n + c.col * kActCols;
-      std::int32_t const b_tile = c.col * (kActCols / 128);
-      std::int32_t const b_tiles = kSwiglu ? 1 : min(BN / 128, p.n_row_tiles - b_tile);
-      std::int64_t const a_scale = static_cast<std::int64_t>(c.row) * p.scale_tiles;
-      std::int64_t const b_scale =
-          (static_cast<std::int64_t>(rows.expert) * p.n_row_tiles + b_tile) * p.scale_tiles;
-      for (std::int32_t kb = kb0; kb < kb1; ++kb) {
-        if (!ptx::mbar_wait(&empty[stage], phase ^ 1u, abort_word, p.timeout_ns)) {
+      load_place const l = place(t);
+      for (std::int32_t kb = kb0 + skip; kb < kb1; ++kb) {
+        if (!ptx::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_word, p.timeout_ns)) {
           if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 51);
           ok = false;
           break;
         }
-        if (lane == 0) {
-          std::int32_t const st0 = kb * cfg::scale_tiles;
-          std::uint32_t const sf_bytes = static_cast<std::uint32_t>(
-              min(cfg::scale_tiles, p.scale_tiles - st0) * kScaleTileBytes);
-          std::uint8_t *const sa = smem + stage * (cfg::a_bytes + cfg::b_bytes);
-          std::uint8_t *const sb = sa + cfg::a_bytes;
-          std::uint8_t *const sfa = scales + stage * (cfg::sfa_bytes + cfg::sfb_bytes);
-          std::uint8_t *const sfb = sfa + cfg::sfa_bytes;
-          ptx::mbar_arrive_expect_tx(
-              &full[stage], static_cast<std::uint32_t>(boxes) * kFp4SmallRows * 128 +
-                                cfg::b_bytes + sf_bytes * (1 + (kSwiglu ? 2 : b_tiles)));
-          std::int32_t const x = kb * 128;
-          if (boxes == 4) {
-            ptx::tma_load_2d(&map_a, &full[stage], sa, x, row);
-          } else {
-            for (std::int32_t i = 0; i < boxes; ++i) {
-              ptx::tma_load_2d(&map_a_small, &full[stage], sa + i * kFp4SmallRows * 128, x,
-                               row + i * kFp4SmallRows);
-            }
-          }
-          ptx::tma_load_2d(&map_b, &full[stage], sb, x, b_row);
-          if constexpr (kSwiglu) {
-            ptx::tma_load_2d(&map_b2, &full[stage], sb + cfg::b_bytes / 2, x, b_row);
-          }
-          ptx::bulk_load(sfa, p.a_scales + (a_scale + st0) * kScaleTileBytes, sf_bytes,
-                         &full[stage]);
-          ptx::bulk_load(sfb, p.b_scales + (b_scale + st0) * kScaleTileBytes, sf_bytes,
-                         &full[stage]);
-          if constexpr (kSwiglu) {
-            ptx::bulk_load(sfb + cfg::sfa_bytes, p.b2_scales + (b_scale + st0) * kScaleTileBytes,
-                           sf_bytes, &full[stage]);
-          } else if constexpr (BN == 256) {
-            if (b_tiles == 2) {
-              ptx::bulk_load(sfb + cfg::sfa_bytes,
-                             p.b_scales + (b_scale + p.scale_tiles + st0) * kScaleTileBytes,
-                             sf_bytes, &full[stage]);
-            }
-          }
-        }
+        __syncwarp();
+        if (lane == 0) load(l, kb, stage);
         __syncwarp();
         ++issued;
         if (++stage == kStages) {
@@ -411,130 +515,148 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
           phase ^= 1u;
         }
       }
+      skip = 0;
     }
-    if (!ok) {
-      // Copies still in flight land before the CTA may exit.
+    if (!ok && leader) {
+      // Copies still in flight land before the CTA may exit (a pair's are all
+      // counted by the leader).
       std::uint32_t const pending = issued < kStages ? issued : kStages;
       for (std::uint32_t i = 0; i < pending; ++i) {
         if (stage == 0) phase ^= 1u;
         stage = stage == 0 ? kStages - 1 : stage - 1;
-        ptx::mbar_wait(&full[stage], phase, nullptr, p.timeout_ns);
+        ptx::mbar_wait(&full[stage], phase, nullptr, kFp4DrainNs);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 && leader) {
     // ---------------- scale copies and MMA issue ----------------
-    if (lane == 0) {
-      std::uint32_t stage = 0, phase = 0, tile_index = 0;
-      std::uint32_t const sf = tmem + cfg::sf_column;
-      bool ok = true;
-      for (std::int32_t t = unit0; ok && t < tiles; t += units, ++tile_index) {
-        if (tile_index > 0 &&
-            !ptx::mbar_wait(acc_free, (tile_index - 1) & 1u, abort_word, p.timeout_ns)) {
-          detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 52);
+    std::uint32_t stage = 0, phase = 0, tile_index = 0;
+    std::uint32_t const sf = tmem + cfg::sf_column;
+    // Descriptors of stage 0; a stage is a multiple of 16 bytes further.
+    std::uint64_t const a_desc0 = ptx::smem_desc_sw128(ptx::smem_addr(smem), 16, 1024);
+    std::uint64_t const b_desc0 = a_desc0 + (cfg::a_bytes >> 4);
+    std::uint64_t const sf_desc0 = ptx::scale_desc(ptx::smem_addr(scales));
+    bool ok = true;
+    for (std::int32_t t = unit0; ok && t < tiles; t += units, ++tile_index) {
+      if (tile_index > 0 &&
+          !ptx::mbar_wait_cluster(acc_free, (tile_index - 1) & 1u, abort_word, p.timeout_ns)) {
+        if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 52);
+        break;
+      }
+      ptx::tc_fence_after_sync();
+      std::uint32_t const acc = tmem + (tile_index & 1u) * cfg::acc1;
+      for (std::int32_t kb = kb0; kb < kb1; ++kb) {
+        if (!ptx::mbar_wait_cluster(&full[stage], phase, abort_word, p.timeout_ns)) {
+          if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 53);
+          ok = false;
           break;
         }
+        __syncwarp();
         ptx::tc_fence_after_sync();
-        std::uint32_t const acc = tmem + (tile_index & 1u) * cfg::acc1;
-        for (std::int32_t kb = kb0; kb < kb1; ++kb) {
-          if (!ptx::mbar_wait(&full[stage], phase, abort_word, p.timeout_ns)) {
-            detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 53);
-            ok = false;
-            break;
+        std::uint32_t const at = stage * ((cfg::a_bytes + cfg::b_bytes) >> 4);
+        std::uint32_t const sf_at = stage * ((cfg::sfa_bytes + cfg::sfb_bytes) >> 4);
+        std::int32_t const steps = min(4, (p.k - kb * kFp4BlockK + 63) / 64);
+        if (ptx::elect_one()) {
+          // All of the stage's scale tiles, then its MMAs.
+          std::int32_t const scale_steps = kNv ? steps : (steps + 1) / 2;
+#pragma unroll
+          for (std::int32_t st = 0; st < cfg::scale_tiles; ++st) {
+            if (st >= scale_steps) break;
+            std::uint32_t const ta = sf + st * 4 * (1 + cfg::b_tiles);
+#pragma unroll
+            for (int h = 0; h < 1 + cfg::b_tiles; ++h) {  // A's, then B's row tiles
+              ptx::copy_scale_tile<kPair>(
+                  ta + 4 * h, sf_desc0 + sf_at + ((h * cfg::sfa_bytes + st * kScaleTileBytes) >> 4));
+            }
           }
-          ptx::tc_fence_after_sync();
-          std::uint32_t const sa = ptx::smem_addr(smem + stage * (cfg::a_bytes + cfg::b_bytes));
-          std::uint32_t const sb = sa + cfg::a_bytes;
-          std::uint32_t const sfa =
-              ptx::smem_addr(scales + stage * (cfg::sfa_bytes + cfg::sfb_bytes));
-          std::uint32_t const sfb = sfa + cfg::sfa_bytes;
-          std::int32_t const steps = min(4, (p.k - kb * kFp4BlockK + 63) / 64);
 #pragma unroll
           for (std::int32_t j = 0; j < 4; ++j) {
             if (j >= steps) break;
             // NV: one scale tile per 64 of K; MX: one per 128, a byte pair each.
-            std::int32_t const st = kNv ? j : j / 2;
-            std::uint32_t const ta = sf + st * 4 * (1 + BN / 128);
-            std::uint32_t const tb = ta + 4;
-            if (kNv || j % 2 == 0) {
-              ptx::copy_scale_tile(ta, ptx::scale_desc(sfa + st * kScaleTileBytes));
-#pragma unroll
-              for (int h = 0; h < BN / 128; ++h) {
-                ptx::copy_scale_tile(tb + 4 * h, ptx::scale_desc(sfb + h * cfg::sfa_bytes +
-                                                                 st * kScaleTileBytes));
-              }
-            }
-            ptx::umma_fp4<kNv>(acc, ptx::smem_desc_sw128(sa + j * 32, 16, 1024),
-                               ptx::smem_desc_sw128(sb + j * 32, 16, 1024),
-                               fp4_idesc<kNv>(kFp4BlockM, BN, kNv ? 0 : j % 2 * 2), ta, tb,
-                               kb > kb0 || j > 0);
+            std::uint32_t const ta = sf + (kNv ? j : j / 2) * 4 * (1 + cfg::b_tiles);
+            ptx::umma_fp4<kNv, kPair>(
+                acc, a_desc0 + at + j * 2, b_desc0 + at + j * 2,
+                fp4_idesc<kNv>(kFp4BlockM * (kPair ? 2 : 1), BN, kNv ? 0 : j % 2 * 2), ta, ta + 4,
+                kb > kb0 || j > 0);
           }
-          ptx::umma_commit(&empty[stage]);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          ptx::commit_fp4<kPair>(&empty[stage]);
         }
-        ptx::umma_commit(acc_full);
-        // MMAs in flight end before the CTA may free its TMEM.
-        if (!ok) ptx::mbar_wait(acc_full, tile_index & 1u, nullptr, p.timeout_ns);
+        __syncwarp();
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
+      if (ptx::elect_one()) ptx::commit_fp4<kPair>(acc_full);
+      __syncwarp();
+      // MMAs in flight end before the CTA may free its TMEM.
+      if (!ok) ptx::mbar_wait_cluster(acc_full, tile_index & 1u, nullptr, kFp4DrainNs);
     }
     __syncwarp();
-  } else {
+  } else if (warp >= 2) {
     // ---------------- epilogue ----------------
-    std::int32_t const quarter = warp & 3;  // TMEM lanes [32 quarter, +32)
-    std::uint8_t *const stage = staging + quarter * 2048;
+    std::int32_t const quarter = warp & 3;       // TMEM lanes [32 quarter, +32)
+    std::int32_t const half = (warp - 2) / 4;    // chunks half, half + 2, ...
+    std::uint8_t *const stage = staging + (warp - 2) * 1024;
     std::uint32_t const lanes = static_cast<std::uint32_t>(quarter * 32) << 16;
+    std::uint32_t const free_bar = kPair ? ptx::map_to_rank(acc_free, 0) : 0;
     std::uint32_t tile_index = 0;
     for (std::int32_t t = unit0; t < tiles; t += units, ++tile_index) {
-      fp4_tile const c = fp4_locate(t, m_tiles, p.n_tiles, p.group_m);
+      fp4_tile const c = locate(t);
       std::int32_t const row = c.row * kFp4BlockM;
       detail::fp4_rows const rows = detail::locate_rows(p, row);
-      std::int32_t const valid = rows.valid - quarter * 32;
       float const alpha = rows.alpha;
-      if (!ptx::mbar_wait(acc_full, tile_index & 1u, abort_word, p.timeout_ns)) {
+      detail::fp4_rows_out const out =
+          detail::rows_out(p, row + quarter * 32, rows.valid - quarter * 32);
+      if (!ptx::mbar_wait_cluster(acc_full, tile_index & 1u, abort_word, p.timeout_ns)) {
         if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 54);
         break;
       }
+      __syncwarp();
       ptx::tc_fence_after_sync();
+      if (split > 1) break;  // the cluster's exchange below
       std::uint32_t const acc = tmem + lanes + (tile_index & 1u) * cfg::acc1;
-      if (split > 1) {
-        // The columns of every slice to its CTA, once every ring is drained
-        // (after the cluster barrier below); kept out of this loop.
-        break;
-      }
-      if (BN < 256 && lane == 0) ptx::mbar_arrive(acc_free);  // the other accumulator is drained
-      // Chunks of 32 output columns, the shared TMEM columns (192..255) first:
-      // in the first accumulator the last ones, in the second the first ones.
-      constexpr int kChunks = kActCols / 32;
-      int const first = BN == 256 && (tile_index & 1u) == 0 ? kChunks - 2 : 0;
-#pragma unroll 1
-      for (int i = 0; i < kChunks; ++i) {
-        int const chunk = i + first < kChunks ? i + first : i + first - kChunks;
-        float v[32];
-        std::uint32_t raw[32];
-        ptx::tmem_load_32x32b_x32(acc + chunk * 32, raw);
-        if constexpr (kSwiglu) {
-          std::uint32_t up[32];
-          ptx::tmem_load_32x32b_x32(acc + kActCols + chunk * 32, up);
-          ptx::tmem_wait_load();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            v[e] = detail::swiglu(alpha * __uint_as_float(raw[e]), alpha * __uint_as_float(up[e]));
+      // The next tile's MMAs may start: with BN = 256 once the shared columns
+      // are drained, else at once, since the other accumulator is.
+      auto release = [&] {
+        ptx::tc_fence_before_sync();
+        if (lane == 0) {
+          if constexpr (kPair) {
+            ptx::mbar_arrive_remote(free_bar);
+          } else {
+            ptx::mbar_arrive(acc_free);
           }
-        } else {
-          ptx::tmem_wait_load();
+        }
+      };
+      if (BN < 256) release();
+      // Chunks of 32 output columns, the shared TMEM columns (192..255) first:
+      // in the first accumulator the last two, in the second the first two.
+      constexpr int kChunks = kActCols / 32;
+      int const first = half + (BN == 256 && (tile_index & 1u) == 0 ? kChunks - 2 : 0);
+      std::uint32_t raw[32], up[kSwiglu ? 32 : 1];
+      auto fetch = [&](int chunk) {
+        ptx::tmem_load_32x32b_x32(acc + chunk * 32, raw);
+        if constexpr (kSwiglu) ptx::tmem_load_32x32b_x32(acc + kActCols + chunk * 32, up);
+      };
+      fetch(first);
+#pragma unroll 1
+      for (int i = 0; i < kChunks / 2; ++i) {
+        int const chunk = (first + 2 * i) % kChunks;
+        float v[32];
+        ptx::tmem_wait_load();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = alpha * __uint_as_float(raw[e]);
+        for (int e = 0; e < 32; ++e) {
+          asm volatile("" : "+r"(raw[e]));  // not used before the wait
+          if constexpr (kSwiglu) asm volatile("" : "+r"(up[e]));
+          if constexpr (kSwiglu) {
+            v[e] = detail::swiglu(alpha * __uint_as_float(raw[e]), alpha * __uint_as_float(up[e]));
+          } else {
+            v[e] = alpha * __uint_as_float(raw[e]);
+          }
         }
-        if (BN == 256 && i == 1) {
-          ptx::tc_fence_before_sync();
-          if (lane == 0) ptx::mbar_arrive(acc_free);
-        }
+        if (BN == 256 && i == 0) release();
+        if (i + 1 < kChunks / 2) fetch((chunk + 2) % kChunks);  // in flight during the stores
         std::int32_t const col = c.col * kActCols + chunk * 32;
-        if (valid > 0 && col < p.n) {
-          detail::store_columns<32>(p, stage, v, row + quarter * 32, valid, col);
-        }
+        if (out.rows > 0 && col < p.n) detail::store_columns(p, stage, v, out, col);
       }
       ptx::tc_fence_before_sync();
     }
@@ -546,49 +668,48 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     // seen its last commit); slices are [rank][part][4 columns][128 rows].
     __syncwarp();
     ptx::cluster_sync();
-    bool const have = unit0 < tiles;
-    fp4_tile const c = have ? fp4_locate(unit0, m_tiles, p.n_tiles, p.group_m) : fp4_tile{0, 0};
-    std::int32_t const row = c.row * kFp4BlockM;
     std::int32_t const slice = kActCols / split;  // output columns per CTA
     constexpr int kParts = kSwiglu ? 2 : 1;
-    std::int32_t valid = 0;
-    float alpha = p.alpha;
-    std::int32_t const quarter = warp & 3;
-    if (have && warp >= 2) {
-      detail::fp4_rows const rows = detail::locate_rows(p, row);
-      valid = rows.valid - quarter * 32;
+    std::int32_t const quarter = warp & 3, half = (warp - 2) / 4;
+    fp4_tile c{0, 0};
+    detail::fp4_rows_out out{nullptr, 0, 0};
+    float alpha = 1.0f;
+    if (warp >= 2 && unit0 < tiles) {
+      c = locate(unit0);
+      detail::fp4_rows const rows = detail::locate_rows(p, c.row * kFp4BlockM);
+      out = detail::rows_out(p, c.row * kFp4BlockM + quarter * 32, rows.valid - quarter * 32);
       alpha = rows.alpha;
-      if (valid > 0) {
-        ptx::tc_fence_after_sync();
-        std::uint32_t const acc = tmem + (static_cast<std::uint32_t>(quarter * 32) << 16);
+    }
+    if (out.rows > 0) {
+      ptx::tc_fence_after_sync();
+      std::uint32_t const acc = tmem + (static_cast<std::uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-        for (int chunk = 0; chunk < BN / 32; ++chunk) {
-          std::uint32_t raw[32];
-          ptx::tmem_load_32x32b_x32(acc + chunk * 32, raw);
-          ptx::tmem_wait_load();
-          if (static_cast<std::int32_t>(lane) < valid) {
+      for (int chunk = half; chunk < BN / 32; chunk += 2) {
+        std::uint32_t raw[32];
+        ptx::tmem_load_32x32b_x32(acc + chunk * 32, raw);
+        ptx::tmem_wait_load();
+        if (static_cast<std::int32_t>(lane) < out.rows) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              std::int32_t const col = chunk * 32 + q * 4;
-              std::int32_t const part = kSwiglu ? col / kActCols : 0;
-              std::int32_t const in = col - part * kActCols;
-              std::int32_t const to = in / slice;
-              std::uint32_t const at = static_cast<std::uint32_t>(
-                  ((rank * kParts + part) * (slice / 4) + (in - to * slice) / 4) * 2048 +
-                  (quarter * 32 + static_cast<std::int32_t>(lane)) * 16);
-              ptx::st_shared_remote_v4(ptx::map_to_rank(smem + at, static_cast<std::uint32_t>(to)),
-                                       raw[q * 4], raw[q * 4 + 1], raw[q * 4 + 2], raw[q * 4 + 3]);
-            }
+          for (int q = 0; q < 8; ++q) {
+            std::int32_t const col = chunk * 32 + q * 4;
+            std::int32_t const part = kSwiglu ? col / kActCols : 0;
+            std::int32_t const in = col - part * kActCols;
+            std::int32_t const to = in / slice;
+            std::uint32_t const at = static_cast<std::uint32_t>(
+                ((rank * kParts + part) * (slice / 4) + (in - to * slice) / 4) * 2048 +
+                (quarter * 32 + static_cast<std::int32_t>(lane)) * 16);
+            ptx::st_shared_remote_v4(ptx::map_to_rank(smem + at, static_cast<std::uint32_t>(to)),
+                                     raw[q * 4], raw[q * 4 + 1], raw[q * 4 + 2], raw[q * 4 + 3]);
           }
         }
       }
     }
     __syncwarp();
     ptx::cluster_sync();
-    if (valid > 0) {
-      std::uint8_t *const stage = staging + quarter * 2048;
+    if (out.rows > 0) {
+      std::uint8_t *const stage = staging + (warp - 2) * 1024;
       std::uint32_t const mine = (static_cast<std::uint32_t>(quarter * 32) + lane) * 16;
-      for (std::int32_t c0 = 0; c0 < slice; c0 += 16) {
+      for (std::int32_t c0 = half * 16; c0 < slice; c0 += 32) {
         std::int32_t const col = c.col * kActCols + rank * slice + c0;
         if (col >= p.n) break;
         float sum[kParts][16] = {};
@@ -612,16 +733,21 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
           v[e] = kSwiglu ? detail::swiglu(alpha * sum[0][e], alpha * sum[kParts - 1][e])
                          : alpha * sum[0][e];
         }
-        detail::store_columns<16>(p, stage, v, row + quarter * 32, valid, col);
+        detail::store_columns(p, stage, v, out, col);
       }
     }
   }
 
   ptx::tc_fence_before_sync();
   __syncthreads();
+  if constexpr (kPair) ptx::cluster_sync();  // no more accesses to the other CTA
   if (warp == 1) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc(tmem, cfg::tmem_columns);
+    if constexpr (kPair) {
+      ptx::tmem_dealloc_pair(tmem, cfg::tmem_columns);
+    } else {
+      ptx::tmem_dealloc(tmem, cfg::tmem_columns);
+    }
   }
 }
 
