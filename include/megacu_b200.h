@@ -489,6 +489,9 @@ megacu_status megacu_cuda_moe_sort(megacu_driver_view driver, const void *expert
                                    void *slot_of_row, void *workspace,
                                    const megacu_moe_problem *problem);
 
+/* In the three calls below an entry of row_of_slot outside [0, sizes[0]) is a
+ * slot without a row. Entries of two slots must not name the same row. */
+
 /* rows[row_of_slot[t, j]] = x[t]; other rows are left as they were. Its
  * gradient is megacu_cuda_moe_combine of the rows' gradient without weights. */
 megacu_status megacu_cuda_moe_dispatch(megacu_driver_view driver, const void *x,
@@ -531,6 +534,7 @@ typedef struct megacu_fp4_matrix {
   int64_t rows;      /* rows of the quantised matrix; 0 is empty */
   int64_t cols;      /* its columns (a product's k); multiple of 32 */
   int64_t stride;    /* elements between rows of the plain matrix as stored; 0 = dense */
+  int64_t x_rows;    /* topk > 0: rows of the plain matrix */
   int32_t format;    /* enum megacu_fp4_format */
   int32_t dtype;     /* of the plain matrix: f16, bf16 or f32 */
   int32_t transpose; /* 1: the plain matrix is stored [cols, rows] */
@@ -550,7 +554,8 @@ megacu_status megacu_b200_fp4_sizes(const megacu_fp4_matrix *matrix, int64_t siz
  * scale; an NV block whose scale rounds to 0 holds zeros. Scale bytes behind
  * the last row or column of a tile are 0. With slot_of_row (int32 [rows], as
  * megacu_cuda_moe_sort writes it) rows whose entry is negative are left as
- * they were, scales included, and x is gathered when topk > 0; NULL: every row.
+ * they were, scales included, and x is gathered when topk > 0 (an entry that
+ * names no row of x counts as negative); NULL: every row.
  */
 megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, const void *x,
                                        const void *slot_of_row, void *data, void *scales,

@@ -18,6 +18,7 @@ per-site detail number.
 from __future__ import annotations
 
 import ctypes
+import functools
 import weakref
 from dataclasses import dataclass
 from typing import Callable, Optional, Sequence
@@ -491,36 +492,48 @@ def mlp_chain(x, w_gate, w_up, w_down, out, *, act, workspace, x_work, events_sw
 # ---- routing of tokens to experts, 4-bit products ---------------------------------------
 
 class _CProblem:
-    """Base of the problem dataclasses passed by pointer: the C struct is built
-    once and reused until a field changes."""
+    """Base of the problem dataclasses passed by pointer: the C struct, the
+    pointer to it and what follows from it are built once and reused until a
+    field changes."""
 
     def __setattr__(self, name, value):
         object.__setattr__(self, name, value)
         self.__dict__.pop("_c", None)
+        self.__dict__.pop("_sizes", None)
 
     def to_c(self):
         c = self.__dict__.get("_c")
         if c is None:
             c = self.__dict__["_c"] = self._build()
+            self.__dict__["_ref"] = ctypes.byref(c)
         return c
 
+    def _pointer(self):
+        self.to_c()
+        return self.__dict__["_ref"]
 
-_TORCH_NAMES = {_capi.DTYPE_F16: "torch.float16", _capi.DTYPE_BF16: "torch.bfloat16",
-                _capi.DTYPE_F32: "torch.float32"}
+
+@functools.lru_cache(None)
+def _types() -> dict:
+    """torch types by their element type code; "u8", "i32" and "i64" too."""
+    import torch
+    return {_capi.DTYPE_F16: torch.float16, _capi.DTYPE_BF16: torch.bfloat16,
+            _capi.DTYPE_F32: torch.float32, "u8": torch.uint8, "i32": torch.int32,
+            "i64": torch.int64}
 
 
-def _buffer(x, name: str, elements: int, size: int, device: int, dtype: int = 0) -> Optional[int]:
-    """The address of ``x``; a tensor must be contiguous, on ``device``, with
-    elements of ``size`` bytes (of ``dtype`` when given) and at least
-    ``elements`` of them. Raw addresses (int) are taken as they are."""
-    if x is None or isinstance(x, int):
+def _buffer(x, name: str, elements: int, dtype, device: int) -> Optional[int]:
+    """The address of ``x``: a contiguous tensor on ``device`` of the type with
+    code ``dtype`` and at least ``elements`` elements. None and raw addresses
+    (int) are taken as they are."""
+    if x is None or x.__class__ is int:
         return x
-    if x.device.type == "cuda" and x.device.index != device:
-        raise ValueError(f"{name} is on {x.device}, the call on device {device}")
-    if x.element_size() != size or (dtype and str(x.dtype) != _TORCH_NAMES[dtype]):
+    if x.dtype is not _types()[dtype]:
         raise ValueError(f"{name} has dtype {x.dtype}")
     if x.numel() < elements or not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous with at least {elements} elements")
+    if x.get_device() not in (device, -1):  # host tensors only pass a validate-only call
+        raise ValueError(f"{name} is on {x.device}, the call on device {device}")
     return x.data_ptr()
 
 
@@ -528,17 +541,15 @@ def _matrix(x, name: str, rows: int, cols: int, stride: int, dtype: int,
             device: int) -> Optional[int]:
     """The address of the row-major matrix ``x``, whose rows are ``stride``
     elements apart (0: dense)."""
-    if x is None or isinstance(x, int):
-        return x
-    if stride == 0 or stride == cols:
-        return _buffer(x, name, rows * cols, 2 if dtype != _capi.DTYPE_F32 else 4, device, dtype)
-    if x.device.type == "cuda" and x.device.index != device:
-        raise ValueError(f"{name} is on {x.device}, the call on device {device}")
-    if str(x.dtype) != _TORCH_NAMES[dtype]:
+    if stride == 0 or stride == cols or x is None or x.__class__ is int:
+        return _buffer(x, name, rows * cols, dtype, device)
+    if x.dtype is not _types()[dtype]:
         raise ValueError(f"{name} has dtype {x.dtype}")
     if (x.dim() != 2 or x.shape[0] < rows or x.shape[1] < cols or x.stride(1) != 1
             or (rows > 1 and x.stride(0) != stride)):
         raise ValueError(f"{name} must be [{rows}, {cols}] with rows {stride} elements apart")
+    if x.get_device() not in (device, -1):
+        raise ValueError(f"{name} is on {x.device}, the call on device {device}")
     return x.data_ptr()
 
 
@@ -563,15 +574,22 @@ class MoeProblem(_CProblem):
                                 align=self.align, dtype=self.dtype, id_bytes=id_bytes,
                                 token_stride=self.token_stride, row_stride=self.row_stride)
 
+    def _wide_ids(self):
+        """The pointer for 64-bit ids."""
+        self.to_c()
+        wide = self.__dict__.get("_wide")
+        if wide is None or wide[0] is not self._c:
+            wide = self.__dict__["_wide"] = (self._c, ctypes.byref(self._build(8)))
+        return wide[1]
+
 
 def _moe_sizes(problem: MoeProblem) -> tuple[int, int]:
-    c = problem.to_c()
     sizes = problem.__dict__.get("_sizes")
-    if sizes is None or sizes[0] is not c:
+    if sizes is None:
         out = (ctypes.c_int64 * 2)()
-        check(lib().megacu_b200_moe_sizes(ctypes.byref(c), out))
-        sizes = problem.__dict__["_sizes"] = (c, out[0], out[1])
-    return sizes[1], sizes[2]
+        check(lib().megacu_b200_moe_sizes(problem._pointer(), out))
+        sizes = problem.__dict__["_sizes"] = (out[0], out[1])
+    return sizes
 
 
 def moe_rows(problem: MoeProblem) -> int:
@@ -592,15 +610,16 @@ def moe_sort(expert_ids, *, counts, offsets, row_of_slot, slot_of_row, problem: 
     elsewhere and rows without a slot. ``workspace``: moe_workspace_bytes()."""
     rows, need = _moe_sizes(problem)
     slots, experts = problem.tokens * problem.topk, problem.experts
-    size = 4 if expert_ids is None or isinstance(expert_ids, int) else expert_ids.element_size()
-    c = problem.to_c() if size == 4 else problem._build(size)
+    wide = getattr(expert_ids, "dtype", None) is _types()["i64"]
     check(lib().megacu_cuda_moe_sort(
-        _launch_view(stream, device, None), _buffer(expert_ids, "expert_ids", slots, size, device),
-        _buffer(counts, "counts", experts, 4, device),
-        _buffer(offsets, "offsets", experts + 1, 4, device),
-        _buffer(row_of_slot, "row_of_slot", slots, 4, device),
-        _buffer(slot_of_row, "slot_of_row", rows, 4, device),
-        _buffer(workspace, "workspace", need, 1, device) if need else None, ctypes.byref(c)))
+        _launch_view(stream, device, None),
+        _buffer(expert_ids, "expert_ids", slots, "i64" if wide else "i32", device),
+        _buffer(counts, "counts", experts, "i32", device),
+        _buffer(offsets, "offsets", experts + 1, "i32", device),
+        _buffer(row_of_slot, "row_of_slot", slots, "i32", device),
+        _buffer(slot_of_row, "slot_of_row", rows, "i32", device),
+        _buffer(workspace, "workspace", need, "u8", device) if need else None,
+        problem._wide_ids() if wide else problem._pointer()))
 
 
 def _token_rows(x, name: str, p: MoeProblem, device: int) -> Optional[int]:
@@ -619,8 +638,8 @@ def moe_dispatch(x, rows, *, row_of_slot, problem: MoeProblem, stream=None,
     p = problem
     check(lib().megacu_cuda_moe_dispatch(
         _launch_view(stream, device, None), _token_rows(x, "x", p, device),
-        _buffer(row_of_slot, "row_of_slot", p.tokens * p.topk, 4, device),
-        _expert_rows(rows, "rows", p, device), ctypes.byref(p.to_c())))
+        _buffer(row_of_slot, "row_of_slot", p.tokens * p.topk, "i32", device),
+        _expert_rows(rows, "rows", p, device), p._pointer()))
 
 
 def moe_combine(rows, y, *, row_of_slot, problem: MoeProblem, weights=None, stream=None,
@@ -630,9 +649,9 @@ def moe_combine(rows, y, *, row_of_slot, problem: MoeProblem, weights=None, stre
     p, slots = problem, problem.tokens * problem.topk
     check(lib().megacu_cuda_moe_combine(
         _launch_view(stream, device, None), _expert_rows(rows, "rows", p, device),
-        _buffer(weights, "weights", slots, 4, device, _capi.DTYPE_F32),
-        _buffer(row_of_slot, "row_of_slot", slots, 4, device), _token_rows(y, "y", p, device),
-        ctypes.byref(p.to_c())))
+        _buffer(weights, "weights", slots, _capi.DTYPE_F32, device),
+        _buffer(row_of_slot, "row_of_slot", slots, "i32", device), _token_rows(y, "y", p, device),
+        p._pointer()))
 
 
 def moe_combine_grad(dy, rows, drows, dweights, *, weights, row_of_slot, problem: MoeProblem,
@@ -644,11 +663,11 @@ def moe_combine_grad(dy, rows, drows, dweights, *, weights, row_of_slot, problem
     check(lib().megacu_cuda_moe_combine_grad(
         _launch_view(stream, device, None), _token_rows(dy, "dy", p, device),
         _expert_rows(rows, "rows", p, device),
-        _buffer(weights, "weights", slots, 4, device, _capi.DTYPE_F32),
-        _buffer(row_of_slot, "row_of_slot", slots, 4, device),
+        _buffer(weights, "weights", slots, _capi.DTYPE_F32, device),
+        _buffer(row_of_slot, "row_of_slot", slots, "i32", device),
         _expert_rows(drows, "drows", p, device),
-        _buffer(dweights, "dweights", slots, 4, device, _capi.DTYPE_F32),
-        ctypes.byref(p.to_c())))
+        _buffer(dweights, "dweights", slots, _capi.DTYPE_F32, device),
+        p._pointer()))
 
 
 @dataclass
@@ -665,8 +684,8 @@ class Fp4Matrix(_CProblem):
     scale: float = 1.0
     stride: int = 0
 
-    def _build(self, topk: int = 0):
-        return _capi.Fp4Matrix(rows=self.rows, cols=self.cols, stride=self.stride,
+    def _build(self, topk: int = 0, x_rows: int = 0):
+        return _capi.Fp4Matrix(rows=self.rows, cols=self.cols, stride=self.stride, x_rows=x_rows,
                                format=self.format, dtype=self.dtype,
                                transpose=1 if self.transpose else 0, topk=topk,
                                scale=self.scale)
@@ -674,35 +693,41 @@ class Fp4Matrix(_CProblem):
 
 def fp4_sizes(problem: Fp4Matrix) -> tuple[int, int]:
     """Bytes of the data and of the scales of a quantised matrix."""
-    c = problem.to_c()
     sizes = problem.__dict__.get("_sizes")
-    if sizes is None or sizes[0] is not c:
+    if sizes is None:
         out = (ctypes.c_int64 * 2)()
-        check(lib().megacu_b200_fp4_sizes(ctypes.byref(c), out))
-        sizes = problem.__dict__["_sizes"] = (c, out[0], out[1])
-    return sizes[1], sizes[2]
+        check(lib().megacu_b200_fp4_sizes(problem._pointer(), out))
+        sizes = problem.__dict__["_sizes"] = (out[0], out[1])
+    return sizes
 
 
 def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, topk: int = 0,
-                 stream=None, device: int = 0) -> None:
+                 x_rows: int = 0, stream=None, device: int = 0) -> None:
     """Quantises ``x`` into ``data`` and ``scales`` (async). With
     ``slot_of_row`` (of :func:`moe_sort`, int32 [rows]) rows whose entry is
     negative are left as they were; with ``topk`` too, row r is taken from
-    x[slot_of_row[r] // topk]."""
+    x[slot_of_row[r] // topk] (``x_rows``: the rows of ``x``, needed only when
+    ``x`` is a raw address)."""
     p = problem
     nbytes, sbytes = fp4_sizes(p)
-    if topk:  # the gathered rows' number is the batch's, known to the caller alone
-        x_ptr = _matrix(x, "x", 0, p.cols, p.stride, p.dtype, device)
-    elif p.transpose:
-        x_ptr = _matrix(x, "x", p.cols, p.rows, p.stride, p.dtype, device)
+    if topk:
+        if x_rows == 0 and x is not None and x.__class__ is not int:
+            x_rows = x.shape[0]
+        x_ptr = _matrix(x, "x", x_rows, p.cols, p.stride, p.dtype, device)
+        key = (topk, x_rows)
+        gathered = p.__dict__.get("_gathered")
+        if gathered is None or gathered[0] is not p.to_c() or gathered[1] != key:
+            gathered = p.__dict__["_gathered"] = (p.to_c(), key, ctypes.byref(p._build(*key)))
+        pointer = gathered[2]
     else:
-        x_ptr = _matrix(x, "x", p.rows, p.cols, p.stride, p.dtype, device)
-    c = p._build(topk) if topk else p.to_c()
+        rows, cols = (p.cols, p.rows) if p.transpose else (p.rows, p.cols)
+        x_ptr = _matrix(x, "x", rows, cols, p.stride, p.dtype, device)
+        pointer = p._pointer()
     check(lib().megacu_cuda_fp4_quantize(
         _launch_view(stream, device, None), x_ptr,
-        _buffer(slot_of_row, "slot_of_row", p.rows, 4, device),
-        _buffer(data, "data", nbytes, 1, device), _buffer(scales, "scales", sbytes, 1, device),
-        ctypes.byref(c)))
+        _buffer(slot_of_row, "slot_of_row", p.rows, "i32", device),
+        _buffer(data, "data", nbytes, "u8", device),
+        _buffer(scales, "scales", sbytes, "u8", device), pointer))
 
 
 def fp4_dequantize(data, scales, out, *, problem: Fp4Matrix, stream=None,
@@ -712,9 +737,9 @@ def fp4_dequantize(data, scales, out, *, problem: Fp4Matrix, stream=None,
     p = problem
     nbytes, sbytes = fp4_sizes(p)
     check(lib().megacu_cuda_fp4_dequantize(
-        _launch_view(stream, device, None), _buffer(data, "data", nbytes, 1, device),
-        _buffer(scales, "scales", sbytes, 1, device),
-        _matrix(out, "out", p.rows, p.cols, p.stride, p.dtype, device), ctypes.byref(p.to_c())))
+        _launch_view(stream, device, None), _buffer(data, "data", nbytes, "u8", device),
+        _buffer(scales, "scales", sbytes, "u8", device),
+        _matrix(out, "out", p.rows, p.cols, p.stride, p.dtype, device), p._pointer()))
 
 
 @dataclass
@@ -751,8 +776,8 @@ def fp4_events_bytes() -> int:
 def _operand(data, scales, name: str, matrices: int, rows: int, p: Fp4Gemm, device: int):
     """Addresses of a quantised operand of ``matrices`` matrices [rows, k]."""
     tiles = -(-p.k // (128 if p.format == _capi.FP4_MX else 64))
-    return (_buffer(data, name, matrices * rows * (p.k // 2), 1, device),
-            _buffer(scales, name + "_scales", matrices * -(-rows // 128) * tiles * 512, 1, device))
+    return (_buffer(data, name, matrices * rows * (p.k // 2), "u8", device),
+            _buffer(scales, name, matrices * -(-rows // 128) * tiles * 512, "u8", device))
 
 
 def _product(fn, weights, a, a_scales, out, offsets, counts, alphas, events, p: Fp4Gemm, stream,
@@ -762,13 +787,12 @@ def _product(fn, weights, a, a_scales, out, offsets, counts, alphas, events, p: 
     for name, data, scales in weights:
         args += _operand(data, scales, name, experts, p.n, p, device)
     check(fn(_launch_view(stream, device, None), *args,
-             _buffer(offsets, "offsets", p.experts + 1, 4, device),
-             _buffer(counts, "counts", p.experts, 4, device),
-             _buffer(alphas, "alphas", p.experts, 4, device, _capi.DTYPE_F32),
+             _buffer(offsets, "offsets", p.experts + 1, "i32", device),
+             _buffer(counts, "counts", p.experts, "i32", device),
+             _buffer(alphas, "alphas", p.experts, _capi.DTYPE_F32, device),
              _matrix(out, "out", p.m, p.n, p.out_stride, p.out_dtype, device),
-             _buffer(events, "events", 256 // events.element_size(), events.element_size(), device)
-             if events is not None and not isinstance(events, int) else events,
-             ctypes.byref(p.to_c())))
+             _buffer(events, "events", 256, "u8", device),
+             p._pointer()))
 
 
 def fp4_gemm(a, a_scales, b, b_scales, out, *, events, problem: Fp4Gemm, offsets=None,

@@ -36,7 +36,7 @@ std::int64_t scale_tiles(std::int64_t cols, bool nv) { return ceil_div(cols, fp4
 
 megacu_status check_matrix(megacu_fp4_matrix const *m, int &log2_scale) {
   if (m == nullptr) return fail(MEGACU_INVALID_ARGUMENT, 2, "missing matrix");
-  if (m->rows < 0 || m->cols < 1 || m->stride < 0 || m->topk < 0) {
+  if (m->rows < 0 || m->cols < 1 || m->stride < 0 || m->topk < 0 || m->x_rows < 0) {
     return fail(MEGACU_INVALID_ARGUMENT, 1, "invalid matrix");
   }
   if (!known_format(m->format)) return fail(MEGACU_INVALID_ARGUMENT, 1, "unknown format");
@@ -66,6 +66,7 @@ fp4_matrix_params matrix_params(megacu_fp4_matrix const &m, int log2_scale, void
   p.tiles = static_cast<std::int32_t>(scale_tiles(m.cols, m.format == MEGACU_FP4_NV));
   p.col_tiles = static_cast<std::uint32_t>(ceil_div(m.cols, kQuantCols));
   p.topk = m.topk;
+  p.x_rows = m.x_rows;
   p.data = static_cast<std::uint8_t *>(data);
   p.scales = static_cast<std::uint8_t *>(scales);
   return p;

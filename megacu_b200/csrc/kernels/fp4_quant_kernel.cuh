@@ -30,6 +30,7 @@ struct fp4_matrix_params {
   std::int32_t tiles;    // scale tiles per row tile
   std::uint32_t col_tiles;  // CTAs per row tile, each kQuantCols columns
   std::int32_t topk;     // > 0: row r is x's row slot_of_row[r] / topk
+  std::int64_t x_rows;   // topk > 0: rows of x; an entry past them has no row
   std::int32_t const *slot_of_row;  // nullptr: every row; < 0: the row is left as it was
   std::uint8_t *data;    // [rows, cols / 2]
   std::uint8_t *scales;
@@ -173,7 +174,10 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
     if (in && p.slot_of_row != nullptr) {
       std::int32_t const slot = p.slot_of_row[row];
       in = slot >= 0;
-      if (p.topk > 0) src = slot / p.topk;
+      if (p.topk > 0) {
+        src = slot / p.topk;
+        in = in && src < p.x_rows;
+      }
     }
     if (in) done |= 1u << pass;
     // Both lanes of an MX block are in or out together (cols % 32 == 0).

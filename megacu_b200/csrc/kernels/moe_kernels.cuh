@@ -188,7 +188,13 @@ struct moe_rows_params {
   std::int64_t token_stride;  // elements between rows of x, y and dy
   std::int64_t row_stride;    // elements between rows of rows and drows
   std::int32_t const *row_of_slot;
+  std::uint32_t rows;  // capacity of the sorted order: an entry at or past it has no row
 };
+
+// The entry's row, or -1.
+__device__ __forceinline__ std::int32_t row_at(moe_rows_params const &p, std::int32_t entry) {
+  return static_cast<std::uint32_t>(entry) < p.rows ? entry : -1;
+}
 
 inline constexpr int kMoeGroup = 8;  // choices whose rows are in flight together
 
@@ -201,7 +207,7 @@ __global__ void moe_dispatch_kernel(moe_rows_params p, T const *x, T *rows) {
   for (int c = threadIdx.x * N; c < p.hidden; c += blockDim.x * N) {
     vec<T, N> const v = load_vec<T, N>(src + c);
     for (int j = 0; j < p.topk; ++j) {
-      std::int32_t const r = at[j];
+      std::int32_t const r = row_at(p, at[j]);
       if (r >= 0) store_vec<T, N>(rows + r * p.row_stride + c, v);
     }
   }
@@ -221,7 +227,7 @@ __global__ void moe_combine_kernel(moe_rows_params p, T const *rows, float const
       std::int32_t r[kMoeGroup];
 #pragma unroll
       for (int j = 0; j < kMoeGroup; ++j) {
-        r[j] = j0 + j < p.topk ? at[j0 + j] : -1;
+        r[j] = j0 + j < p.topk ? row_at(p, at[j0 + j]) : -1;
         if (r[j] >= 0) v[j] = load_vec<T, N>(rows + r[j] * p.row_stride + c);
       }
 #pragma unroll
@@ -256,7 +262,7 @@ __global__ void moe_combine_grad_kernel(moe_rows_params p, T const *dy, T const 
     float f[kMoeGroup], dot[kMoeGroup];
 #pragma unroll
     for (int j = 0; j < kMoeGroup; ++j) {
-      r[j] = j0 + j < p.topk ? at[j0 + j] : -1;
+      r[j] = j0 + j < p.topk ? row_at(p, at[j0 + j]) : -1;
       f[j] = r[j] >= 0 ? w[j0 + j] : 0.0f;
       dot[j] = 0.0f;
     }

@@ -54,6 +54,8 @@ megacu_status check_problem(megacu_moe_problem const *p) {
     return fail(MEGACU_UNSUPPORTED, 22,
                 "at most 32 choices, 1024 experts, an alignment of 1024 and 2^30 slots");
   }
+  static_assert(kMaxSlots + static_cast<std::int64_t>(kMoeMaxExperts) * kMaxAlign < 1ll << 31,
+                "rows are 32-bit");
   return ok_status();
 }
 
@@ -183,6 +185,7 @@ megacu_status run_rows(rows_op op, megacu_driver_view const &driver, rows_buffer
   prm.token_stride = p->token_stride != 0 ? p->token_stride : p->hidden;
   prm.row_stride = p->row_stride != 0 ? p->row_stride : p->hidden;
   prm.row_of_slot = row_of_slot;
+  prm.rows = static_cast<std::uint32_t>(capacity(*p));
   int const size = element_size(p->dtype);
   bool const vec = p->hidden * size % 16 == 0 && prm.token_stride * size % 16 == 0 &&
                    prm.row_stride * size % 16 == 0 && aligned_to(buffers[0], 16) &&

@@ -208,6 +208,19 @@ def test_quantize_gathered(align, fmt):
         assert (scales[at[~used]] == 0xEE).all()
 
 
+def test_gathered_entries_that_name_no_row_are_skipped():
+    x = torch.randn(6, 64).to(torch.bfloat16)
+    good = torch.tensor([0, -1, 11, -1, 5, -1], dtype=torch.int32)
+    bad = torch.tensor([0, 12, 11, 2 ** 31 - 1, 5, -2 ** 31], dtype=torch.int32)
+    m = mb.Fp4Matrix(6, 64)
+    got = []
+    for slots in (good, bad):
+        got.append(_buffers(m))
+        mb.fp4_quantize(x.cuda(), *got[-1], problem=m, slot_of_row=slots.cuda(), topk=2,
+                        stream=_stream())
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
 # ---- products ------------------------------------------------------------------------
 
 def _run(fn, *args, problem, **kw):

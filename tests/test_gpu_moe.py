@@ -240,3 +240,23 @@ def test_rows_beyond_2_31_elements():
     y = torch.zeros_like(x)
     mb.moe_combine(rows, y, row_of_slot=at, problem=p, stream=torch.cuda.current_stream())
     assert torch.equal(y[:, -1], x[:, -1])
+
+
+def test_entries_that_name_no_row_are_skipped():
+    """Entries outside the sorted order's capacity count as slots without a row."""
+    p = mb.MoeProblem(4, 2, 3, hidden=32, dtype=mb.DTYPE_F32)
+    cap = mb.moe_rows(p)
+    good = torch.tensor([[0, 1], [2, -1], [-1, -1], [5, 7]], dtype=torch.int32)
+    bad = torch.tensor([[0, 1], [2, cap], [2 ** 31 - 1, -2 ** 31], [5, 7]], dtype=torch.int32)
+    x, w = torch.randn(4, 32), torch.rand(4, 2)
+    got = []
+    for at in (good, bad):
+        kw = dict(row_of_slot=at.cuda(), problem=p, stream=torch.cuda.current_stream())
+        rows, y, drows = (torch.zeros(n, 32, device="cuda") for n in (cap, 4, cap))
+        dw = torch.empty(4, 2, device="cuda")
+        mb.moe_dispatch(x.cuda(), rows, **kw)
+        mb.moe_combine(rows, y, weights=w.cuda(), **kw)
+        mb.moe_combine_grad(x.cuda(), rows, drows, dw, weights=w.cuda(), **kw)
+        got.append((rows, y, drows, dw))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
