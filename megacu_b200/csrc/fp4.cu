@@ -45,7 +45,7 @@ megacu_status check_matrix(megacu_fp4_matrix const *m, int &log2_scale) {
     return fail(MEGACU_INVALID_ARGUMENT, 21, "cols must be a multiple of 32 (16-byte rows)");
   }
   if (m->rows > kMaxDim || m->cols > kMaxDim ||
-      ceil_div(m->rows, kScaleTileRows) * ceil_div(m->cols, kQuantCols) > 0x7fffffffll) {
+      4 * ceil_div(m->rows, kScaleTileRows) * ceil_div(m->cols, kQuantCols) > 0x7fffffffll) {
     return fail(MEGACU_UNSUPPORTED, 22, "dimension too large");
   }
   int e = 0;
@@ -383,8 +383,8 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
   if (guard.status() != cudaSuccess) return cuda_fail(guard.status(), 10);
   fp4_matrix_params prm = matrix_params(m, log2_scale, data, scales, transpose);
   prm.slot_of_row = static_cast<std::int32_t const *>(slot_of_row);
-  auto const grid =
-      static_cast<unsigned>(ceil_div(m.rows, kScaleTileRows) * prm.col_tiles);
+  auto const grid = static_cast<unsigned>(ceil_div(m.rows, kScaleTileRows) * prm.col_tiles *
+                                          (transpose ? 2 : 4));
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
   by_type(m.dtype, m.format, [&](auto value, auto nv) {
     using T = decltype(value);
@@ -393,11 +393,11 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
     if (transpose) {
       // Pairs of columns are read together when every row starts on a pair.
       if (m.rows % 2 == 0 && prm.stride % 2 == 0 && aligned_to(x, 2 * size)) {
-        fp4_quantize_t_kernel<T, kNv, true><<<grid, kQuantTThreads, 0, stream>>>(prm, src);
+        fp4_quantize_t_kernel<T, kNv, true><<<grid, kQuantThreads, 0, stream>>>(prm, src);
       } else {
-        fp4_quantize_t_kernel<T, kNv, false><<<grid, kQuantTThreads, 0, stream>>>(prm, src);
+        fp4_quantize_t_kernel<T, kNv, false><<<grid, kQuantThreads, 0, stream>>>(prm, src);
       }
-    } else if (prm.stride * size % 16 == 0 && aligned_to(x, 16)) {
+    } else if (prm.stride * size % 32 == 0 && aligned_to(x, 32)) {
       fp4_quantize_kernel<T, kNv, true><<<grid, kQuantThreads, 0, stream>>>(prm, src);
     } else {
       fp4_quantize_kernel<T, kNv, false><<<grid, kQuantThreads, 0, stream>>>(prm, src);
@@ -434,10 +434,9 @@ extern "C" megacu_status megacu_cuda_fp4_dequantize(megacu_driver_view driver, v
   if (guard.status() != cudaSuccess) return cuda_fail(guard.status(), 10);
   fp4_matrix_params const prm =
       matrix_params(m, log2_scale, const_cast<void *>(data), const_cast<void *>(scales), false);
-  auto const grid = static_cast<unsigned>(
-      std::min<std::int64_t>(ceil_div(m.rows * (m.cols / 16), kQuantThreads), 1 << 20));
+  auto const grid = static_cast<unsigned>(ceil_div(m.rows, kQuantRows) * prm.col_tiles);
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
-  bool const vec = prm.stride * size % 16 == 0 && aligned_to(out, 16);
+  bool const vec = prm.stride * size % 32 == 0 && aligned_to(out, 32);
   by_type(m.dtype, m.format, [&](auto value, auto nv) {
     using T = decltype(value);
     constexpr bool kNv = decltype(nv)::value;

@@ -122,53 +122,101 @@ __device__ __forceinline__ std::uint32_t encode8(float const *x, fp4_block_scale
   return empty ? 0u : w;
 }
 
-template <class T>
-__device__ __forceinline__ std::uint32_t abs_bits(T v) {
-  return __float_as_uint(to_f32(v)) & 0x7fffffffu;
+// The largest |v[i]| of 16-bit pairs or 32-bit words as a 32-bit float pattern.
+// Magnitudes of one type order as their bit patterns do, NaN above infinity.
+template <class T, int kWords>
+__device__ __forceinline__ std::uint32_t max_abs(std::uint32_t const *w) {
+  if constexpr (sizeof(T) == 4) {
+    std::uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m;
+  } else {
+    std::uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      return m << 16;
+    } else {
+      return __float_as_uint(__half2float(__ushort_as_half(static_cast<std::uint16_t>(m))));
+    }
+  }
 }
 
-// 16 consecutive elements, by 16-byte loads when the rows allow it.
-template <class T, bool kVec>
-__device__ __forceinline__ void load16(T const *p, T (&v)[16]) {
-  if constexpr (kVec) {
-    constexpr int kN = 16 / sizeof(T);
+template <class T>
+__device__ __forceinline__ float element(std::uint32_t const *w, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(w[i]);
+  } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  } else {
+    return __half2float(__ushort_as_half(static_cast<std::uint16_t>(w[i / 2] >> (16 * (i % 2)))));
+  }
+}
+
+// Eight elements from element `first` of `w` to one 32-bit word.
+template <class T, bool kNv>
+__device__ __forceinline__ std::uint32_t encode_words(std::uint32_t const *w, int first,
+                                                      fp4_block_scale const &b) {
+  float f[8];
 #pragma unroll
-    for (int i = 0; i < 16 / kN; ++i) {
-      *reinterpret_cast<vec<T, kN> *>(&v[i * kN]) = load_vec<T, kN>(p + i * kN);
+  for (int i = 0; i < 8; ++i) f[i] = element<T>(w, first + i);
+  return encode8<kNv, std::is_same_v<T, float>>(f, b);
+}
+
+// 16 consecutive elements as words, by 32-byte loads when the rows allow it.
+template <class T, bool kVec>
+__device__ __forceinline__ void load16(T const *p, std::uint32_t (&w)[4 * sizeof(T)]) {
+  if constexpr (kVec) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+      bytes32 const v = load32_once(reinterpret_cast<char const *>(p) + 32 * i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[8 * i + j] = v.w[j];
     }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = reinterpret_cast<std::uint32_t const *>(p)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = p[i];
+    for (int i = 0; i < 8; ++i) {
+      std::uint16_t const *const q = reinterpret_cast<std::uint16_t const *>(p) + 2 * i;
+      w[i] = q[0] | static_cast<std::uint32_t>(q[1]) << 16;
+    }
   }
 }
 
 inline constexpr int kQuantThreads = 256;
-inline constexpr int kQuantCols = 256;  // columns of a CTA's tile of 128 rows
+inline constexpr int kQuantCols = 256;  // columns of a CTA
+inline constexpr int kQuantRows = 32;   // rows of a CTA: 8 of each 32 rows of a scale tile
 
-// A CTA quantises 128 rows x 256 columns: 16 lanes per row with 16 elements
-// each (512 bytes of a 16-bit row, 128 bytes of elements out), so that it
-// owns whole scale tiles and writes them as 16-byte vectors.
+// A CTA quantises 32 rows x 256 columns: 16 lanes per row with 16 elements
+// each (512 bytes of a 16-bit row, 128 bytes of elements out). Its rows are
+// rows [8 s, 8 s + 8) of each quarter of a 128-row scale tile, so that the
+// scale bytes it owns are 128 contiguous bytes of each of its scale tiles.
+// Two passes per CTA, both rows' loads in flight.
 template <class T, bool kNv, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_params p,
                                                                     T const *x) {
   constexpr bool kWide = std::is_same_v<T, float>;
   constexpr int kTileCols = fp4_tile_cols(kNv);
   constexpr int kTiles = kQuantCols / kTileCols;
-  __shared__ alignas(16) std::uint8_t smem[kTiles * kScaleTileBytes];
-  std::int64_t const row_tile = blockIdx.x / p.col_tiles;
-  std::int64_t const row0 = row_tile * kScaleTileRows;
-  int const col0 = static_cast<int>(blockIdx.x % p.col_tiles) * kQuantCols;
-  int const lane16 = threadIdx.x % 16, sub = threadIdx.x / 16;
+  constexpr int kPasses = kQuantRows / 16;
+  // [tile][row of the slice][quarter] of four scale bytes
+  __shared__ std::uint32_t bytes[kTiles][8][4];
+  std::int64_t const row_tile = blockIdx.x / (4 * p.col_tiles);
+  int const slice = static_cast<int>(blockIdx.x % 4);
+  int const col0 = static_cast<int>(blockIdx.x / 4 % p.col_tiles) * kQuantCols;
+  int const lane16 = threadIdx.x % 16;
   int const col = col0 + lane16 * 16;
-  for (int i = threadIdx.x; i < kTiles * kScaleTileBytes / 4; i += kQuantThreads) {
-    reinterpret_cast<std::uint32_t *>(smem)[i] = 0;
-  }
-  __syncthreads();
-  std::uint32_t done = 0;  // passes that wrote this thread's row
-#pragma unroll 2
-  for (int pass = 0; pass < kScaleTileRows / 16; ++pass) {
-    int const r = pass * 16 + sub;
-    std::int64_t const row = row0 + r;
+
+  std::uint32_t w[kPasses][4 * sizeof(T)];
+  std::int64_t rows[kPasses];  // -1: nothing of this row is written
+#pragma unroll
+  for (int pass = 0; pass < kPasses; ++pass) {
+    int const l = pass * 16 + threadIdx.x / 16;
+    std::int64_t const row = row_tile * kScaleTileRows + l / 8 * 32 + slice * 8 + l % 8;
     std::int64_t src = row;
     bool in = row < p.rows;
     if (in && p.slot_of_row != nullptr) {
@@ -179,117 +227,144 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
         in = in && src < p.x_rows;
       }
     }
-    if (in) done |= 1u << pass;
+    rows[pass] = in ? row : -1;
+    if (in && col < p.cols) load16<T, kVec>(x + src * p.stride + col, w[pass]);
+  }
+#pragma unroll
+  for (int pass = 0; pass < kPasses; ++pass) {
+    int const l = pass * 16 + threadIdx.x / 16;
+    fp4_block_scale b{};
     // Both lanes of an MX block are in or out together (cols % 32 == 0).
-    if (!in || col >= p.cols) continue;
-    T v[16];
-    load16<T, kVec>(x + src * p.stride + col, v);
-    std::uint32_t bits = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bits = max(bits, abs_bits(v[i]));
-    if constexpr (!kNv) {
-      bits = max(bits, __shfl_xor_sync(3u << (threadIdx.x % 32 & ~1u), bits, 1));
+    if (rows[pass] >= 0 && col < p.cols) {
+      std::uint32_t bits = max_abs<T, 4 * sizeof(T)>(w[pass]);
+      if constexpr (!kNv) {
+        bits = max(bits, __shfl_xor_sync(3u << (threadIdx.x % 32 & ~1u), bits, 1));
+      }
+      b = block_scale<kNv, kWide>(bits, p.log2_scale);
+      uint2 out;
+      out.x = encode_words<T, kNv>(w[pass], 0, b);
+      out.y = encode_words<T, kNv>(w[pass], 8, b);
+      *reinterpret_cast<uint2 *>(p.data + rows[pass] * (p.cols / 2) + col / 2) = out;
     }
-    fp4_block_scale const b = block_scale<kNv, kWide>(bits, p.log2_scale);
-    float f[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = to_f32(v[i]);
-    uint2 out;
-    out.x = encode8<kNv, kWide>(f, b);
-    out.y = encode8<kNv, kWide>(f + 8, b);
-    *reinterpret_cast<uint2 *>(p.data + row * (p.cols / 2) + col / 2) = out;
     if (kNv || lane16 % 2 == 0) {
       int const blk = lane16 * 16 / fp4_block(kNv);
-      smem[blk / 4 * kScaleTileBytes + scale_byte(r, blk)] = static_cast<std::uint8_t>(b.byte);
+      reinterpret_cast<std::uint8_t *>(&bytes[blk / 4][l % 8][l / 8])[blk % 4] =
+          static_cast<std::uint8_t>(b.byte);
     }
   }
   __syncthreads();
   int const tile0 = col0 / kTileCols;
   int const tiles = min(kTiles, p.tiles - tile0);
-  std::uint8_t *const dst = p.scales + (row_tile * p.tiles + tile0) * kScaleTileBytes;
+  std::uint8_t *const dst = p.scales + (row_tile * p.tiles + tile0) * kScaleTileBytes + slice * 128;
   if (p.slot_of_row == nullptr) {
-    for (int i = threadIdx.x; i < tiles * kScaleTileBytes / 16; i += kQuantThreads) {
-      reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<uint4 const *>(smem)[i];
+    if (static_cast<int>(threadIdx.x) < tiles * 8) {
+      int const tile = threadIdx.x / 8, r = threadIdx.x % 8;
+      *reinterpret_cast<uint4 *>(dst + tile * kScaleTileBytes + r * 16) =
+          *reinterpret_cast<uint4 const *>(bytes[tile][r]);
     }
   } else if (lane16 < tiles) {
     // Only the rows written above: their four bytes of each tile.
 #pragma unroll
-    for (int pass = 0; pass < kScaleTileRows / 16; ++pass) {
-      if ((done >> pass & 1u) == 0) continue;
-      int const at = lane16 * kScaleTileBytes + scale_byte(pass * 16 + sub, 0);
-      *reinterpret_cast<std::uint32_t *>(dst + at) =
-          *reinterpret_cast<std::uint32_t const *>(smem + at);
+    for (int pass = 0; pass < kPasses; ++pass) {
+      int const l = pass * 16 + threadIdx.x / 16;
+      if (rows[pass] < 0) continue;
+      *reinterpret_cast<std::uint32_t *>(dst + lane16 * kScaleTileBytes + l % 8 * 16 + l / 8 * 4) =
+          bytes[lane16][l % 8][l / 8];
     }
   }
 }
 
-inline constexpr int kQuantTThreads = 512;
+inline constexpr int kQuantTRows = 64;  // rows of the quantised matrix per CTA
 
 // The transpose: x is [cols, rows] as stored and its columns become the rows
 // of the quantised matrix. A thread reads 32 elements down two neighbouring
 // columns (a warp reads 64 neighbouring columns of each row, 128 bytes of a
-// 16-bit type); the CTA's 128 x 256 tile of elements is turned in shared
+// 16-bit type); the CTA's 64 x 256 tile of elements is turned in shared
 // memory so that each row leaves as 128 contiguous bytes.
 template <class T, bool kNv, bool kPair>
-__global__ void __launch_bounds__(kQuantTThreads) fp4_quantize_t_kernel(fp4_matrix_params p,
-                                                                       T const *x) {
+__global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_matrix_params p,
+                                                                         T const *x) {
   constexpr bool kWide = std::is_same_v<T, float>;
   constexpr int kTileCols = fp4_tile_cols(kNv);
   constexpr int kTiles = kQuantCols / kTileCols;
-  __shared__ alignas(16) std::uint8_t scales[kTiles * kScaleTileBytes];
-  __shared__ uint4 turned[kScaleTileRows][8];
-  std::int64_t const row_tile = blockIdx.x / p.col_tiles;
-  std::int64_t const row0 = row_tile * kScaleTileRows;
-  int const col0 = static_cast<int>(blockIdx.x % p.col_tiles) * kQuantCols;
-  for (int i = threadIdx.x; i < kTiles * kScaleTileBytes / 4; i += kQuantTThreads) {
-    reinterpret_cast<std::uint32_t *>(scales)[i] = 0;
-  }
-  __syncthreads();
-  int const r = threadIdx.x % 64 * 2, chunk = threadIdx.x / 64;
+  constexpr int kBlock = fp4_block(kNv);
+  constexpr int kWordBlock = kBlock * sizeof(T) / 4;
+  // [tile][row % 32][row / 32] of four scale bytes
+  __shared__ std::uint32_t bytes[kTiles][32][2];
+  __shared__ uint4 turned[kQuantTRows][8];
+  std::int64_t const row_tile = blockIdx.x / (2 * p.col_tiles);
+  int const part = static_cast<int>(blockIdx.x % 2);
+  std::int64_t const row0 = row_tile * kScaleTileRows + part * kQuantTRows;
+  int const col0 = static_cast<int>(blockIdx.x / 2 % p.col_tiles) * kQuantCols;
+  int const r = threadIdx.x % 32 * 2, chunk = threadIdx.x / 32;
   std::int64_t const row = row0 + r;
   int const col = col0 + chunk * 32;
-  if (col < p.cols && row < p.rows) {
-    bool const two = row + 1 < p.rows;
-    T v[2][32];
+  bool const in = col < p.cols && row < p.rows;
+  bool const two = row + 1 < p.rows;
+  std::uint32_t w[2][8 * sizeof(T)];
+  if (in) {
     T const *src = x + col * p.stride + row;
 #pragma unroll
     for (int i = 0; i < 32; ++i, src += p.stride) {
-      if constexpr (kPair) {
-        vec<T, 2> const pair = *reinterpret_cast<vec<T, 2> const *>(src);
-        v[0][i] = pair.v[0];
-        v[1][i] = pair.v[1];
+      if constexpr (sizeof(T) == 4) {
+        if constexpr (kPair) {
+          uint2 const v = *reinterpret_cast<uint2 const *>(src);
+          w[0][i] = v.x;
+          w[1][i] = v.y;
+        } else {
+          w[0][i] = __float_as_uint(src[0]);
+          w[1][i] = two ? __float_as_uint(src[1]) : 0;
+        }
       } else {
-        v[0][i] = src[0];
-        v[1][i] = two ? src[1] : from_f32<T>(0.0f);
+        std::uint32_t v;
+        if constexpr (kPair) {
+          v = *reinterpret_cast<std::uint32_t const *>(src);
+        } else {
+          auto const *const q = reinterpret_cast<std::uint16_t const *>(src);
+          v = q[0] | (two ? static_cast<std::uint32_t>(q[1]) << 16 : 0u);
+        }
+        // One word holds a column pair of one row; pack rows 2k, 2k + 1 of
+        // each column into a word below.
+        w[i % 2][i / 2] = v;
       }
     }
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h == 1 && !two) break;
-      std::uint32_t out[4];
-      constexpr int kBlock = fp4_block(kNv);
+      for (int i = 0; i < 16; ++i) {
+        std::uint32_t const even = w[0][i], odd = w[1][i];
+        w[0][i] = __byte_perm(even, odd, 0x5410);
+        w[1][i] = __byte_perm(even, odd, 0x7632);
+      }
+    }
+  }
 #pragma unroll
-      for (int k = 0; k < 32 / kBlock; ++k) {
-        std::uint32_t bits = 0;
+  for (int h = 0; h < 2; ++h) {
+    std::uint32_t out[4];
+    std::uint32_t scale[32 / kBlock];
 #pragma unroll
-        for (int i = 0; i < kBlock; ++i) bits = max(bits, abs_bits(v[h][k * kBlock + i]));
-        fp4_block_scale const b = block_scale<kNv, kWide>(bits, p.log2_scale);
+    for (int k = 0; k < 32 / kBlock; ++k) {
+      scale[k] = 0;
+      if (in && (h == 0 || two)) {
+        std::uint32_t const *const v = w[h] + k * kWordBlock;
+        fp4_block_scale const b =
+            block_scale<kNv, kWide>(max_abs<T, kWordBlock>(v), p.log2_scale);
 #pragma unroll
         for (int i = 0; i < kBlock / 8; ++i) {
-          float f[8];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) f[c] = to_f32(v[h][k * kBlock + i * 8 + c]);
-          out[k * (kBlock / 8) + i] = encode8<kNv, kWide>(f, b);
+          out[k * (kBlock / 8) + i] = encode_words<T, kNv>(v, i * 8, b);
         }
-        int const blk = chunk * (32 / kBlock) + k;
-        scales[blk / 4 * kScaleTileBytes + scale_byte(r + h, blk)] =
-            static_cast<std::uint8_t>(b.byte);
+        scale[k] = b.byte;
       }
+      int const blk = chunk * (32 / kBlock) + k;
+      reinterpret_cast<std::uint8_t *>(&bytes[blk / 4][(r + h) % 32][(r + h) / 32])[blk % 4] =
+          static_cast<std::uint8_t>(scale[k]);
+    }
+    if (in && (h == 0 || two)) {
       turned[r + h][chunk ^ (r / 2 % 8)] = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kScaleTileRows * 8; i += kQuantTThreads) {
+#pragma unroll
+  for (int i = threadIdx.x; i < kQuantTRows * 8; i += kQuantThreads) {
     int const rr = i / 8, c = i % 8;
     if (row0 + rr < p.rows && col0 + c * 32 < p.cols) {
       *reinterpret_cast<uint4 *>(p.data + (row0 + rr) * (p.cols / 2) + col0 / 2 + c * 16) =
@@ -298,9 +373,11 @@ __global__ void __launch_bounds__(kQuantTThreads) fp4_quantize_t_kernel(fp4_matr
   }
   int const tile0 = col0 / kTileCols;
   int const tiles = min(kTiles, p.tiles - tile0);
-  std::uint8_t *const dst = p.scales + (row_tile * p.tiles + tile0) * kScaleTileBytes;
-  for (int i = threadIdx.x; i < tiles * kScaleTileBytes / 16; i += kQuantTThreads) {
-    reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<uint4 const *>(scales)[i];
+  std::uint8_t *const dst = p.scales + (row_tile * p.tiles + tile0) * kScaleTileBytes + part * 8;
+  if (static_cast<int>(threadIdx.x) < tiles * 32) {
+    int const tile = threadIdx.x / 32, rr = threadIdx.x % 32;
+    *reinterpret_cast<uint2 *>(dst + tile * kScaleTileBytes + rr * 16) =
+        *reinterpret_cast<uint2 const *>(bytes[tile][rr]);
   }
 }
 
@@ -308,15 +385,17 @@ __global__ void __launch_bounds__(kQuantTThreads) fp4_quantize_t_kernel(fp4_matr
 // thread decodes 16 elements.
 template <class T, bool kNv, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matrix_params p, T *y) {
-  int const per_row = p.cols / 16;
-  std::int64_t const total = p.rows * per_row;
-  std::int64_t const step = static_cast<std::int64_t>(gridDim.x) * kQuantThreads;
-  for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * kQuantThreads + threadIdx.x;
-       i < total; i += step) {
-    std::int64_t const row = i / per_row;
-    int const col = static_cast<int>(i - row * per_row) * 16;
+  std::uint32_t const per_row = static_cast<std::uint32_t>(p.cols) / 16;
+  std::uint32_t const i = blockIdx.x % p.col_tiles * 16 + threadIdx.x % 16;
+  if (i >= per_row) return;
+  int const col = static_cast<int>(i) * 16;
+  int const blk = col / fp4_block(kNv);
+  std::int64_t const row0 = static_cast<std::int64_t>(blockIdx.x / p.col_tiles) * kQuantRows;
+#pragma unroll
+  for (int pass = 0; pass < kQuantRows / 16; ++pass) {
+    std::int64_t const row = row0 + pass * 16 + threadIdx.x / 16;
+    if (row >= p.rows) break;
     uint2 const d = *reinterpret_cast<uint2 const *>(p.data + row * (p.cols / 2) + col / 2);
-    int const blk = col / fp4_block(kNv);
     std::uint32_t const byte =
         p.scales[((row / kScaleTileRows) * p.tiles + blk / 4) * kScaleTileBytes +
                  scale_byte(static_cast<int>(row % kScaleTileRows), blk)];
@@ -330,7 +409,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matri
       s1 = byte == 0xffu ? __int_as_float(0x7fffffff) : pow2(e / 2);
       s2 = pow2(e - e / 2);
     }
-    T out[16];
+    alignas(32) T out[16];
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
       std::uint32_t const w = b < 4 ? d.x : d.y;
@@ -340,10 +419,10 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matri
     }
     T *const dst = y + row * p.stride + col;
     if constexpr (kVec) {
-      constexpr int kN = 16 / sizeof(T);
 #pragma unroll
-      for (int c = 0; c < 16 / kN; ++c) {
-        store_vec<T, kN>(dst + c * kN, *reinterpret_cast<vec<T, kN> const *>(&out[c * kN]));
+      for (int c = 0; c < static_cast<int>(sizeof(T)) / 2; ++c) {
+        store32(reinterpret_cast<char *>(dst) + 32 * c,
+                reinterpret_cast<bytes32 const *>(out)[c]);
       }
     } else {
 #pragma unroll

@@ -19,8 +19,8 @@ namespace megacu_b200 {
 
 inline constexpr int kMoeMaxExperts = 1024;
 inline constexpr int kMoeMaxTopk = 32;
-inline constexpr int kMoeSortThreads = 1024;
-inline constexpr int kMoeSortWarps = kMoeSortThreads / 32;
+inline constexpr int kMoeSortThreads = 1024;  // at most; fewer for few slots
+inline constexpr int kMoeMaxChunk = 8192;     // slots per CTA
 
 struct moe_sort_params {
   void const *ids;
@@ -49,17 +49,17 @@ template <class Id>
 __global__ void __launch_bounds__(kMoeSortThreads) moe_count_kernel(moe_sort_params p) {
   extern __shared__ std::int32_t moe_smem[];
   asm volatile("griddepcontrol.launch_dependents;");
-  for (int e = threadIdx.x; e < p.experts; e += kMoeSortThreads) moe_smem[e] = 0;
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) moe_smem[e] = 0;
   __syncthreads();
   std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
   std::int64_t const end = min(begin + p.chunk, p.slots);
-  for (std::int64_t s = begin + threadIdx.x; s < end; s += kMoeSortThreads) {
+  for (std::int64_t s = begin + threadIdx.x; s < end; s += blockDim.x) {
     std::int32_t const e = local_expert<Id>(p, s);
     if (e >= 0) atomicAdd(&moe_smem[e], 1);
   }
   __syncthreads();
   std::int32_t *const mine = p.histogram + static_cast<std::int64_t>(blockIdx.x) * p.experts;
-  for (int e = threadIdx.x; e < p.experts; e += kMoeSortThreads) mine[e] = moe_smem[e];
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) mine[e] = moe_smem[e];
 }
 
 // Places one chunk of slots per CTA. Every warp owns a contiguous part of the
@@ -67,27 +67,40 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_count_kernel(moe_sort_par
 // first row of each expert is the expert's start, plus what earlier chunks
 // and earlier warps hold of it; within 32 slots, lanes of one expert rank
 // themselves by a warp match. No counter is kept between calls and nothing
-// depends on the order of atomics.
+// depends on the order of atomics (they add whole numbers). Bound by the
+// latency of a handful of dependent steps, so the ids are read once and kept
+// as 16-bit local experts.
+//
+// Shared memory: cursor [warps][experts], total [experts], start [experts],
+// then the chunk's local experts (int16).
+__host__ __device__ inline int moe_place_smem(int warps, int experts, int chunk) {
+  return (warps + 2) * experts * 4 + chunk * 2;
+}
+
 template <class Id>
 __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_params p) {
   extern __shared__ std::int32_t moe_smem[];
-  __shared__ std::int32_t warp_sums[kMoeSortWarps];
-  int const experts = p.experts;
-  std::int32_t *const cursor = moe_smem;                           // [warps][experts]
-  std::int32_t *const total = moe_smem + kMoeSortWarps * experts;  // [experts]
-  std::int32_t *const start = total + experts;                     // [experts]
+  __shared__ std::int32_t warp_sums[32];
+  int const experts = p.experts, threads = blockDim.x, warps = threads / 32;
+  std::int32_t *const cursor = moe_smem;
+  std::int32_t *const total = moe_smem + warps * experts;
+  std::int32_t *const start = total + experts;
+  auto *const local = reinterpret_cast<std::int16_t *>(start + experts);
   int const tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
 
-  for (int i = tid; i < (kMoeSortWarps + 2) * experts; i += kMoeSortThreads) moe_smem[i] = 0;
-  __syncthreads();
   std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
-  std::int64_t const end = min(begin + p.chunk, p.slots);
-  std::int32_t const part = (p.chunk + kMoeSortThreads - 1) / kMoeSortThreads * 32;
-  std::int64_t const w0 = min(begin + static_cast<std::int64_t>(warp) * part, end);
-  std::int64_t const w1 = min(w0 + part, end);
+  std::int32_t const here = static_cast<std::int32_t>(min(p.chunk + begin, p.slots) - begin);
+  std::int32_t const part = (p.chunk + threads - 1) / threads * 32;
+  std::int32_t const w0 = min(warp * part, here), w1 = min(w0 + part, here);
   std::int32_t *const mine = cursor + warp * experts;
-  for (std::int64_t s = w0 + lane; s < w1; s += 32) {
-    std::int32_t const e = local_expert<Id>(p, s);
+  for (int e = lane; e < experts; e += 32) mine[e] = 0;
+  if (gridDim.x > 1) {
+    for (int e = tid; e < 2 * experts; e += threads) total[e] = 0;
+  }
+  __syncwarp();
+  for (std::int32_t s = w0 + lane; s < w1; s += 32) {
+    std::int32_t const e = local_expert<Id>(p, begin + s);
+    local[s] = static_cast<std::int16_t>(e);
     if (e >= 0) atomicAdd(&mine[e], 1);
   }
   // The histograms of every chunk are complete past this point.
@@ -96,10 +109,11 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_par
 
   // total[e] = slots of e anywhere, start[e] = slots of e in earlier chunks.
   if (gridDim.x > 1) {
-    int const lanes = kMoeSortThreads / experts;  // threads that share an expert's column
+    int const lanes = threads / experts;  // threads that share an expert's column
     if (tid < lanes * experts) {
       int const e = tid % experts, first = tid / experts;
       std::int32_t all = 0, before = 0;
+#pragma unroll 8
       for (int c = first; c < static_cast<int>(gridDim.x); c += lanes) {
         std::int32_t const n = p.histogram[static_cast<std::int64_t>(c) * experts + e];
         all += n;
@@ -108,19 +122,23 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_par
       if (all) atomicAdd(&total[e], all);
       if (before) atomicAdd(&start[e], before);
     }
-  } else {
-    for (int e = tid; e < experts; e += kMoeSortThreads) {
-      std::int32_t all = 0;
-#pragma unroll 8
-      for (int w = 0; w < kMoeSortWarps; ++w) all += cursor[w * experts + e];
-      total[e] = all;
-    }
+    __syncthreads();
   }
-  __syncthreads();
 
-  // Exclusive scan of the padded counts (one thread per expert).
-  std::int32_t const count = tid < experts ? total[tid] : 0;
-  std::int32_t const before = tid < experts ? start[tid] : 0;
+  // One thread per expert: its rows of each warp, and an exclusive scan of the
+  // padded counts.
+  std::int32_t count = 0, before = 0;
+  if (tid < experts) {
+    std::int32_t sum = 0;
+#pragma unroll 8
+    for (int w = 0; w < warps; ++w) {
+      std::int32_t const n = cursor[w * experts + tid];
+      cursor[w * experts + tid] = sum;
+      sum += n;
+    }
+    count = gridDim.x > 1 ? total[tid] : sum;
+    before = gridDim.x > 1 ? start[tid] : 0;
+  }
   std::int32_t const padded = (count + p.align - 1) / p.align * p.align;
   std::int32_t sum = padded;
 #pragma unroll
@@ -130,54 +148,43 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_par
   }
   if (lane == 31) warp_sums[warp] = sum;
   __syncthreads();
-  if (warp == 0) {
-    std::int32_t v = warp_sums[lane];
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      std::int32_t const up = __shfl_up_sync(0xffffffffu, v, d);
-      if (lane >= d) v += up;
-    }
-    warp_sums[lane] = v;
+  std::int32_t offset = sum - padded, used = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w < warp) offset += warp_sums[w];
+    used += warp_sums[w];
   }
-  __syncthreads();
-  std::int32_t const offset = sum - padded + (warp > 0 ? warp_sums[warp - 1] : 0);
-  std::int32_t const used = warp_sums[kMoeSortWarps - 1];
   if (tid < experts) {
-    std::int32_t next = offset + before;
-#pragma unroll 8
-    for (int w = 0; w < kMoeSortWarps; ++w) {
-      std::int32_t const n = cursor[w * experts + tid];
-      cursor[w * experts + tid] = next;
-      next += n;
-    }
+    total[tid] = offset + count;      // first row of the padding
+    start[tid] = offset + before;     // first row of this chunk's slots
     if (blockIdx.x == 0) {
       p.counts[tid] = count;
       p.offsets[tid] = offset;
       if (tid == experts - 1) p.offsets[experts] = used;
     }
-    // Padding rows of the experts of this CTA's share.
-    if (tid % gridDim.x == blockIdx.x) {
-      for (std::int32_t r = offset + count; r < offset + padded; ++r) p.slot_of_row[r] = -1;
-    }
-  }
-  for (std::int64_t r = used + static_cast<std::int64_t>(blockIdx.x) * kMoeSortThreads + tid;
-       r < p.rows; r += static_cast<std::int64_t>(gridDim.x) * kMoeSortThreads) {
-    p.slot_of_row[r] = -1;
   }
   __syncthreads();
-
-  for (std::int64_t s0 = w0; s0 < w1; s0 += 32) {
-    std::int64_t const s = s0 + lane;
-    bool const in = s < w1;
-    std::int32_t const e = in ? local_expert<Id>(p, s) : -1;
+  for (std::int32_t s0 = w0; s0 < w1; s0 += 32) {
+    std::int32_t const s = s0 + lane;
+    std::int32_t const e = s < w1 ? local[s] : -1;
     std::uint32_t const same = __match_any_sync(0xffffffffu, e);
     std::int32_t row = -1;
-    if (e >= 0) row = mine[e] + __popc(same & ((1u << lane) - 1u));
+    if (e >= 0) row = start[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
     if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
     __syncwarp();
-    if (in) p.row_of_slot[s] = row;
-    if (row >= 0) p.slot_of_row[row] = static_cast<std::int32_t>(s);
+    if (s < w1) p.row_of_slot[begin + s] = row;
+    if (row >= 0) p.slot_of_row[row] = static_cast<std::int32_t>(begin + s);
+  }
+  // Padding: a warp per expert of this CTA's share, then the rows behind.
+  for (int e = warp * gridDim.x + blockIdx.x; e < experts; e += warps * gridDim.x) {
+    std::int32_t const first = total[e];
+    for (std::int32_t r = first + lane; r < (first + p.align - 1) / p.align * p.align; r += 32) {
+      p.slot_of_row[r] = -1;
+    }
+  }
+  for (std::int64_t r = used + static_cast<std::int64_t>(blockIdx.x) * threads + tid; r < p.rows;
+       r += static_cast<std::int64_t>(gridDim.x) * threads) {
+    p.slot_of_row[r] = -1;
   }
 }
 

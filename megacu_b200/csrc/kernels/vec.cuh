@@ -38,6 +38,29 @@ __device__ __forceinline__ uint4 load_once(void const *p) {
   return v;
 }
 
+// 32 bytes at a time (addresses multiples of 32): a lane's whole sector in one
+// access, so that neighbouring lanes do not each touch half of one twice.
+struct alignas(32) bytes32 {
+  std::uint32_t w[8];
+};
+
+__device__ __forceinline__ bytes32 load32_once(void const *p) {
+  bytes32 v;
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]),
+                 "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store32(void *p, bytes32 const &v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               :: "l"(p), "r"(v.w[0]), "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]),
+                  "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+               : "memory");
+}
+
 template <class T, int N>
 struct alignas(sizeof(T) * N) vec {
   T v[N];

@@ -19,16 +19,17 @@ constexpr std::int64_t kMaxSlots = 1ll << 30;
 constexpr std::int32_t kMaxAlign = 1024;
 constexpr int kMaxDevices = 64;
 
-// One CTA sorts up to this many slots; more are sorted in chunks, counted by
-// one launch and placed by a second.
+// One CTA sorts up to this many slots in one launch; more are sorted in
+// chunks, counted by one launch and placed by a second.
 constexpr std::int64_t kSingleCtaSlots = 8192;
 constexpr std::int64_t kMinChunk = 2048;
-constexpr std::int64_t kMaxChunks = 128;
+constexpr std::int64_t kChunks = 128;  // CTAs wanted, about one per SM
+static_assert(kSingleCtaSlots <= kMoeMaxChunk, "a chunk's local experts are kept on chip");
 
 std::int32_t chunk_of(std::int64_t slots) {
   if (slots <= kSingleCtaSlots) return static_cast<std::int32_t>(std::max<std::int64_t>(slots, 1));
-  std::int64_t const even = (slots + kMaxChunks - 1) / kMaxChunks;
-  std::int64_t const chunk = std::max(even, kMinChunk);
+  std::int64_t const even = (slots + kChunks - 1) / kChunks;
+  std::int64_t const chunk = std::clamp<std::int64_t>(even, kMinChunk, kMoeMaxChunk);
   return static_cast<std::int32_t>((chunk + kMoeSortThreads - 1) / kMoeSortThreads *
                                    kMoeSortThreads);
 }
@@ -91,17 +92,20 @@ cudaError_t launch_sort(moe_sort_params const &prm, std::int64_t chunks, int dev
                         cudaStream_t stream) {
   static std::atomic<bool> configured[kMaxDevices] = {};
   bool const known = device >= 0 && device < kMaxDevices;
-  int const place_smem = (kMoeSortWarps + 2) * prm.experts * 4;
+  // A thread per slot and per expert, as far as they go.
+  std::int64_t const wanted = std::max<std::int64_t>(prm.chunk, prm.experts);
+  int const threads =
+      static_cast<int>(std::min<std::int64_t>((wanted + 31) / 32 * 32, kMoeSortThreads));
   if (!known || !configured[device].load(std::memory_order_acquire)) {
     cudaError_t const e =
         cudaFuncSetAttribute(moe_place_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (kMoeSortWarps + 2) * kMoeMaxExperts * 4);
+                             moe_place_smem(kMoeSortThreads / 32, kMoeMaxExperts, kMoeMaxChunk));
     if (e != cudaSuccess) return e;
     if (known) configured[device].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(chunks));
-  cfg.blockDim = dim3(kMoeSortThreads);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   if (chunks > 1) {
@@ -114,7 +118,8 @@ cudaError_t launch_sort(moe_sort_params const &prm, std::int64_t chunks, int dev
     cfg.attrs = attr;
     cfg.numAttrs = 1;
   }
-  cfg.dynamicSmemBytes = static_cast<std::size_t>(place_smem);
+  cfg.dynamicSmemBytes =
+      static_cast<std::size_t>(moe_place_smem(threads / 32, prm.experts, prm.chunk));
   return cudaLaunchKernelEx(&cfg, moe_place_kernel<Id>, prm);
 }
 
