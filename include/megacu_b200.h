@@ -481,7 +481,7 @@ megacu_status megacu_b200_moe_sizes(const megacu_moe_problem *problem, int64_t s
  * row of expert e, offsets[experts] the rows in use, padding included),
  * row_of_slot [tokens, topk] (-1: not here) and slot_of_row [sizes[0]] (-1:
  * padding and rows behind the last). Rows of an expert are in slot order.
- * workspace: sizes[1] bytes, need not be initialised, nothing is kept in it
+ * workspace: sizes[1] bytes, 16-byte aligned, need not be initialised, nothing is kept in it
  * between calls; one per concurrent call.
  */
 megacu_status megacu_cuda_moe_sort(megacu_driver_view driver, const void *expert_ids,

@@ -18,7 +18,6 @@ per-site detail number.
 from __future__ import annotations
 
 import ctypes
-import functools
 import weakref
 from dataclasses import dataclass
 from typing import Callable, Optional, Sequence
@@ -513,42 +512,49 @@ class _CProblem:
         return self.__dict__["_ref"]
 
 
-@functools.lru_cache(None)
-def _types() -> dict:
-    """torch types by their element type code; "u8", "i32" and "i64" too."""
-    import torch
-    return {_capi.DTYPE_F16: torch.float16, _capi.DTYPE_BF16: torch.bfloat16,
-            _capi.DTYPE_F32: torch.float32, "u8": torch.uint8, "i32": torch.int32,
-            "i64": torch.int64}
+class _Types(dict):
+    """torch types by their element type code; "u8", "i32" and "i64" too.
+    Filled on first use (importing this package does not import torch)."""
+
+    def __missing__(self, key):
+        import torch
+        self.update({_capi.DTYPE_F16: torch.float16, _capi.DTYPE_BF16: torch.bfloat16,
+                     _capi.DTYPE_F32: torch.float32, "u8": torch.uint8, "i32": torch.int32,
+                     "i64": torch.int64})
+        return self[key]
 
 
-def _buffer(x, name: str, elements: int, dtype, device: int) -> Optional[int]:
-    """The address of ``x``: a contiguous tensor on ``device`` of the type with
-    code ``dtype`` and at least ``elements`` elements. None and raw addresses
-    (int) are taken as they are."""
+_TYPES = _Types()
+
+
+def _buffer(x, name: str, elements: int, dtype, device: Optional[int]) -> Optional[int]:
+    """The address of ``x``: a contiguous tensor on ``device`` (None: anywhere,
+    for calls that only validate) of the type with code ``dtype`` and at least
+    ``elements`` elements. None and raw addresses (int) are taken as they are."""
     if x is None or x.__class__ is int:
         return x
-    if x.dtype is not _types()[dtype]:
+    if (x.dtype is _TYPES[dtype] and x.numel() >= elements and x.is_contiguous()
+            and (device is None or x.get_device() == device)):
+        return x.data_ptr()
+    if x.dtype is not _TYPES[dtype]:
         raise ValueError(f"{name} has dtype {x.dtype}")
     if x.numel() < elements or not x.is_contiguous():
         raise ValueError(f"{name} must be contiguous with at least {elements} elements")
-    if x.get_device() not in (device, -1):  # host tensors only pass a validate-only call
-        raise ValueError(f"{name} is on {x.device}, the call on device {device}")
-    return x.data_ptr()
+    raise ValueError(f"{name} is on {x.device}, the call on device {device}")
 
 
 def _matrix(x, name: str, rows: int, cols: int, stride: int, dtype: int,
-            device: int) -> Optional[int]:
+            device: Optional[int]) -> Optional[int]:
     """The address of the row-major matrix ``x``, whose rows are ``stride``
     elements apart (0: dense)."""
     if stride == 0 or stride == cols or x is None or x.__class__ is int:
         return _buffer(x, name, rows * cols, dtype, device)
-    if x.dtype is not _types()[dtype]:
+    if x.dtype is not _TYPES[dtype]:
         raise ValueError(f"{name} has dtype {x.dtype}")
     if (x.dim() != 2 or x.shape[0] < rows or x.shape[1] < cols or x.stride(1) != 1
             or (rows > 1 and x.stride(0) != stride)):
         raise ValueError(f"{name} must be [{rows}, {cols}] with rows {stride} elements apart")
-    if x.get_device() not in (device, -1):
+    if device is not None and x.get_device() != device:
         raise ValueError(f"{name} is on {x.device}, the call on device {device}")
     return x.data_ptr()
 
@@ -608,26 +614,27 @@ def moe_sort(expert_ids, *, counts, offsets, row_of_slot, slot_of_row, problem: 
     [experts], ``offsets`` [experts + 1], ``row_of_slot`` [tokens, topk] and
     ``slot_of_row`` [moe_rows(problem)]; -1 marks slots whose expert is
     elsewhere and rows without a slot. ``workspace``: moe_workspace_bytes()."""
+    where = None if stream is None else device
     rows, need = _moe_sizes(problem)
     slots, experts = problem.tokens * problem.topk, problem.experts
-    wide = getattr(expert_ids, "dtype", None) is _types()["i64"]
+    wide = getattr(expert_ids, "dtype", None) is _TYPES["i64"]
     check(lib().megacu_cuda_moe_sort(
         _launch_view(stream, device, None),
-        _buffer(expert_ids, "expert_ids", slots, "i64" if wide else "i32", device),
-        _buffer(counts, "counts", experts, "i32", device),
-        _buffer(offsets, "offsets", experts + 1, "i32", device),
-        _buffer(row_of_slot, "row_of_slot", slots, "i32", device),
-        _buffer(slot_of_row, "slot_of_row", rows, "i32", device),
-        _buffer(workspace, "workspace", need, "u8", device) if need else None,
+        _buffer(expert_ids, "expert_ids", slots, "i64" if wide else "i32", where),
+        _buffer(counts, "counts", experts, "i32", where),
+        _buffer(offsets, "offsets", experts + 1, "i32", where),
+        _buffer(row_of_slot, "row_of_slot", slots, "i32", where),
+        _buffer(slot_of_row, "slot_of_row", rows, "i32", where),
+        _buffer(workspace, "workspace", need, "u8", where) if need else None,
         problem._wide_ids() if wide else problem._pointer()))
 
 
-def _token_rows(x, name: str, p: MoeProblem, device: int) -> Optional[int]:
-    return _matrix(x, name, p.tokens, p.hidden, p.token_stride, p.dtype, device)
+def _token_rows(x, name: str, p: MoeProblem, where: Optional[int]) -> Optional[int]:
+    return _matrix(x, name, p.tokens, p.hidden, p.token_stride, p.dtype, where)
 
 
-def _expert_rows(x, name: str, p: MoeProblem, device: int) -> Optional[int]:
-    return _matrix(x, name, moe_rows(p), p.hidden, p.row_stride, p.dtype, device)
+def _expert_rows(x, name: str, p: MoeProblem, where: Optional[int]) -> Optional[int]:
+    return _matrix(x, name, moe_rows(p), p.hidden, p.row_stride, p.dtype, where)
 
 
 def moe_dispatch(x, rows, *, row_of_slot, problem: MoeProblem, stream=None,
@@ -635,11 +642,11 @@ def moe_dispatch(x, rows, *, row_of_slot, problem: MoeProblem, stream=None,
     """rows[row_of_slot[t, j]] = x[t] (async); other rows are left as they
     were. The gradient is :func:`moe_combine` of the rows' gradient without
     weights."""
-    p = problem
+    p, where = problem, None if stream is None else device
     check(lib().megacu_cuda_moe_dispatch(
-        _launch_view(stream, device, None), _token_rows(x, "x", p, device),
-        _buffer(row_of_slot, "row_of_slot", p.tokens * p.topk, "i32", device),
-        _expert_rows(rows, "rows", p, device), p._pointer()))
+        _launch_view(stream, device, None), _token_rows(x, "x", p, where),
+        _buffer(row_of_slot, "row_of_slot", p.tokens * p.topk, "i32", where),
+        _expert_rows(rows, "rows", p, where), p._pointer()))
 
 
 def moe_combine(rows, y, *, row_of_slot, problem: MoeProblem, weights=None, stream=None,
@@ -647,10 +654,11 @@ def moe_combine(rows, y, *, row_of_slot, problem: MoeProblem, weights=None, stre
     """y[t] = sum over j of weights[t, j] * rows[row_of_slot[t, j]] (async), fp32
     sums in the order of j, one rounding; ``weights`` fp32, None = 1."""
     p, slots = problem, problem.tokens * problem.topk
+    where = None if stream is None else device
     check(lib().megacu_cuda_moe_combine(
-        _launch_view(stream, device, None), _expert_rows(rows, "rows", p, device),
-        _buffer(weights, "weights", slots, _capi.DTYPE_F32, device),
-        _buffer(row_of_slot, "row_of_slot", slots, "i32", device), _token_rows(y, "y", p, device),
+        _launch_view(stream, device, None), _expert_rows(rows, "rows", p, where),
+        _buffer(weights, "weights", slots, _capi.DTYPE_F32, where),
+        _buffer(row_of_slot, "row_of_slot", slots, "i32", where), _token_rows(y, "y", p, where),
         p._pointer()))
 
 
@@ -660,13 +668,14 @@ def moe_combine_grad(dy, rows, drows, dweights, *, weights, row_of_slot, problem
     dy at the rows of each token (other rows are left as they were), dweights
     [tokens, topk] fp32 = <dy[t], rows[...]>, 0 for a slot without a row."""
     p, slots = problem, problem.tokens * problem.topk
+    where = None if stream is None else device
     check(lib().megacu_cuda_moe_combine_grad(
-        _launch_view(stream, device, None), _token_rows(dy, "dy", p, device),
-        _expert_rows(rows, "rows", p, device),
-        _buffer(weights, "weights", slots, _capi.DTYPE_F32, device),
-        _buffer(row_of_slot, "row_of_slot", slots, "i32", device),
-        _expert_rows(drows, "drows", p, device),
-        _buffer(dweights, "dweights", slots, _capi.DTYPE_F32, device),
+        _launch_view(stream, device, None), _token_rows(dy, "dy", p, where),
+        _expert_rows(rows, "rows", p, where),
+        _buffer(weights, "weights", slots, _capi.DTYPE_F32, where),
+        _buffer(row_of_slot, "row_of_slot", slots, "i32", where),
+        _expert_rows(drows, "drows", p, where),
+        _buffer(dweights, "dweights", slots, _capi.DTYPE_F32, where),
         p._pointer()))
 
 
@@ -708,12 +717,12 @@ def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, topk:
     negative are left as they were; with ``topk`` too, row r is taken from
     x[slot_of_row[r] // topk] (``x_rows``: the rows of ``x``, needed only when
     ``x`` is a raw address)."""
-    p = problem
+    p, where = problem, None if stream is None else device
     nbytes, sbytes = fp4_sizes(p)
     if topk:
         if x_rows == 0 and x is not None and x.__class__ is not int:
             x_rows = x.shape[0]
-        x_ptr = _matrix(x, "x", x_rows, p.cols, p.stride, p.dtype, device)
+        x_ptr = _matrix(x, "x", x_rows, p.cols, p.stride, p.dtype, where)
         key = (topk, x_rows)
         gathered = p.__dict__.get("_gathered")
         if gathered is None or gathered[0] is not p.to_c() or gathered[1] != key:
@@ -721,25 +730,25 @@ def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, topk:
         pointer = gathered[2]
     else:
         rows, cols = (p.cols, p.rows) if p.transpose else (p.rows, p.cols)
-        x_ptr = _matrix(x, "x", rows, cols, p.stride, p.dtype, device)
+        x_ptr = _matrix(x, "x", rows, cols, p.stride, p.dtype, where)
         pointer = p._pointer()
     check(lib().megacu_cuda_fp4_quantize(
         _launch_view(stream, device, None), x_ptr,
-        _buffer(slot_of_row, "slot_of_row", p.rows, "i32", device),
-        _buffer(data, "data", nbytes, "u8", device),
-        _buffer(scales, "scales", sbytes, "u8", device), pointer))
+        _buffer(slot_of_row, "slot_of_row", p.rows, "i32", where),
+        _buffer(data, "data", nbytes, "u8", where),
+        _buffer(scales, "scales", sbytes, "u8", where), pointer))
 
 
 def fp4_dequantize(data, scales, out, *, problem: Fp4Matrix, stream=None,
                    device: int = 0) -> None:
     """The values of a quantised matrix (async): out [rows, cols] = element *
     scale / problem.scale, rounded once to problem.dtype."""
-    p = problem
+    p, where = problem, None if stream is None else device
     nbytes, sbytes = fp4_sizes(p)
     check(lib().megacu_cuda_fp4_dequantize(
-        _launch_view(stream, device, None), _buffer(data, "data", nbytes, "u8", device),
-        _buffer(scales, "scales", sbytes, "u8", device),
-        _matrix(out, "out", p.rows, p.cols, p.stride, p.dtype, device), p._pointer()))
+        _launch_view(stream, device, None), _buffer(data, "data", nbytes, "u8", where),
+        _buffer(scales, "scales", sbytes, "u8", where),
+        _matrix(out, "out", p.rows, p.cols, p.stride, p.dtype, where), p._pointer()))
 
 
 @dataclass
@@ -773,25 +782,25 @@ def fp4_events_bytes() -> int:
     return out.value
 
 
-def _operand(data, scales, name: str, matrices: int, rows: int, p: Fp4Gemm, device: int):
+def _operand(data, scales, name: str, matrices: int, rows: int, p: Fp4Gemm, where: Optional[int]):
     """Addresses of a quantised operand of ``matrices`` matrices [rows, k]."""
     tiles = -(-p.k // (128 if p.format == _capi.FP4_MX else 64))
-    return (_buffer(data, name, matrices * rows * (p.k // 2), "u8", device),
-            _buffer(scales, name, matrices * -(-rows // 128) * tiles * 512, "u8", device))
+    return (_buffer(data, name, matrices * rows * (p.k // 2), "u8", where),
+            _buffer(scales, name, matrices * -(-rows // 128) * tiles * 512, "u8", where))
 
 
 def _product(fn, weights, a, a_scales, out, offsets, counts, alphas, events, p: Fp4Gemm, stream,
              device: int) -> None:
-    experts = max(p.experts, 1)
-    args = [*_operand(a, a_scales, "a", 1, p.m, p, device)]
+    experts, where = max(p.experts, 1), None if stream is None else device
+    args = [*_operand(a, a_scales, "a", 1, p.m, p, where)]
     for name, data, scales in weights:
-        args += _operand(data, scales, name, experts, p.n, p, device)
+        args += _operand(data, scales, name, experts, p.n, p, where)
     check(fn(_launch_view(stream, device, None), *args,
-             _buffer(offsets, "offsets", p.experts + 1, "i32", device),
-             _buffer(counts, "counts", p.experts, "i32", device),
-             _buffer(alphas, "alphas", p.experts, _capi.DTYPE_F32, device),
-             _matrix(out, "out", p.m, p.n, p.out_stride, p.out_dtype, device),
-             _buffer(events, "events", 256, "u8", device),
+             _buffer(offsets, "offsets", p.experts + 1, "i32", where),
+             _buffer(counts, "counts", p.experts, "i32", where),
+             _buffer(alphas, "alphas", p.experts, _capi.DTYPE_F32, where),
+             _matrix(out, "out", p.m, p.n, p.out_stride, p.out_dtype, where),
+             _buffer(events, "events", 256, "u8", where),
              p._pointer()))
 
 

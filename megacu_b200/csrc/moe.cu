@@ -22,8 +22,8 @@ constexpr int kMaxDevices = 64;
 // One CTA sorts up to this many slots in one launch; more are sorted in
 // chunks, counted by one launch and placed by a second.
 constexpr std::int64_t kSingleCtaSlots = 8192;
-constexpr std::int64_t kMinChunk = 2048;
-constexpr std::int64_t kChunks = 128;  // CTAs wanted, about one per SM
+constexpr std::int64_t kMinChunk = 4096;
+constexpr std::int64_t kChunks = 64;  // CTAs wanted; each reads every chunk's histogram
 static_assert(kSingleCtaSlots <= kMoeMaxChunk, "a chunk's local experts are kept on chip");
 
 std::int32_t chunk_of(std::int64_t slots) {
@@ -214,7 +214,7 @@ extern "C" megacu_status megacu_b200_moe_sizes(megacu_moe_problem const *problem
   if (sizes == nullptr) return fail(MEGACU_INVALID_ARGUMENT, 2, "missing output");
   std::int64_t const chunks = chunks_of(problem->tokens * problem->topk);
   sizes[0] = capacity(*problem);
-  sizes[1] = chunks > 1 ? chunks * problem->experts * 4 : 0;
+  sizes[1] = chunks > 1 ? (chunks + 7) / 8 * 16 * problem->experts : 0;
   return ok_status();
 }
 
@@ -237,8 +237,8 @@ extern "C" megacu_status megacu_cuda_moe_sort(megacu_driver_view driver, void co
   }
   if (!aligned_to(expert_ids, p.id_bytes == 8 ? 8 : 4) || !aligned_to(counts, 4) ||
       !aligned_to(offsets, 4) || !aligned_to(row_of_slot, 4) || !aligned_to(slot_of_row, 4) ||
-      !aligned_to(workspace, 4)) {
-    return fail(MEGACU_INVALID_ARGUMENT, 21, "indices must be aligned to their element");
+      !aligned_to(workspace, 16)) {
+    return fail(MEGACU_INVALID_ARGUMENT, 21, "indices must be aligned to their element, the workspace to 16 bytes");
   }
   if (driver.launch.stream == nullptr) return ok_status();
   int const device = driver.launch.device_ordinal;
@@ -252,7 +252,8 @@ extern "C" megacu_status megacu_cuda_moe_sort(megacu_driver_view driver, void co
   prm.experts = p.experts;
   prm.first = p.first_expert;
   prm.align = p.align;
-  prm.histogram = static_cast<std::int32_t *>(workspace);
+  prm.histogram = static_cast<std::uint16_t *>(workspace);
+  prm.chunks_pad = static_cast<std::int32_t>((chunks + 7) / 8 * 8);
   prm.counts = static_cast<std::int32_t *>(counts);
   prm.offsets = static_cast<std::int32_t *>(offsets);
   prm.row_of_slot = static_cast<std::int32_t *>(row_of_slot);
