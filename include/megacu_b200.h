@@ -575,8 +575,9 @@ typedef struct megacu_fp4_gemm_problem {
   int32_t format;      /* enum megacu_fp4_format, of both operands */
   int32_t out_dtype;   /* f16, bf16 or f32 */
   int32_t experts;     /* 0: one B; else B is [experts, n, k], at most 1024 */
-  int32_t tile_n;      /* 0 = auto; else 128 or 256 accumulator columns per tile */
-  int32_t split;       /* 0 = auto; else 1, 2, 4 or 8 CTAs share a tile's K */
+  int32_t tile_n;      /* 0 = auto; else 64, 128 or 256 accumulator columns per tile */
+  int32_t split;       /* 0 = auto; else 1, 2, 4 or 8 CTAs share a tile's K (at most
+                          tile_n / 16 and ceil(k / 256)) */
   float alpha;         /* 1 / (g_a * g_b) undoes the operands' scales */
   uint64_t timeout_ns; /* bound of every wait inside the launch; 0 = 4 s */
 } megacu_fp4_gemm_problem;

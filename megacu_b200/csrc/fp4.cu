@@ -129,31 +129,38 @@ struct fp4_plan {
   std::int64_t m_tiles = 0, n_tiles = 0;
 };
 
-// Tile width and K split with the least work on the busiest SM, in units of
-// one 128 x 128 x 256 block of MMAs, which costs about as much as its loads;
-// a tile adds about 3 units of start-up and epilogue, a split 4 more for the
-// exchange.
+// Tile width and K split with the least time on the busiest SM, in us, fitted
+// to measured calls on a B200 (16 to 128 rows, N 8192, K 256 / 3584 / 14336):
+// a call's start-up and end, a k-block of 256 at each width (what an SM can
+// load in a time that its MMAs do not exceed), a further tile on the same SM,
+// and the exchange of a split, which grows with the tile's accumulators.
+// 16 x 8192 x 3584: tile_n 64 takes 7.3 us, 128 7.2, 256 9.4, 128 split in two
+// 7.7, 256 split in four 8.7.
 megacu_status make_plan(megacu_fp4_gemm_problem const &p, bool swiglu, int sms, fp4_plan &out) {
   std::int64_t const k_blocks = ceil_div(p.k, kFp4BlockK);
-  std::int64_t best = -1;
-  for (int tile_n : {256, 128}) {
+  double best = -1.0;
+  for (int tile_n : {256, 128, 64}) {
     if ((swiglu && tile_n != 256) || (p.tile_n != 0 && p.tile_n != tile_n)) continue;
+    double const start = tile_n == 256 ? 4.6 : tile_n == 128 ? 3.8 : 3.6;
+    double const per_block = tile_n == 256 ? 0.40 : tile_n == 128 ? 0.25 : 0.21;
     for (int split : {1, 2, 4, 8}) {
-      if (split > k_blocks || (p.split != 0 && p.split != split)) continue;
+      if (split > k_blocks || 16 * split > tile_n || (p.split != 0 && p.split != split)) continue;
       std::int64_t const m_tiles = ceil_div(p.m, kFp4BlockM);
       std::int64_t const n_tiles = ceil_div(p.n, swiglu ? tile_n / 2 : tile_n);
-      std::int64_t const waves = ceil_div(m_tiles * n_tiles * split, sms);
-      std::int64_t const per_tile =
-          ceil_div(k_blocks, split) * (tile_n / 128) + 3 + (split > 1 ? 4 : 0);
-      std::int64_t const cost = waves * per_tile;
-      if (best < 0 || cost < best) {
+      std::int64_t const waves = std::max<std::int64_t>(ceil_div(m_tiles * n_tiles * split, sms), 1);
+      double const rows = static_cast<double>(std::min<std::int64_t>(p.m, kFp4BlockM));
+      double const exchange = split > 1 ? 1.5 + 0.035 * rows * tile_n / 256 : 0.0;
+      double const cost = start + 0.6 * static_cast<double>(waves - 1) +
+                          static_cast<double>(waves) *
+                              (per_block * static_cast<double>(ceil_div(k_blocks, split)) + exchange);
+      if (best < 0.0 || cost < best) {
         best = cost;
         out = {tile_n, split, false, m_tiles, n_tiles};
       }
     }
   }
+  if (best < 0.0) return fail(MEGACU_UNSUPPORTED, 22, "tile_n or split not possible");
   out.pair = p.experts == 0 && out.tile_n == 256 && out.split == 1 && out.m_tiles > 1;
-  if (best < 0) return fail(MEGACU_UNSUPPORTED, 22, "tile_n or split not possible");
   if (out.m_tiles * out.n_tiles * out.split > (1 << 28)) {
     return fail(MEGACU_UNSUPPORTED, 22, "too many tiles");
   }
@@ -164,11 +171,11 @@ struct fp4_operands {
   void const *a, *a_scales, *b, *b_scales, *b2, *b2_scales;
 };
 
-template <bool kNv, bool kSwiglu, int BN, bool kPair>
+template <bool kNv, bool kSwiglu, int BN, bool kPair = false, int kRows = kFp4BlockM>
 cudaError_t launch_gemm(int device, int grid, cudaStream_t stream, fp4_maps const &maps,
                         fp4_gemm_params const &prm) {
-  constexpr auto kKernel = &fp4_gemm_kernel<kNv, kSwiglu, BN, kPair>;
-  constexpr int kSmem = fp4_config<kNv, BN, kPair>::smem_bytes;
+  constexpr auto kKernel = &fp4_gemm_kernel<kNv, kSwiglu, BN, kPair, kRows>;
+  constexpr int kSmem = fp4_config<kNv, BN, kPair, kRows>::smem_bytes;
   static std::atomic<bool> configured[kMaxDevices] = {};
   bool const known = device >= 0 && device < kMaxDevices;
   if (!known || !configured[device].load(std::memory_order_acquire)) {
@@ -211,13 +218,19 @@ cudaError_t launch_plan(fp4_plan const &plan, bool swiglu, int device, int grid,
                         cudaStream_t stream, fp4_maps const &maps, fp4_gemm_params const &prm) {
   if (swiglu) {
     return plan.pair ? launch_gemm<kNv, true, 256, true>(device, grid, stream, maps, prm)
-                     : launch_gemm<kNv, true, 256, false>(device, grid, stream, maps, prm);
+                     : launch_gemm<kNv, true, 256>(device, grid, stream, maps, prm);
   }
   if (plan.tile_n == 256) {
     return plan.pair ? launch_gemm<kNv, false, 256, true>(device, grid, stream, maps, prm)
-                     : launch_gemm<kNv, false, 256, false>(device, grid, stream, maps, prm);
+                     : launch_gemm<kNv, false, 256>(device, grid, stream, maps, prm);
   }
-  return launch_gemm<kNv, false, 128, false>(device, grid, stream, maps, prm);
+  if (plan.tile_n == 128) return launch_gemm<kNv, false, 128>(device, grid, stream, maps, prm);
+  // At most 32 rows: stages without the missing rows, so more of them (13 to
+  // 15 against 7 or 8, the weights of most K's whole tile in flight).
+  if (prm.experts == 0 && prm.rows <= kFp4SmallRows) {
+    return launch_gemm<kNv, false, 64, false, kFp4SmallRows>(device, grid, stream, maps, prm);
+  }
+  return launch_gemm<kNv, false, 64>(device, grid, stream, maps, prm);
 }
 
 megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &op,

@@ -82,16 +82,24 @@ struct fp4_gemm_params {
   unsigned long long timeout_ns;
 };
 
-template <bool kNv, int BN, bool kPair>
+// kRows: rows of A that a stage holds, 128, or 32 for products of at most 32
+// rows; the MMA still reads 128, whatever follows, into accumulators that are
+// never stored.
+template <bool kNv, int BN, bool kPair, int kRows>
 struct fp4_config {
   static constexpr int scale_tiles = kFp4BlockK / fp4_tile_cols(kNv);  // per row tile and stage
-  static constexpr int b_tiles = BN / 128;  // row tiles of B whose scales a CTA holds
-  static constexpr int a_bytes = kFp4BlockM * 128;
+  static constexpr int b_tiles = BN > 128 ? BN / 128 : 1;  // row tiles of B whose scales it holds
+  static constexpr int a_bytes = kRows * 128;
   static constexpr int b_bytes = BN * 128 / (kPair ? 2 : 1);
   static constexpr int sfa_bytes = scale_tiles * kScaleTileBytes;
   static constexpr int sfb_bytes = b_tiles * sfa_bytes;
   static constexpr int stage_bytes = a_bytes + b_bytes + sfa_bytes + sfb_bytes;
-  static constexpr int staging_bytes = kFp4EpilogueWarps * 1024;
+  // Bytes of a row that an epilogue warp stores at a time. 64 leave faster
+  // than 32 (a 2048 x 1792 SwiGLU's last tile 2.7 against 3.2 us) but their
+  // staging must not cost the fourth stage.
+  static constexpr int segment =
+      BN == 256 && (232448 - 1280 - kFp4EpilogueWarps * 2048) / stage_bytes >= 4 ? 64 : 32;
+  static constexpr int staging_bytes = kFp4EpilogueWarps * 32 * segment;
   static constexpr int overhead = 1024 + staging_bytes + 256;
   static constexpr int stages = (232448 - overhead) / stage_bytes;
   static constexpr int ring_bytes = stages * stage_bytes;
@@ -99,9 +107,11 @@ struct fp4_config {
   static constexpr int acc1 = BN == 256 ? 192 : BN;  // columns of the second accumulator
   static constexpr int sf_column = acc1 + BN;
   static constexpr int tmem_columns = 512;
-  static_assert(stages >= 4 && stages <= 8, "stage ring");
+  static_assert(stages >= 4 && stages <= 15, "stage ring and its barriers");
   static_assert(sf_column + scale_tiles * 4 * (1 + b_tiles) <= tmem_columns, "TMEM");
   static_assert(BN * 128 * 4 <= ring_bytes, "the split's exchange fits the ring");
+  static_assert(kFp4BlockM * 128 <= a_bytes + b_bytes + stages * (sfa_bytes + sfb_bytes),
+                "the last stage's 128 rows end inside the ring");
 };
 
 namespace ptx {
@@ -110,7 +120,8 @@ namespace ptx {
 // registers; in a branch on this predicate the compiler knows that one lane
 // runs and keeps the operands there. In a branch on `lane == 0` it moves each
 // into place first: 170 cycles per MMA and 62 per scale copy at issue, against
-// MMAs of 128 cycles (measured; 4096 x 8192 x 8192 MX: 156 -> 105 us).
+// MMAs of 128 cycles (measured; 4096 x 8192 x 8192 MX: 156 -> 105 us). The same
+// holds for TMA loads.
 __device__ __forceinline__ bool elect_one() {
   std::uint32_t elected;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
@@ -169,6 +180,33 @@ __device__ __forceinline__ void commit_fp4(std::uint64_t *bar) {
   } else {
     umma_commit(bar);
   }
+}
+
+// Shared memory by its own address space (the generic one costs more and
+// keeps the compiler from ordering these freely against global stores).
+__device__ __forceinline__ void st_shared_v4(std::uint32_t at, std::uint32_t a, std::uint32_t b,
+                                             std::uint32_t c, std::uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+               :: "r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared_v4(std::uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ std::uint32_t ld_shared_u32(std::uint32_t at) {
+  std::uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ std::uint32_t ld_shared_u16(std::uint32_t at) {
+  std::uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+  return v;
 }
 
 // Descriptor of a scale tile: no swizzle, 8-row groups 128 bytes apart.
@@ -265,54 +303,63 @@ struct fp4_rows_out {
 };
 
 // Stores kCount consecutive columns from `col` of a warp's 32 rows (lane = row
-// on entry), 32 bytes of each row at a time: turned through `stage` (1 KB, no
-// bank conflicts) so that two neighbouring lanes write a row's 32 bytes, or,
-// where the rows do not allow 16-byte stores, neighbouring lanes neighbouring
-// elements.
-template <bool kWide, int kCount>
-__device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uint8_t *stage,
+// on entry), kSegment bytes of each row at a time: turned through `stage` (no
+// bank conflicts) so that neighbouring lanes write a row's segment in 16-byte
+// pieces, or, where the rows do not allow 16-byte stores, its elements.
+template <bool kWide, int kSegment, int kCount>
+__device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uint32_t stage,
                                               float const (&v)[kCount], fp4_rows_out const &out,
                                               std::int32_t col) {
   using element = std::conditional_t<kWide, std::uint32_t, std::uint16_t>;
   constexpr int kSize = sizeof(element);
-  constexpr int kCols = 32 / kSize;
+  constexpr int kBytes = kCount * kSize < kSegment ? kCount * kSize : kSegment;
+  constexpr int kCols = kBytes / kSize;
+  constexpr std::uint32_t kPieces = kBytes / 16;
   std::uint32_t const lane = ptx::lane_id();
   auto slot = [stage](std::uint32_t r, std::uint32_t c) {
-    return stage + r * 32 + ((c ^ (r >> 2)) & 1u) * 16;
+    return stage + r * kBytes + ((c ^ (r * kPieces >> 3)) % kPieces) * 16;
   };
 #pragma unroll
   for (int u = 0; u < kCount / kCols; ++u) {
     std::int32_t const first = col + u * kCols;
     if (first >= p.n) break;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      uint4 q;
-      std::uint32_t *const w = &q.x;
+    for (std::uint32_t c = 0; c < kPieces; ++c) {
+      std::uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        int const e = u * kCols + c * (16 / kSize);
+        int const e = u * kCols + static_cast<int>(c) * (16 / kSize);
         w[i] = kWide ? __float_as_uint(v[(e + i) % kCount])
                      : pack16(p.out_dtype, v[(e + 2 * i) % kCount], v[(e + 2 * i + 1) % kCount]);
       }
-      *reinterpret_cast<uint4 *>(slot(lane, c)) = q;
+      ptx::st_shared_v4(slot(lane, c), w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
     std::uint8_t *const dst = out.base + static_cast<std::int64_t>(first) * kSize;
     if (p.vec_store && first + kCols <= p.n) {
+      uint4 q[kPieces];
 #pragma unroll
-      for (std::uint32_t r = lane / 2, h = 0; h < 2; ++h, r += 16) {
+      for (std::uint32_t h = 0; h < kPieces; ++h) {
+        q[h] = ptx::ld_shared_v4(slot(lane / kPieces + h * (32 / kPieces), lane % kPieces));
+      }
+#pragma unroll
+      for (std::uint32_t h = 0; h < kPieces; ++h) {
+        std::uint32_t const r = lane / kPieces + h * (32 / kPieces);
         if (static_cast<std::int32_t>(r) < out.rows) {
-          *reinterpret_cast<uint4 *>(dst + r * out.stride + lane % 2 * 16) =
-              *reinterpret_cast<uint4 const *>(slot(r, lane % 2));
+          *reinterpret_cast<uint4 *>(dst + r * out.stride + lane % kPieces * 16) = q[h];
         }
       }
     } else {
-      std::uint32_t const e = lane % kCols;
-      for (std::uint32_t r = lane / kCols; static_cast<std::int32_t>(r) < min(out.rows, 32);
-           r += 32 / kCols) {
-        if (first + static_cast<std::int32_t>(e) < p.n) {
-          *reinterpret_cast<element *>(dst + r * out.stride + e * kSize) =
-              *reinterpret_cast<element const *>(slot(r, e * kSize / 16) + e * kSize % 16);
+      // kCols lanes per row (16 or 32 of them: one column each; 8: a row's all).
+      std::uint32_t const e = lane % kCols, step = 32 / kCols;
+      if (first + static_cast<std::int32_t>(e) < p.n) {
+#pragma unroll 4
+        for (std::uint32_t r = lane / kCols; r < 32; r += step) {
+          if (static_cast<std::int32_t>(r) >= out.rows) break;
+          std::uint32_t const at = slot(r, e * kSize / 16) + e * kSize % 16;
+          element const x = kWide ? static_cast<element>(ptx::ld_shared_u32(at))
+                                  : static_cast<element>(ptx::ld_shared_u16(at));
+          *reinterpret_cast<element *>(dst + r * out.stride + e * kSize) = x;
         }
       }
     }
@@ -320,14 +367,14 @@ __device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uin
   }
 }
 
-template <int kCount>
-__device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uint8_t *stage,
+template <int kSegment, int kCount>
+__device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uint32_t stage,
                                               float const (&v)[kCount], fp4_rows_out const &out,
                                               std::int32_t col) {
   if (p.out_dtype == 3) {
-    store_columns<true, kCount>(p, stage, v, out, col);
+    store_columns<true, kSegment, kCount>(p, stage, v, out, col);
   } else {
-    store_columns<false, kCount>(p, stage, v, out, col);
+    store_columns<false, kSegment, kCount>(p, stage, v, out, col);
   }
 }
 
@@ -343,11 +390,11 @@ __device__ __forceinline__ float swiglu(float g, float u) {
 
 }  // namespace detail
 
-template <bool kNv, bool kSwiglu, int BN, bool kPair>
+template <bool kNv, bool kSwiglu, int BN, bool kPair, int kRows>
 __global__ void __launch_bounds__(kFp4Threads, 1)
     fp4_gemm_kernel(__grid_constant__ fp4_maps const maps,
                     __grid_constant__ fp4_gemm_params const p) {
-  using cfg = fp4_config<kNv, BN, kPair>;
+  using cfg = fp4_config<kNv, BN, kPair, kRows>;
   static_assert(!kSwiglu || BN == 256, "128 gate and 128 up columns");
   static_assert(!kPair || BN == 256, "pairs compute 256 x 256 tiles");
   constexpr std::uint32_t kStages = cfg::stages;
@@ -401,11 +448,11 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     load_place l;
     l.row = c.row * kFp4BlockM;
     detail::fp4_rows const rows = detail::locate_rows(p, l.row);
-    l.boxes = min(max((rows.valid + kFp4SmallRows - 1) / kFp4SmallRows, 1), 4);
+    l.boxes = min(max((rows.valid + kFp4SmallRows - 1) / kFp4SmallRows, 1), kRows / kFp4SmallRows);
     if constexpr (kPair) l.boxes = 4;  // both CTAs' bytes are counted by the leader
     l.a_tile = min(c.row, m_tiles - 1) * p.scale_tiles;  // a pair's second tile may not exist
     l.b_row = rows.expert * p.n + c.col * kActCols;
-    l.b_tile = (rows.expert * p.n_row_tiles + c.col * (kActCols / 128)) * p.scale_tiles;
+    l.b_tile = (rows.expert * p.n_row_tiles + c.col * kActCols / 128) * p.scale_tiles;
     return l;
   };
   auto load = [&](load_place const &l, std::int32_t kb, std::uint32_t stage) {
@@ -468,12 +515,12 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     ptx::fence_proxy_async_shared();
   };
   if (warp == 0) {
-    if (lane == 0) set_up_barriers();
+    if (ptx::elect_one()) set_up_barriers();
     __syncwarp();
     if (!kPair && unit0 < tiles) {
       load_place const l = place(unit0);
       issued = static_cast<std::uint32_t>(min(kb1 - kb0, static_cast<std::int32_t>(kStages)));
-      if (lane == 0) {
+      if (ptx::elect_one()) {
         for (std::uint32_t s = 0; s < issued; ++s) load(l, kb0 + static_cast<std::int32_t>(s), s);
       }
       __syncwarp();
@@ -507,7 +554,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
           break;
         }
         __syncwarp();
-        if (lane == 0) load(l, kb, stage);
+        if (ptx::elect_one()) load(l, kb, stage);
         __syncwarp();
         ++issued;
         if (++stage == kStages) {
@@ -544,6 +591,8 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       }
       ptx::tc_fence_after_sync();
       std::uint32_t const acc = tmem + (tile_index & 1u) * cfg::acc1;
+      // A tile of 64 columns uses half of a scale tile's four TMEM columns.
+      std::uint32_t const b_half = BN == 64 ? (locate(t).col & 1) * 2u : 0u;
       for (std::int32_t kb = kb0; kb < kb1; ++kb) {
         if (!ptx::mbar_wait_cluster(&full[stage], phase, abort_word, p.timeout_ns)) {
           if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 53);
@@ -575,7 +624,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
             std::uint32_t const ta = sf + (kNv ? j : j / 2) * 4 * (1 + cfg::b_tiles);
             ptx::umma_fp4<kNv, kPair>(
                 acc, a_desc0 + at + j * 2, b_desc0 + at + j * 2,
-                fp4_idesc<kNv>(kFp4BlockM * (kPair ? 2 : 1), BN, kNv ? 0 : j % 2 * 2), ta, ta + 4,
+                fp4_idesc<kNv>(kFp4BlockM * (kPair ? 2 : 1), BN, kNv ? 0 : j % 2 * 2), ta, ta + 4 + b_half,
                 kb > kb0 || j > 0);
           }
           ptx::commit_fp4<kPair>(&empty[stage]);
@@ -596,7 +645,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     // ---------------- epilogue ----------------
     std::int32_t const quarter = warp & 3;       // TMEM lanes [32 quarter, +32)
     std::int32_t const half = (warp - 2) / 4;    // chunks half, half + 2, ...
-    std::uint8_t *const stage = staging + (warp - 2) * 1024;
+    std::uint32_t const stage = ptx::smem_addr(staging + (warp - 2) * 32 * cfg::segment);
     std::uint32_t const lanes = static_cast<std::uint32_t>(quarter * 32) << 16;
     std::uint32_t const free_bar = kPair ? ptx::map_to_rank(acc_free, 0) : 0;
     std::uint32_t tile_index = 0;
@@ -656,7 +705,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
         if (BN == 256 && i == 0) release();
         if (i + 1 < kChunks / 2) fetch((chunk + 2) % kChunks);  // in flight during the stores
         std::int32_t const col = c.col * kActCols + chunk * 32;
-        if (out.rows > 0 && col < p.n) detail::store_columns(p, stage, v, out, col);
+        if (out.rows > 0 && col < p.n) detail::store_columns<cfg::segment>(p, stage, v, out, col);
       }
       ptx::tc_fence_before_sync();
     }
@@ -707,7 +756,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     __syncwarp();
     ptx::cluster_sync();
     if (out.rows > 0) {
-      std::uint8_t *const stage = staging + (warp - 2) * 1024;
+      std::uint32_t const stage = ptx::smem_addr(staging + (warp - 2) * 32 * cfg::segment);
       std::uint32_t const mine = (static_cast<std::uint32_t>(quarter * 32) + lane) * 16;
       for (std::int32_t c0 = half * 16; c0 < slice; c0 += 32) {
         std::int32_t const col = c.col * kActCols + rank * slice + c0;
@@ -733,7 +782,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
           v[e] = kSwiglu ? detail::swiglu(alpha * sum[0][e], alpha * sum[kParts - 1][e])
                          : alpha * sum[0][e];
         }
-        detail::store_columns(p, stage, v, out, col);
+        detail::store_columns<cfg::segment>(p, stage, v, out, col);
       }
     }
   }

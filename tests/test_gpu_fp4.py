@@ -252,7 +252,8 @@ def test_gemm(m, n, k, fmt):
     want, mag = ref.product(ref.values(*a, fmt), ref.values(*b, fmt), 0.375)
     ag, bg = _gpu(a), _gpu(b)
     for dtype, t in DTYPES.items():
-        for tile_n, split in ((0, 0), (128, 1), (256, 1), (128, 2), (256, 4), (128, 8), (256, 8)):
+        for tile_n, split in ((0, 0), (128, 1), (256, 1), (128, 2), (256, 4), (128, 8), (256, 8),
+                              (64, 1), (64, 2), (64, 4)):
             if split > -(-k // 256):
                 continue
             p = mb.Fp4Gemm(m, n, k, format=fmt, out_dtype=dtype, alpha=0.375, tile_n=tile_n,
@@ -269,11 +270,25 @@ def test_gemm_many_tiles_per_sm(fmt):
     m, n, k = 1500, 4300, 1312
     a, b = ref.random_operand(gen, m, k, fmt), ref.random_operand(gen, n, k, fmt)
     want, mag = ref.product(ref.values(*a, fmt), ref.values(*b, fmt))
-    for tile_n in (128, 256):
+    for tile_n in (64, 128, 256):
         p = mb.Fp4Gemm(m, n, k, format=fmt, out_dtype=mb.DTYPE_F32, tile_n=tile_n, split=1)
         out = torch.empty(m, n, device="cuda")
         _run(mb.fp4_gemm, *_gpu(a), *_gpu(b), out, problem=p)
         _assert_close(out.cpu(), want, k * 2.0 ** -23 * mag, torch.float32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 31, 32, 33])
+def test_gemm_few_rows_many_tiles(m, fmt):
+    """Several tiles per SM around the 32 rows that a small stage holds."""
+    gen = torch.Generator().manual_seed(m)
+    n, k = 12000, 800
+    a, b = ref.random_operand(gen, m, k, fmt), ref.random_operand(gen, n, k, fmt)
+    want, mag = ref.product(ref.values(*a, fmt), ref.values(*b, fmt))
+    out = torch.empty(m, n, device="cuda")
+    _run(mb.fp4_gemm, *_gpu(a), *_gpu(b), out, problem=mb.Fp4Gemm(
+        m, n, k, format=fmt, out_dtype=mb.DTYPE_F32, tile_n=64, split=1))
+    _assert_close(out.cpu(), want, k * 2.0 ** -23 * mag, torch.float32)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)

@@ -182,7 +182,7 @@ def _gemm(**kw):
     (dict(m=-1), (1, 1)), (dict(n=0), (1, 1)), (dict(k=0), (1, 1)), (dict(k=40), (1, 21)),
     (dict(format=3), (1, 1)), (dict(out_dtype=0), (2, 20)), (dict(out_stride=95), (1, 1)),
     (dict(experts=-1), (1, 1)), (dict(experts=1025), (2, 22)), (dict(experts=4, m=130), (2, 22)),
-    (dict(tile_n=64), (2, 22)), (dict(split=3), (2, 22)), (dict(split=2), (2, 22)),
+    (dict(tile_n=32), (2, 22)), (dict(tile_n=64, split=8, k=4096), (2, 22)), (dict(split=3), (2, 22)), (dict(split=2), (2, 22)),
     (dict(split=2, k=512), (0, 0)), (dict(m=1 << 31), (2, 22)), (dict(n=1 << 29, experts=4), (2, 22)),
     (dict(), (0, 0)), (dict(m=0), (0, 0)), (dict(experts=4), (0, 0)), (dict(m=1, n=1, k=32), (0, 0))])
 def test_products_refuse(bad, want):
