@@ -1,5 +1,5 @@
-// Groups of N elements of a row as 32-bit floats: one 16-byte access when the
-// rows allow it (N = 16 / sizeof(T)), single elements otherwise (N = 1).
+// Groups of N elements of a row as 32-bit floats: one access of 32 or 16 bytes
+// when the rows allow it, single elements otherwise (N = 1).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -69,7 +69,10 @@ struct alignas(sizeof(T) * N) vec {
 
 template <class T, int N>
 __device__ __forceinline__ vec<T, N> load_vec(T const *p) {
-  if constexpr (sizeof(T) * N == 16) {
+  if constexpr (sizeof(T) * N == 32) {
+    bytes32 const raw = load32_once(p);
+    return *reinterpret_cast<vec<T, N> const *>(&raw);
+  } else if constexpr (sizeof(T) * N == 16) {
     uint4 const raw = load_once(p);
     return *reinterpret_cast<vec<T, N> const *>(&raw);
   } else {
@@ -79,7 +82,11 @@ __device__ __forceinline__ vec<T, N> load_vec(T const *p) {
 
 template <class T, int N>
 __device__ __forceinline__ void store_vec(T *p, vec<T, N> const &v) {
-  *reinterpret_cast<vec<T, N> *>(p) = v;
+  if constexpr (sizeof(T) * N == 32) {
+    store32(p, *reinterpret_cast<bytes32 const *>(&v));
+  } else {
+    *reinterpret_cast<vec<T, N> *>(p) = v;
+  }
 }
 
 }  // namespace megacu_b200

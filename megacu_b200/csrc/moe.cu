@@ -137,8 +137,10 @@ template <class T, int N>
 void launch_rows(rows_op op, moe_rows_params const &prm, rows_buffers const &b,
                  cudaStream_t stream) {
   auto const grid = static_cast<unsigned>(prm.tokens);
-  int const vectors = (prm.hidden + N - 1) / N;
-  int const threads = std::min(256, (vectors + 31) / 32 * 32);
+  int const most = op == rows_op::dispatch  ? kDispatchThreads
+                   : op == rows_op::combine ? kCombineThreads
+                                            : kGradThreads;
+  int const threads = std::min(most, ((prm.hidden + N - 1) / N + 31) / 32 * 32);
   switch (op) {
     case rows_op::dispatch:
       moe_dispatch_kernel<T, N><<<grid, threads, 0, stream>>>(
@@ -156,10 +158,17 @@ void launch_rows(rows_op op, moe_rows_params const &prm, rows_buffers const &b,
   }
 }
 
+// The widest access, up to 32 bytes for the dispatch and 16 for the calls
+// that hold several rows, that every row's start and length allow.
 template <class T>
-void launch_rows_typed(rows_op op, moe_rows_params const &prm, rows_buffers const &b, bool vec,
+void launch_rows_typed(rows_op op, moe_rows_params const &prm, rows_buffers const &b, int bytes,
                        cudaStream_t stream) {
-  if (vec) {
+  if (bytes == 32 && op == rows_op::dispatch) {
+    moe_dispatch_kernel<T, 32 / sizeof(T)>
+        <<<static_cast<unsigned>(prm.tokens),
+           std::min<int>(kDispatchThreads, (prm.hidden * sizeof(T) / 32 + 31) / 32 * 32), 0,
+           stream>>>(prm, static_cast<T const *>(b.in), static_cast<T *>(b.out));
+  } else if (bytes >= 16) {
     launch_rows<T, 16 / sizeof(T)>(op, prm, b, stream);
   } else {
     launch_rows<T, 1>(op, prm, b, stream);
@@ -192,9 +201,12 @@ megacu_status run_rows(rows_op op, megacu_driver_view const &driver, rows_buffer
   prm.row_of_slot = row_of_slot;
   prm.rows = static_cast<std::uint32_t>(capacity(*p));
   int const size = element_size(p->dtype);
-  bool const vec = p->hidden * size % 16 == 0 && prm.token_stride * size % 16 == 0 &&
-                   prm.row_stride * size % 16 == 0 && aligned_to(buffers[0], 16) &&
-                   aligned_to(buffers[1], 16) && aligned_to(buffers[2], 16);
+  auto fits = [&](int n) {
+    return p->hidden * size % n == 0 && prm.token_stride * size % n == 0 &&
+           prm.row_stride * size % n == 0 && aligned_to(buffers[0], n) &&
+           aligned_to(buffers[1], n) && aligned_to(buffers[2], n);
+  };
+  int const vec = fits(32) ? 32 : fits(16) ? 16 : 0;
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
   switch (p->dtype) {
     case MEGACU_DTYPE_F16: launch_rows_typed<__half>(op, prm, b, vec, stream); break;
