@@ -34,26 +34,34 @@ MEGACU_FP4_HD constexpr int scale_byte(int row, int block) {
 
 #if defined(__CUDACC__)
 
-// Two floats to two e2m1 (round to nearest even, saturating), `lo` in the
-// lower nibble.
-__device__ __forceinline__ std::uint32_t e2m1x2(float lo, float hi) {
+// Eight floats to eight e2m1 (round to nearest even, saturating), f[0] in the
+// lowest nibble.
+__device__ __forceinline__ std::uint32_t e2m1x8(float const (&f)[8]) {
   std::uint32_t r;
-  asm("{\n\t.reg .b8 b;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\t"
-      "cvt.u32.u8 %0, b;\n\t}"
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(r)
-      : "f"(lo), "f"(hi));
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
   return r;
 }
 
-__device__ __forceinline__ __half2 from_e2m1x2(std::uint32_t byte) {
-  std::uint32_t r;
-  asm("{\n\t.reg .b8 b;\n\t"
-      "cvt.u8.u32 b, %1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
-      : "=r"(r)
-      : "r"(byte));
-  return *reinterpret_cast<__half2 *>(&r);
+// Eight e2m1 to four pairs.
+__device__ __forceinline__ void from_e2m1x8(std::uint32_t w, __half2 (&h)[4]) {
+  std::uint32_t r[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2 *>(&r[i]);
 }
 
 // e4m3 of a non-negative float (round to nearest even, at most 448).

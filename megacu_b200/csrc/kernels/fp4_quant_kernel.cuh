@@ -1,13 +1,15 @@
 // Quantisation of matrices to the 4-bit block formats, and the values back.
 //
-// Bound by memory: 2 (or 4) bytes read and 0.53-0.56 written per element, so
-// the arithmetic has about 14 lane operations per 16-bit element. Every
-// decision (scale and element) is the exact value's:
+// Bound by memory as long as an element costs few instructions: 2 (or 4) bytes
+// read and 0.53-0.56 written per element leave about 14 per 16-bit element at
+// full issue rate. Every decision (scale and element) is the exact value's:
 //  * MX divides by a power of two, which is exact.
-//  * NV with 16-bit inputs: z / s is a multiple of 2^-2 (a tie) or at least
-//    2^-14 away from every tie (11-bit over 4-bit mantissas), so rounding
-//    z * (1 / s), which is within 2^-20, to multiples of 2^-16 restores every
-//    tie and crosses none. One FMA with 1.5 * 2^7 and one subtraction do it.
+//  * NV with 16-bit inputs: amax / 6 is a tie between two scales or at least
+//    2^-11 of itself away from every tie (11-bit against 7-bit integers), so
+//    amax * (1 / 6), within 2^-22, rounded to 13 significant bits restores
+//    every tie and crosses none. Likewise z / s is a multiple of 2^-2 (a tie)
+//    or at least 2^-14 away from one: z * (1 / s), within 2^-20, is rounded to
+//    multiples of 2^-16 by one FMA with 1.5 * 2^7 and one subtraction.
 //  * NV with 32-bit inputs compares |z| with the seven borders times s, each
 //    exact in 32 bits; the scale divides with a sticky bit (round to odd).
 #pragma once
@@ -36,47 +38,58 @@ struct fp4_matrix_params {
   std::uint8_t *scales;
 };
 
-// Scale byte and multiplier of one block. `bits` is the largest |x| as its
-// 32-bit float pattern (so that NaN sorts above infinity above numbers).
+// Scale byte and multiplier of one block.
 struct fp4_block_scale {
   std::uint32_t byte;
-  float mul;    // MX: z / scale = x * mul * mul2. NV: 16-bit x: x * mul; 32-bit x: see encode
-  float mul2;
+  float mul;   // MX: z / scale = x * mul * mul2. NV: 16-bit x: x * mul; 32-bit x: see scaled()
+  float mul2;  // MX: 1 but for tiny blocks
+  bool empty;  // a NaN block or an NV scale of zero: the elements are zeros
 };
 
+// `bits` is the largest |x| as its 32-bit float pattern (NaN sorts above
+// infinity above numbers).
 template <bool kNv, bool kWide>
 __device__ __forceinline__ fp4_block_scale block_scale(std::uint32_t bits, int log2_scale) {
   fp4_block_scale b;
   b.mul2 = 1.0f;
-  if (bits >= 0x7f800000u) {  // infinity or NaN: the whole block is NaN
-    b.byte = kNv ? 0x7fu : 0xffu;
-    b.mul = 0.0f;
-    return b;
-  }
-  float const amax = __uint_as_float(bits);
   if constexpr (!kNv) {
-    int const fl = bits >= 0x00800000u ? static_cast<int>(bits >> 23) - 127
-                                       : 31 - __clz(static_cast<int>(bits)) - 149;
-    int e = fl + log2_scale - 2;
-    e = bits == 0 ? -127 : min(max(e, -127), 127);
-    int const f = log2_scale - e;
-    b.byte = static_cast<std::uint32_t>(e + 127);
-    b.mul = pow2(min(max(f, -126), 126));
-    if (f > 126) b.mul2 = pow2(f - 126);  // tiny blocks: exact in two steps
+    // amax = 2^(E - 127) * 1.f: byte E + log2 g - 2, multiplier 2^(129 - E + 127 - 127).
+    int const exponent = static_cast<int>(bits >> 23);
+    int const byte = exponent + log2_scale - 2;
+    b.byte = static_cast<std::uint32_t>(byte);
+    b.mul = __int_as_float((256 - exponent) << 23);
+    b.empty = false;
+    if (exponent < 2 || exponent == 255 || byte < 0 || byte > 254) {
+      // Zero, subnormal, infinite or NaN blocks and scales at the ends of the range.
+      int const fl = exponent > 0 ? exponent - 127
+                                  : 31 - __clz(static_cast<int>(bits)) - 149;
+      int const e = bits == 0 ? -127 : min(max(fl + log2_scale - 2, -127), 127);
+      int const f = log2_scale - e;
+      b.byte = static_cast<std::uint32_t>(e + 127);
+      b.mul = pow2(min(max(f, -126), 126));
+      if (f > 126) b.mul2 = pow2(f - 126);  // exact in two steps
+      b.empty = exponent == 255;
+      if (b.empty) b.byte = 0xffu;
+    }
   } else {
     float const g = pow2(log2_scale);
-    float const a = fminf(amax * g, 4096.0f);  // past 6 * 448 the scale stays 448
+    float const a = fminf(__uint_as_float(bits) * g, 4096.0f);  // past 6 * 448 it stays 448
     float v;
     if constexpr (kWide) {
       v = __fdiv_rz(a, 6.0f);
       if (fmaf(-6.0f, v, a) != 0.0f) v = __uint_as_float(__float_as_uint(v) | 1u);
     } else {
-      v = __fdiv_rn(a, 6.0f);
+      v = __uint_as_float((__float_as_uint(a * (1.0f / 6.0f)) + 0x400u) & ~0x7ffu);
     }
     b.byte = to_e4m3(v);
     float const s = from_e4m3(b.byte);
-    b.mul = s == 0.0f ? 0.0f : kWide ? s : __fdiv_rn(g, s);
+    b.mul = kWide ? s : g * __frcp_rn(s);
     b.mul2 = g;
+    b.empty = b.byte == 0;
+    if (bits >= 0x7f800000u) {
+      b.byte = 0x7fu;
+      b.empty = true;
+    }
   }
   return b;
 }
@@ -98,28 +111,20 @@ __device__ __forceinline__ float scaled(float x, fp4_block_scale const &b) {
     q = z > 2.5f * s ? 3.0f : q;
     q = z >= 3.5f * s ? 4.0f : q;
     q = z > 5.0f * s ? 6.0f : q;
-    return copysignf(s == 0.0f ? 0.0f : q, x);
+    return copysignf(q, x);
   }
 }
 
 // Eight elements to one 32-bit word.
 template <bool kNv, bool kWide>
-__device__ __forceinline__ std::uint32_t encode8(float const *x, fp4_block_scale const &b) {
-  float y[8];
+__device__ __forceinline__ std::uint32_t encode8(float (&x)[8], fp4_block_scale const &b) {
+  if (!kNv && b.mul2 != 1.0f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float v = x[i];
-    if constexpr (!kNv) {
-      if (b.mul2 != 1.0f) v *= b.mul2;
-    }
-    y[i] = scaled<kNv, kWide>(v, b);
+    for (int i = 0; i < 8; ++i) x[i] *= b.mul2;
   }
-  std::uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w |= e2m1x2(y[2 * i], y[2 * i + 1]) << (8 * i);
-  // A NaN block holds zeros; so does an NV block whose scale rounds to zero.
-  bool const empty = kNv ? b.mul == 0.0f : b.byte == 0xffu;
-  return empty ? 0u : w;
+  for (int i = 0; i < 8; ++i) x[i] = scaled<kNv, kWide>(x[i], b);
+  return b.empty ? 0u : e2m1x8(x);
 }
 
 // The largest |v[i]| of 16-bit pairs or 32-bit words as a 32-bit float pattern.
@@ -132,9 +137,12 @@ __device__ __forceinline__ std::uint32_t max_abs(std::uint32_t const *w) {
     for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7fffffffu);
     return m;
   } else {
-    std::uint32_t m = 0;
+    std::uint32_t m = w[0] & 0x7fff7fffu;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    for (int i = 1; i + 1 < kWords; i += 2) {
+      m = __vimax3_u16x2(m, w[i] & 0x7fff7fffu, w[i + 1] & 0x7fff7fffu);
+    }
+    if constexpr (kWords % 2 == 0) m = __vmaxu2(m, w[kWords - 1] & 0x7fff7fffu);
     m = max(m & 0xffffu, m >> 16);
     if constexpr (std::is_same_v<T, __nv_bfloat16>) {
       return m << 16;
@@ -195,7 +203,9 @@ inline constexpr int kQuantRows = 32;   // rows of a CTA: 8 of each 32 rows of a
 // each (512 bytes of a 16-bit row, 128 bytes of elements out). Its rows are
 // rows [8 s, 8 s + 8) of each quarter of a 128-row scale tile, so that the
 // scale bytes it owns are 128 contiguous bytes of each of its scale tiles.
-// Two passes per CTA, both rows' loads in flight.
+// With slot_of_row they are 32 consecutive rows instead: an expert's rows fill
+// the front of its tiles, so most CTAs of few rows per expert have none and
+// end at once. Two passes per CTA, both rows' loads in flight.
 template <class T, bool kNv, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_params p,
                                                                     T const *x) {
@@ -203,23 +213,28 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
   constexpr int kTileCols = fp4_tile_cols(kNv);
   constexpr int kTiles = kQuantCols / kTileCols;
   constexpr int kPasses = kQuantRows / 16;
-  // [tile][row of the slice][quarter] of four scale bytes
-  __shared__ std::uint32_t bytes[kTiles][8][4];
+  // [tile][row] of four scale bytes: whole matrices in the scale tile's order
+  __shared__ alignas(16) std::uint32_t bytes[kTiles][kQuantRows];
   std::int64_t const row_tile = blockIdx.x / (4 * p.col_tiles);
   int const slice = static_cast<int>(blockIdx.x % 4);
   int const col0 = static_cast<int>(blockIdx.x / 4 % p.col_tiles) * kQuantCols;
   int const lane16 = threadIdx.x % 16;
   int const col = col0 + lane16 * 16;
 
+  bool const masked = p.slot_of_row != nullptr;
+  // Where row l of the CTA lies in its row tile, and in `bytes`.
+  auto tile_row = [&](int l) { return masked ? slice * 32 + l : l / 8 * 32 + slice * 8 + l % 8; };
+  auto byte_row = [&](int l) { return masked ? l : l % 8 * 4 + l / 8; };
+
   std::uint32_t w[kPasses][4 * sizeof(T)];
   std::int64_t rows[kPasses];  // -1: nothing of this row is written
 #pragma unroll
   for (int pass = 0; pass < kPasses; ++pass) {
     int const l = pass * 16 + threadIdx.x / 16;
-    std::int64_t const row = row_tile * kScaleTileRows + l / 8 * 32 + slice * 8 + l % 8;
+    std::int64_t const row = row_tile * kScaleTileRows + tile_row(l);
     std::int64_t src = row;
     bool in = row < p.rows;
-    if (in && p.slot_of_row != nullptr) {
+    if (in && masked) {
       std::int32_t const slot = p.slot_of_row[row];
       in = slot >= 0;
       if (p.topk > 0) {
@@ -230,6 +245,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
     rows[pass] = in ? row : -1;
     if (in && col < p.cols) load16<T, kVec>(x + src * p.stride + col, w[pass]);
   }
+  if (masked && __syncthreads_or(rows[0] >= 0 || rows[kPasses - 1] >= 0) == 0) return;
 #pragma unroll
   for (int pass = 0; pass < kPasses; ++pass) {
     int const l = pass * 16 + threadIdx.x / 16;
@@ -248,19 +264,19 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
     }
     if (kNv || lane16 % 2 == 0) {
       int const blk = lane16 * 16 / fp4_block(kNv);
-      reinterpret_cast<std::uint8_t *>(&bytes[blk / 4][l % 8][l / 8])[blk % 4] =
+      reinterpret_cast<std::uint8_t *>(&bytes[blk / 4][byte_row(l)])[blk % 4] =
           static_cast<std::uint8_t>(b.byte);
     }
   }
   __syncthreads();
   int const tile0 = col0 / kTileCols;
   int const tiles = min(kTiles, p.tiles - tile0);
-  std::uint8_t *const dst = p.scales + (row_tile * p.tiles + tile0) * kScaleTileBytes + slice * 128;
-  if (p.slot_of_row == nullptr) {
+  std::uint8_t *const dst = p.scales + (row_tile * p.tiles + tile0) * kScaleTileBytes;
+  if (!masked) {
     if (static_cast<int>(threadIdx.x) < tiles * 8) {
       int const tile = threadIdx.x / 8, r = threadIdx.x % 8;
-      *reinterpret_cast<uint4 *>(dst + tile * kScaleTileBytes + r * 16) =
-          *reinterpret_cast<uint4 const *>(bytes[tile][r]);
+      *reinterpret_cast<uint4 *>(dst + tile * kScaleTileBytes + (slice * 8 + r) * 16) =
+          *reinterpret_cast<uint4 const *>(&bytes[tile][r * 4]);
     }
   } else if (lane16 < tiles) {
     // Only the rows written above: their four bytes of each tile.
@@ -268,8 +284,8 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
     for (int pass = 0; pass < kPasses; ++pass) {
       int const l = pass * 16 + threadIdx.x / 16;
       if (rows[pass] < 0) continue;
-      *reinterpret_cast<std::uint32_t *>(dst + lane16 * kScaleTileBytes + l % 8 * 16 + l / 8 * 4) =
-          bytes[lane16][l % 8][l / 8];
+      *reinterpret_cast<std::uint32_t *>(dst + lane16 * kScaleTileBytes +
+                                         scale_byte(tile_row(l), 0)) = bytes[lane16][l];
     }
   }
 }
@@ -381,8 +397,7 @@ __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_ma
   }
 }
 
-// The values: element * scale / g, exact in 32 bits and rounded once. A
-// thread decodes 16 elements.
+// The values: element * scale / g, rounded once. A thread decodes 16 elements.
 template <class T, bool kNv, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matrix_params p, T *y) {
   std::uint32_t const per_row = static_cast<std::uint32_t>(p.cols) / 16;
@@ -399,23 +414,35 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matri
     std::uint32_t const byte =
         p.scales[((row / kScaleTileRows) * p.tiles + blk / 4) * kScaleTileBytes +
                  scale_byte(static_cast<int>(row % kScaleTileRows), blk)];
-    // scale / g as two factors, each a normal power of two (or e4m3 / 2^k).
-    float s1, s2;
+    // scale / g: one factor, or two where it is no normal power of two (the
+    // first product is exact, the second rounds once).
+    float s1, s2 = 1.0f;
     if constexpr (kNv) {
-      s1 = from_e4m3(byte);
-      s2 = pow2(-p.log2_scale);
+      s1 = from_e4m3(byte) * pow2(-p.log2_scale);
     } else {
       int const e = static_cast<int>(byte) - 127 - p.log2_scale;
-      s1 = byte == 0xffu ? __int_as_float(0x7fffffff) : pow2(e / 2);
-      s2 = pow2(e - e / 2);
+      bool const normal = e >= -126 && e <= 127;
+      s1 = pow2(normal ? e : e < 0 ? -100 : 100);
+      if (!normal) s2 = pow2(e < 0 ? e + 100 : e - 100);
+      if (byte == 0xffu) s1 = __int_as_float(0x7fffffff);
     }
     alignas(32) T out[16];
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      std::uint32_t const w = b < 4 ? d.x : d.y;
-      float2 const f = __half22float2(from_e2m1x2(w >> (8 * (b % 4)) & 0xffu));
-      out[2 * b] = from_f32<T>(f.x * s1 * s2);
-      out[2 * b + 1] = from_f32<T>(f.y * s1 * s2);
+    for (int b = 0; b < 2; ++b) {
+      __half2 h[4];
+      from_e2m1x8(b == 0 ? d.x : d.y, h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 f = __half22float2(h[i]);
+        f.x *= s1;
+        f.y *= s1;
+        if (!kNv && s2 != 1.0f) {
+          f.x *= s2;
+          f.y *= s2;
+        }
+        out[8 * b + 2 * i] = from_f32<T>(f.x);
+        out[8 * b + 2 * i + 1] = from_f32<T>(f.y);
+      }
     }
     T *const dst = y + row * p.stride + col;
     if constexpr (kVec) {
