@@ -45,7 +45,7 @@ megacu_status check_matrix(megacu_fp4_matrix const *m, int &log2_scale) {
     return fail(MEGACU_INVALID_ARGUMENT, 21, "cols must be a multiple of 32 (16-byte rows)");
   }
   if (m->rows > kMaxDim || m->cols > kMaxDim ||
-      4 * ceil_div(m->rows, kScaleTileRows) * ceil_div(m->cols, kQuantCols) > 0x7fffffffll) {
+      2 * ceil_div(m->rows, kScaleTileRows) * ceil_div(m->cols, kQuantCols) > 0x7fffffffll) {
     return fail(MEGACU_UNSUPPORTED, 22, "dimension too large");
   }
   int e = 0;
@@ -396,8 +396,9 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
   if (guard.status() != cudaSuccess) return cuda_fail(guard.status(), 10);
   fp4_matrix_params prm = matrix_params(m, log2_scale, data, scales, transpose);
   prm.slot_of_row = static_cast<std::int32_t const *>(slot_of_row);
-  auto const grid = static_cast<unsigned>(ceil_div(m.rows, kScaleTileRows) * prm.col_tiles *
-                                          (transpose ? 2 : 4));
+  static_assert(kScaleTileRows == 2 * kQuantRows && kQuantRows == kQuantTRows, "two CTAs deep");
+  auto const grid =
+      static_cast<unsigned>(2 * ceil_div(m.rows, kScaleTileRows) * prm.col_tiles);
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
   by_type(m.dtype, m.format, [&](auto value, auto nv) {
     using T = decltype(value);

@@ -30,7 +30,7 @@ struct fp4_matrix_params {
   std::int64_t stride;   // elements between the rows of x (of x as stored)
   std::int32_t log2_scale;
   std::int32_t tiles;    // scale tiles per row tile
-  std::uint32_t col_tiles;  // CTAs per row tile, each kQuantCols columns
+  std::uint32_t col_tiles;  // CTAs that share their rows, each kQuantCols columns
   std::int32_t topk;     // > 0: row r is x's row slot_of_row[r] / topk
   std::int64_t x_rows;   // topk > 0: rows of x; an entry past them has no row
   std::int32_t const *slot_of_row;  // nullptr: every row; < 0: the row is left as it was
@@ -38,13 +38,22 @@ struct fp4_matrix_params {
   std::uint8_t *scales;
 };
 
-// Scale byte and multiplier of one block.
+// Scale byte and multipliers of one block.
 struct fp4_block_scale {
   std::uint32_t byte;
   float mul;   // MX: z / scale = x * mul * mul2. NV: 16-bit x: x * mul; 32-bit x: see scaled()
-  float mul2;  // MX: 1 but for tiny blocks
+  float mul2;  // MX: 1 in an ordinary block
   bool empty;  // a NaN block or an NV scale of zero: the elements are zeros
 };
+
+// MX blocks whose scale is E + log2 g - 2 and whose multiplier is 2^(129 - E)
+// for amax = 1.f * 2^(E - 127): all but zero, subnormal, infinite and NaN ones
+// and scales at the ends of the range.
+__device__ __forceinline__ bool ordinary_mx(std::uint32_t bits, int log2_scale) {
+  int const exponent = static_cast<int>(bits >> 23);
+  int const byte = exponent + log2_scale - 2;
+  return exponent >= 2 && exponent < 255 && byte >= 0 && byte <= 254;
+}
 
 // `bits` is the largest |x| as its 32-bit float pattern (NaN sorts above
 // infinity above numbers).
@@ -52,25 +61,11 @@ template <bool kNv, bool kWide>
 __device__ __forceinline__ fp4_block_scale block_scale(std::uint32_t bits, int log2_scale) {
   fp4_block_scale b;
   b.mul2 = 1.0f;
-  if constexpr (!kNv) {
-    // amax = 2^(E - 127) * 1.f: byte E + log2 g - 2, multiplier 2^(129 - E + 127 - 127).
+  if constexpr (!kNv) {  // ordinary blocks
     int const exponent = static_cast<int>(bits >> 23);
-    int const byte = exponent + log2_scale - 2;
-    b.byte = static_cast<std::uint32_t>(byte);
+    b.byte = static_cast<std::uint32_t>(exponent + log2_scale - 2);
     b.mul = __int_as_float((256 - exponent) << 23);
     b.empty = false;
-    if (exponent < 2 || exponent == 255 || byte < 0 || byte > 254) {
-      // Zero, subnormal, infinite or NaN blocks and scales at the ends of the range.
-      int const fl = exponent > 0 ? exponent - 127
-                                  : 31 - __clz(static_cast<int>(bits)) - 149;
-      int const e = bits == 0 ? -127 : min(max(fl + log2_scale - 2, -127), 127);
-      int const f = log2_scale - e;
-      b.byte = static_cast<std::uint32_t>(e + 127);
-      b.mul = pow2(min(max(f, -126), 126));
-      if (f > 126) b.mul2 = pow2(f - 126);  // exact in two steps
-      b.empty = exponent == 255;
-      if (b.empty) b.byte = 0xffu;
-    }
   } else {
     float const g = pow2(log2_scale);
     float const a = fminf(__uint_as_float(bits) * g, 4096.0f);  // past 6 * 448 it stays 448
@@ -83,7 +78,9 @@ __device__ __forceinline__ fp4_block_scale block_scale(std::uint32_t bits, int l
     }
     b.byte = to_e4m3(v);
     float const s = from_e4m3(b.byte);
-    b.mul = kWide ? s : g * __frcp_rn(s);
+    float inverse;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(s));
+    b.mul = kWide ? s : g * inverse;
     b.mul2 = g;
     b.empty = b.byte == 0;
     if (bits >= 0x7f800000u) {
@@ -91,6 +88,20 @@ __device__ __forceinline__ fp4_block_scale block_scale(std::uint32_t bits, int l
       b.empty = true;
     }
   }
+  return b;
+}
+
+// Every other MX block.
+__device__ __forceinline__ fp4_block_scale rare_mx(std::uint32_t bits, int log2_scale) {
+  int const exponent = static_cast<int>(bits >> 23);
+  int const fl = exponent > 0 ? exponent - 127 : 31 - __clz(static_cast<int>(bits)) - 149;
+  int const e = bits == 0 ? -127 : min(max(fl + log2_scale - 2, -127), 127);
+  int const f = log2_scale - e;
+  fp4_block_scale b;
+  b.empty = exponent == 255;
+  b.byte = b.empty ? 0xffu : static_cast<std::uint32_t>(e + 127);
+  b.mul = pow2(min(max(f, -126), 126));
+  b.mul2 = f > 126 ? pow2(f - 126) : 1.0f;  // exact in two steps
   return b;
 }
 
@@ -118,13 +129,9 @@ __device__ __forceinline__ float scaled(float x, fp4_block_scale const &b) {
 // Eight elements to one 32-bit word.
 template <bool kNv, bool kWide>
 __device__ __forceinline__ std::uint32_t encode8(float (&x)[8], fp4_block_scale const &b) {
-  if (!kNv && b.mul2 != 1.0f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= b.mul2;
-  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = scaled<kNv, kWide>(x[i], b);
-  return b.empty ? 0u : e2m1x8(x);
+  return kNv && b.empty ? 0u : e2m1x8(x);
 }
 
 // The largest |v[i]| of 16-bit pairs or 32-bit words as a 32-bit float pattern.
@@ -173,9 +180,53 @@ __device__ __forceinline__ std::uint32_t encode_words(std::uint32_t const *w, in
   return encode8<kNv, std::is_same_v<T, float>>(f, b);
 }
 
+// The elements of a block, or of half of one, plain and coded.
+template <class T, int kElements>
+struct fp4_words {
+  std::uint32_t w[kElements * sizeof(T) / 4];
+};
+template <int kElements>
+struct fp4_coded {
+  std::uint32_t w[kElements / 8];
+  std::uint32_t byte;
+};
+
+// A call, not inlined: predicated into the ordinary path, these instructions
+// cost every block.
+template <class T, int kElements>
+__device__ __noinline__ fp4_coded<kElements> encode_rare_mx(fp4_words<T, kElements> v,
+                                                            std::uint32_t bits, int log2_scale) {
+  fp4_block_scale const b = rare_mx(bits, log2_scale);
+  fp4_coded<kElements> out;
+#pragma unroll
+  for (int k = 0; k < kElements / 8; ++k) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = element<T>(v.w, k * 8 + i) * b.mul2;
+    out.w[k] = b.empty ? 0u : encode8<false, std::is_same_v<T, float>>(f, b);
+  }
+  out.byte = b.byte;
+  return out;
+}
+
+template <class T, bool kNv, int kElements>
+__device__ __forceinline__ fp4_coded<kElements> encode_block(fp4_words<T, kElements> const &v,
+                                                             std::uint32_t bits, int log2_scale) {
+  if (!kNv && !ordinary_mx(bits, log2_scale)) {
+    return encode_rare_mx<T, kElements>(v, bits, log2_scale);
+  }
+  fp4_block_scale const b = block_scale<kNv, std::is_same_v<T, float>>(bits, log2_scale);
+  fp4_coded<kElements> out;
+#pragma unroll
+  for (int k = 0; k < kElements / 8; ++k) out.w[k] = encode_words<T, kNv>(v.w, k * 8, b);
+  out.byte = b.byte;
+  return out;
+}
+
 // 16 consecutive elements as words, by 32-byte loads when the rows allow it.
 template <class T, bool kVec>
-__device__ __forceinline__ void load16(T const *p, std::uint32_t (&w)[4 * sizeof(T)]) {
+__device__ __forceinline__ void load16(T const *p, fp4_words<T, 16> &words) {
+  std::uint32_t *const w = words.w;
   if constexpr (kVec) {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
@@ -197,37 +248,43 @@ __device__ __forceinline__ void load16(T const *p, std::uint32_t (&w)[4 * sizeof
 
 inline constexpr int kQuantThreads = 256;
 inline constexpr int kQuantCols = 256;  // columns of a CTA
-inline constexpr int kQuantRows = 32;   // rows of a CTA: 8 of each 32 rows of a scale tile
+inline constexpr int kQuantRows = 64;   // rows of a CTA: 16 of each 32 rows of a scale tile
 
-// A CTA quantises 32 rows x 256 columns: 16 lanes per row with 16 elements
-// each (512 bytes of a 16-bit row, 128 bytes of elements out). Its rows are
-// rows [8 s, 8 s + 8) of each quarter of a 128-row scale tile, so that the
-// scale bytes it owns are 128 contiguous bytes of each of its scale tiles.
-// With slot_of_row they are 32 consecutive rows instead: an expert's rows fill
-// the front of its tiles, so most CTAs of few rows per expert have none and
-// end at once. Two passes per CTA, both rows' loads in flight.
+// A CTA quantises 64 rows x 256 columns (neighbouring CTAs neighbouring
+// columns, so that rows stream through DRAM in order): 16 lanes per row with 16
+// elements each (512 bytes of a 16-bit row, 128 bytes of elements out). Its
+// rows are rows [16 s, 16 s + 16) of each quarter of a 128-row scale tile,
+// so that the scale bytes it owns are 256 contiguous bytes of each of its scale
+// tiles. With slot_of_row they are 64 consecutive rows instead: an expert's
+// rows fill the front of its tiles, so CTAs without any end at once. Four
+// passes per CTA, all four rows' loads in flight: with two, what a thread does
+// once (addresses, barriers) was a third of its instructions.
 template <class T, bool kNv, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_params p,
                                                                     T const *x) {
-  constexpr bool kWide = std::is_same_v<T, float>;
   constexpr int kTileCols = fp4_tile_cols(kNv);
   constexpr int kTiles = kQuantCols / kTileCols;
   constexpr int kPasses = kQuantRows / 16;
   // [tile][row] of four scale bytes: whole matrices in the scale tile's order
   __shared__ alignas(16) std::uint32_t bytes[kTiles][kQuantRows];
-  std::int64_t const row_tile = blockIdx.x / (4 * p.col_tiles);
-  int const slice = static_cast<int>(blockIdx.x % 4);
-  int const col0 = static_cast<int>(blockIdx.x / 4 % p.col_tiles) * kQuantCols;
+  constexpr int kSlices = kScaleTileRows / kQuantRows;
+  constexpr int kPer = kQuantRows / 4;  // rows of each quarter
+  std::uint32_t const rows_cta = blockIdx.x / p.col_tiles;
+  std::int64_t const row_tile = rows_cta / kSlices;
+  int const slice = static_cast<int>(rows_cta % kSlices);
+  int const col0 = static_cast<int>(blockIdx.x - rows_cta * p.col_tiles) * kQuantCols;
   int const lane16 = threadIdx.x % 16;
   int const col = col0 + lane16 * 16;
 
   bool const masked = p.slot_of_row != nullptr;
   // Where row l of the CTA lies in its row tile, and in `bytes`.
-  auto tile_row = [&](int l) { return masked ? slice * 32 + l : l / 8 * 32 + slice * 8 + l % 8; };
-  auto byte_row = [&](int l) { return masked ? l : l % 8 * 4 + l / 8; };
+  auto tile_row = [&](int l) {
+    return masked ? slice * kQuantRows + l : l / kPer * 32 + slice * kPer + l % kPer;
+  };
+  auto byte_row = [&](int l) { return masked ? l : l % kPer * 4 + l / kPer; };
 
-  std::uint32_t w[kPasses][4 * sizeof(T)];
-  std::int64_t rows[kPasses];  // -1: nothing of this row is written
+  fp4_words<T, 16> w[kPasses];
+  std::uint32_t have = 0;  // passes whose row is written
 #pragma unroll
   for (int pass = 0; pass < kPasses; ++pass) {
     int const l = pass * 16 + threadIdx.x / 16;
@@ -242,30 +299,30 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
         in = in && src < p.x_rows;
       }
     }
-    rows[pass] = in ? row : -1;
+    if (in) have |= 1u << pass;
     if (in && col < p.cols) load16<T, kVec>(x + src * p.stride + col, w[pass]);
   }
-  if (masked && __syncthreads_or(rows[0] >= 0 || rows[kPasses - 1] >= 0) == 0) return;
+  if (masked && __syncthreads_or(have != 0) == 0) return;
 #pragma unroll
   for (int pass = 0; pass < kPasses; ++pass) {
     int const l = pass * 16 + threadIdx.x / 16;
-    fp4_block_scale b{};
+    std::uint32_t byte = 0;
     // Both lanes of an MX block are in or out together (cols % 32 == 0).
-    if (rows[pass] >= 0 && col < p.cols) {
-      std::uint32_t bits = max_abs<T, 4 * sizeof(T)>(w[pass]);
+    if ((have >> pass & 1u) && col < p.cols) {
+      std::uint32_t bits = max_abs<T, 4 * sizeof(T)>(w[pass].w);
       if constexpr (!kNv) {
         bits = max(bits, __shfl_xor_sync(3u << (threadIdx.x % 32 & ~1u), bits, 1));
       }
-      b = block_scale<kNv, kWide>(bits, p.log2_scale);
-      uint2 out;
-      out.x = encode_words<T, kNv>(w[pass], 0, b);
-      out.y = encode_words<T, kNv>(w[pass], 8, b);
-      *reinterpret_cast<uint2 *>(p.data + rows[pass] * (p.cols / 2) + col / 2) = out;
+      fp4_coded<16> const coded = encode_block<T, kNv, 16>(w[pass], bits, p.log2_scale);
+      byte = coded.byte;
+      std::int64_t const row = row_tile * kScaleTileRows + tile_row(l);
+      *reinterpret_cast<uint2 *>(p.data + row * (p.cols / 2) + col / 2) =
+          make_uint2(coded.w[0], coded.w[1]);
     }
     if (kNv || lane16 % 2 == 0) {
       int const blk = lane16 * 16 / fp4_block(kNv);
       reinterpret_cast<std::uint8_t *>(&bytes[blk / 4][byte_row(l)])[blk % 4] =
-          static_cast<std::uint8_t>(b.byte);
+          static_cast<std::uint8_t>(byte);
     }
   }
   __syncthreads();
@@ -273,9 +330,9 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
   int const tiles = min(kTiles, p.tiles - tile0);
   std::uint8_t *const dst = p.scales + (row_tile * p.tiles + tile0) * kScaleTileBytes;
   if (!masked) {
-    if (static_cast<int>(threadIdx.x) < tiles * 8) {
-      int const tile = threadIdx.x / 8, r = threadIdx.x % 8;
-      *reinterpret_cast<uint4 *>(dst + tile * kScaleTileBytes + (slice * 8 + r) * 16) =
+    if (static_cast<int>(threadIdx.x) < tiles * kPer) {
+      int const tile = threadIdx.x / kPer, r = threadIdx.x % kPer;
+      *reinterpret_cast<uint4 *>(dst + tile * kScaleTileBytes + (slice * kPer + r) * 16) =
           *reinterpret_cast<uint4 const *>(&bytes[tile][r * 4]);
     }
   } else if (lane16 < tiles) {
@@ -283,7 +340,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
 #pragma unroll
     for (int pass = 0; pass < kPasses; ++pass) {
       int const l = pass * 16 + threadIdx.x / 16;
-      if (rows[pass] < 0) continue;
+      if ((have >> pass & 1u) == 0) continue;
       *reinterpret_cast<std::uint32_t *>(dst + lane16 * kScaleTileBytes +
                                          scale_byte(tile_row(l), 0)) = bytes[lane16][l];
     }
@@ -300,7 +357,6 @@ inline constexpr int kQuantTRows = 64;  // rows of the quantised matrix per CTA
 template <class T, bool kNv, bool kPair>
 __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_matrix_params p,
                                                                          T const *x) {
-  constexpr bool kWide = std::is_same_v<T, float>;
   constexpr int kTileCols = fp4_tile_cols(kNv);
   constexpr int kTiles = kQuantCols / kTileCols;
   constexpr int kBlock = fp4_block(kNv);
@@ -308,10 +364,11 @@ __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_ma
   // [tile][row % 32][row / 32] of four scale bytes
   __shared__ std::uint32_t bytes[kTiles][32][2];
   __shared__ uint4 turned[kQuantTRows][8];
-  std::int64_t const row_tile = blockIdx.x / (2 * p.col_tiles);
-  int const part = static_cast<int>(blockIdx.x % 2);
+  std::uint32_t const rows_cta = blockIdx.x / p.col_tiles;
+  std::int64_t const row_tile = rows_cta / 2;
+  int const part = static_cast<int>(rows_cta % 2);
   std::int64_t const row0 = row_tile * kScaleTileRows + part * kQuantTRows;
-  int const col0 = static_cast<int>(blockIdx.x / 2 % p.col_tiles) * kQuantCols;
+  int const col0 = static_cast<int>(blockIdx.x - rows_cta * p.col_tiles) * kQuantCols;
   int const r = threadIdx.x % 32 * 2, chunk = threadIdx.x / 32;
   std::int64_t const row = row0 + r;
   int const col = col0 + chunk * 32;
@@ -356,23 +413,22 @@ __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_ma
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     std::uint32_t out[4];
-    std::uint32_t scale[32 / kBlock];
 #pragma unroll
     for (int k = 0; k < 32 / kBlock; ++k) {
-      scale[k] = 0;
+      std::uint32_t byte = 0;
       if (in && (h == 0 || two)) {
-        std::uint32_t const *const v = w[h] + k * kWordBlock;
-        fp4_block_scale const b =
-            block_scale<kNv, kWide>(max_abs<T, kWordBlock>(v), p.log2_scale);
+        fp4_words<T, kBlock> v;
 #pragma unroll
-        for (int i = 0; i < kBlock / 8; ++i) {
-          out[k * (kBlock / 8) + i] = encode_words<T, kNv>(v, i * 8, b);
-        }
-        scale[k] = b.byte;
+        for (int i = 0; i < kWordBlock; ++i) v.w[i] = w[h][k * kWordBlock + i];
+        fp4_coded<kBlock> const coded = encode_block<T, kNv, kBlock>(
+            v, max_abs<T, kWordBlock>(v.w), p.log2_scale);
+#pragma unroll
+        for (int i = 0; i < kBlock / 8; ++i) out[k * (kBlock / 8) + i] = coded.w[i];
+        byte = coded.byte;
       }
       int const blk = chunk * (32 / kBlock) + k;
       reinterpret_cast<std::uint8_t *>(&bytes[blk / 4][(r + h) % 32][(r + h) / 32])[blk % 4] =
-          static_cast<std::uint8_t>(scale[k]);
+          static_cast<std::uint8_t>(byte);
     }
     if (in && (h == 0 || two)) {
       turned[r + h][chunk ^ (r / 2 % 8)] = make_uint4(out[0], out[1], out[2], out[3]);
@@ -401,11 +457,12 @@ __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_ma
 template <class T, bool kNv, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matrix_params p, T *y) {
   std::uint32_t const per_row = static_cast<std::uint32_t>(p.cols) / 16;
-  std::uint32_t const i = blockIdx.x % p.col_tiles * 16 + threadIdx.x % 16;
+  std::uint32_t const rows_cta = blockIdx.x / p.col_tiles;
+  std::uint32_t const i = (blockIdx.x - rows_cta * p.col_tiles) * 16 + threadIdx.x % 16;
   if (i >= per_row) return;
   int const col = static_cast<int>(i) * 16;
   int const blk = col / fp4_block(kNv);
-  std::int64_t const row0 = static_cast<std::int64_t>(blockIdx.x / p.col_tiles) * kQuantRows;
+  std::int64_t const row0 = static_cast<std::int64_t>(rows_cta) * kQuantRows;
 #pragma unroll
   for (int pass = 0; pass < kQuantRows / 16; ++pass) {
     std::int64_t const row = row0 + pass * 16 + threadIdx.x / 16;
