@@ -615,6 +615,47 @@ megacu_status megacu_cuda_fp4_gemm_swiglu(megacu_driver_view driver, const void 
                                           void *events,
                                           const megacu_fp4_gemm_problem *problem);
 
+typedef struct megacu_moe_mlp_problem {
+  int64_t tokens;       /* 0 is an empty batch */
+  int64_t hidden;       /* multiple of 32 */
+  int64_t inter;        /* this PE's slice of the intermediate size; multiple of 32 */
+  int32_t topk;         /* as megacu_moe_problem, down to id_bytes */
+  int32_t experts;
+  int32_t first_expert;
+  int32_t dtype;        /* of x, y and the rows between the products */
+  int32_t id_bytes;
+  int32_t format;       /* enum megacu_fp4_format, of weights and activations */
+  float x_scale;        /* powers of two that multiply x and act before they are */
+  float act_scale;      /* quantised (undone in the products); 0 = 1 */
+  float up_alpha;       /* factor of gate and up, 1 / the weights' scale */
+  float down_alpha;     /* factor of down */
+  uint64_t timeout_ns;  /* bound of every wait inside the products; 0 = 4 s */
+} megacu_moe_mlp_problem;
+
+megacu_status megacu_b200_moe_mlp_workspace_bytes(const megacu_moe_mlp_problem *problem,
+                                                  int64_t *bytes);
+
+/*
+ * A routed MLP block: for every token t and choice j whose expert e is here,
+ *   y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t]))
+ * as megacu_cuda_moe_sort (align 128), _fp4_quantize (gathered),
+ * _fp4_gemm_swiglu, _fp4_quantize, _fp4_gemm and _moe_combine on one
+ * workspace; the results are those of the calls. x, y: [tokens, hidden];
+ * gate, up: quantised [experts, inter, hidden]; down: [experts, hidden,
+ * inter]; up_alphas, down_alphas: fp32 [experts] or NULL. With experts or
+ * inter spread over PEs, y is this PE's part of the sum. workspace: 256-byte
+ * aligned, need not be initialised, one per concurrent call; events as the
+ * products'.
+ */
+megacu_status megacu_cuda_moe_mlp_fp4(megacu_driver_view driver, const void *x,
+                                      const void *expert_ids, const void *weights,
+                                      const void *gate, const void *gate_scales,
+                                      const void *up, const void *up_scales,
+                                      const void *down, const void *down_scales,
+                                      const void *up_alphas, const void *down_alphas,
+                                      void *y, void *workspace, void *events,
+                                      const megacu_moe_mlp_problem *problem);
+
 /* ---- team: symmetric heap over NVLink peer mappings ---------------------- */
 
 /* Size of the opaque handle a PE exports for its heap. */

@@ -92,6 +92,14 @@ class Fp4GemmProblem(ctypes.Structure):
                 ("timeout_ns", c_uint64)]
 
 
+class MoeMlpProblem(ctypes.Structure):
+    _fields_ = [("tokens", c_int64), ("hidden", c_int64), ("inter", c_int64), ("topk", c_int32),
+                ("experts", c_int32), ("first_expert", c_int32), ("dtype", c_int32),
+                ("id_bytes", c_int32), ("format", c_int32), ("x_scale", ctypes.c_float),
+                ("act_scale", ctypes.c_float), ("up_alpha", ctypes.c_float),
+                ("down_alpha", ctypes.c_float), ("timeout_ns", c_uint64)]
+
+
 _PROTOTYPES = {
     # name: (restype, argtypes)
     "megacu_cuda_gemm_swiglu_bf16":
@@ -136,7 +144,9 @@ _PROTOTYPES = {
         (Status, [GemmArProblemV2, c_int32, c_int32, ctypes.POINTER(c_int32)]),
     "megacu_b200_events_status": (Status, [c_void_p, c_void_p, ctypes.POINTER(c_int64)]),
     "megacu_b200_events_counters": (Status, [c_void_p, c_void_p, ctypes.POINTER(c_uint64)]),
-    # The last argument of these is a pointer to MoeProblem / Fp4Matrix / Fp4GemmProblem.
+    # A problem structure of these is passed by pointer.
+    "megacu_b200_moe_mlp_workspace_bytes": (Status, [c_void_p, ctypes.POINTER(c_int64)]),
+    "megacu_cuda_moe_mlp_fp4": (Status, [DriverView, *[c_void_p] * 15]),
     "megacu_b200_moe_sizes": (Status, [c_void_p, ctypes.POINTER(c_int64)]),
     "megacu_cuda_moe_sort": (Status, [DriverView, *[c_void_p] * 7]),
     "megacu_cuda_moe_dispatch": (Status, [DriverView, *[c_void_p] * 4]),

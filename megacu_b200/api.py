@@ -824,6 +824,76 @@ def fp4_gemm_swiglu(a, a_scales, gate, gate_scales, up, up_scales, act, *, event
              a, a_scales, act, offsets, counts, alphas, events, problem, stream, device)
 
 
+@dataclass
+class MoeMlp(_CProblem):
+    """megacu_moe_mlp_problem: a routed MLP block with 4-bit weights (see
+    :func:`moe_mlp_fp4`)."""
+    tokens: int
+    hidden: int
+    inter: int          # this PE's slice of the intermediate size
+    topk: int
+    experts: int
+    first_expert: int = 0
+    dtype: int = _capi.DTYPE_BF16
+    format: int = _capi.FP4_MX
+    x_scale: float = 1.0
+    act_scale: float = 1.0
+    up_alpha: float = 1.0
+    down_alpha: float = 1.0
+    timeout_ns: int = 0
+
+    def _build(self, id_bytes: int = 0):
+        return _capi.MoeMlpProblem(
+            tokens=self.tokens, hidden=self.hidden, inter=self.inter, topk=self.topk,
+            experts=self.experts, first_expert=self.first_expert, dtype=self.dtype,
+            id_bytes=id_bytes, format=self.format, x_scale=self.x_scale,
+            act_scale=self.act_scale, up_alpha=self.up_alpha, down_alpha=self.down_alpha,
+            timeout_ns=self.timeout_ns)
+
+    _wide_ids = MoeProblem._wide_ids
+
+
+def moe_mlp_workspace_bytes(problem: MoeMlp) -> int:
+    sizes = problem.__dict__.get("_sizes")
+    if sizes is None:
+        out = ctypes.c_int64()
+        check(lib().megacu_b200_moe_mlp_workspace_bytes(problem._pointer(), ctypes.byref(out)))
+        sizes = problem.__dict__["_sizes"] = (out.value,)
+    return sizes[0]
+
+
+def moe_mlp_fp4(x, expert_ids, weights, gate, gate_scales, up, up_scales, down, down_scales, y, *,
+                workspace, events, problem: MoeMlp, up_alphas=None, down_alphas=None, stream=None,
+                device: int = 0) -> None:
+    """A routed MLP block (async): y[t] = sum over the choices j of token t whose
+    expert e is here of weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])),
+    on weights quantised by :func:`fp4_quantize`: ``gate``, ``up`` [experts,
+    inter, hidden], ``down`` [experts, hidden, inter]. The calls of this module
+    in a row on one ``workspace`` (moe_mlp_workspace_bytes(), uint8, 256-byte
+    aligned); with experts or inter spread over PEs, y is this PE's part of
+    the sum."""
+    p, where = problem, None if stream is None else device
+    wide = getattr(expert_ids, "dtype", None) is _TYPES["i64"]
+    slots = p.tokens * p.topk
+    need = moe_mlp_workspace_bytes(p)
+    up_shape = Fp4Gemm(0, p.inter, p.hidden, format=p.format)
+    down_shape = Fp4Gemm(0, p.hidden, p.inter, format=p.format)
+    check(lib().megacu_cuda_moe_mlp_fp4(
+        _launch_view(stream, device, None),
+        _matrix(x, "x", p.tokens, p.hidden, 0, p.dtype, where),
+        _buffer(expert_ids, "expert_ids", slots, "i64" if wide else "i32", where),
+        _buffer(weights, "weights", slots, _capi.DTYPE_F32, where),
+        *_operand(gate, gate_scales, "gate", p.experts, p.inter, up_shape, where),
+        *_operand(up, up_scales, "up", p.experts, p.inter, up_shape, where),
+        *_operand(down, down_scales, "down", p.experts, p.hidden, down_shape, where),
+        _buffer(up_alphas, "up_alphas", p.experts, _capi.DTYPE_F32, where),
+        _buffer(down_alphas, "down_alphas", p.experts, _capi.DTYPE_F32, where),
+        _matrix(y, "y", p.tokens, p.hidden, 0, p.dtype, where),
+        _buffer(workspace, "workspace", need, "u8", where),
+        _buffer(events, "events", 256, "u8", where),
+        p._wide_ids() if wide else p._pointer()))
+
+
 def events_status(events, stream=None) -> list[int]:
     """Synchronises ``stream`` and raises MegacuError if a device wait failed."""
     info = (ctypes.c_int64 * 4)()

@@ -552,3 +552,75 @@ def test_routed_mlp(tokens, fmt):
     res, mag = ref.combine(out_h, w, at.cpu())
     _assert_close(y.cpu(), res, topk * 2.0 ** -24 * mag, torch.bfloat16)
     mb.events_status(kw["events"], _stream())
+
+
+@pytest.mark.parametrize("ids_type", [torch.int32, torch.int64])
+@pytest.mark.parametrize("tokens,fmt,dtype", [(1, mb.FP4_MX, mb.DTYPE_BF16),
+                                              (37, mb.FP4_NV, mb.DTYPE_F16),
+                                              (700, mb.FP4_MX, mb.DTYPE_BF16)])
+def test_routed_mlp_block_is_its_calls(tokens, fmt, dtype, ids_type):
+    """moe_mlp_fp4 gives bit for bit what its calls give one by one, directly
+    and replayed from a graph, whatever its workspace holds before."""
+    gen = torch.Generator().manual_seed(tokens)
+    t = DTYPES[dtype]
+    topk, experts, first, hidden, inter = 3, 6, 2, 320, 160
+    ids = torch.randint(0, experts + 3, (tokens, topk), generator=gen).to(ids_type).cuda()
+    x = torch.randn(tokens, hidden, generator=gen).to(t).cuda()
+    w = torch.rand(tokens, topk, generator=gen).cuda()
+
+    def weights(n, k):
+        parts = [ref.random_operand(gen, n, k, fmt) for _ in range(experts)]
+        return tuple(torch.cat([q[i] for q in parts]).cuda() for i in (0, 1))
+
+    gate, up, down = weights(inter, hidden), weights(inter, hidden), weights(hidden, inter)
+    alphas = (torch.rand(experts, generator=gen) + 0.5).cuda()
+    p = mb.MoeMlp(tokens, hidden, inter, topk, experts, first_expert=first, dtype=dtype,
+                  format=fmt, x_scale=2.0, act_scale=0.5, up_alpha=2.0 ** -5,
+                  down_alpha=2.0 ** -6)
+    events = torch.zeros(256, dtype=torch.uint8, device="cuda")
+    ws = torch.full((mb.moe_mlp_workspace_bytes(p),), 0xA5, dtype=torch.uint8, device="cuda")
+    y = torch.empty(tokens, hidden, dtype=t, device="cuda")
+
+    def block():
+        mb.moe_mlp_fp4(x, ids, w, *gate, *up, *down, y, workspace=ws, events=events, problem=p,
+                       up_alphas=alphas, down_alphas=None, stream=_stream())
+
+    block()
+    direct = y.clone()
+
+    route = mb.MoeProblem(tokens, topk, experts, hidden=hidden, first_expert=first, align=128,
+                          dtype=dtype)
+    rows = mb.moe_rows(route)
+    new = lambda *shape, u=torch.int32: torch.zeros(shape, dtype=u, device="cuda")
+    counts, offsets, at, slots = new(experts), new(experts + 1), new(tokens, topk), new(rows)
+    sort_ws = new(max(mb.moe_workspace_bytes(route), 1), u=torch.uint8)
+    kw = dict(stream=_stream())
+    mb.moe_sort(ids, counts=counts, offsets=offsets, row_of_slot=at, slot_of_row=slots,
+                workspace=sort_ws, problem=route, **kw)
+    xm = mb.Fp4Matrix(rows, hidden, format=fmt, dtype=dtype, scale=2.0)
+    am = mb.Fp4Matrix(rows, inter, format=fmt, dtype=dtype, scale=0.5)
+    xq, aq = _buffers(xm), _buffers(am)
+    mb.fp4_quantize(x, *xq, problem=xm, slot_of_row=slots, topk=topk, **kw)
+    act, out = new(rows, inter, u=t), new(rows, hidden, u=t)
+    group = dict(offsets=offsets, counts=counts, events=events, **kw)
+    mb.fp4_gemm_swiglu(*xq, *gate, *up, act, alphas=alphas, problem=mb.Fp4Gemm(
+        rows, inter, hidden, format=fmt, out_dtype=dtype, experts=experts, alpha=2.0 ** -6),
+        **group)
+    mb.fp4_quantize(act, *aq, problem=am, slot_of_row=slots, **kw)
+    mb.fp4_gemm(*aq, *down, out, problem=mb.Fp4Gemm(
+        rows, hidden, inter, format=fmt, out_dtype=dtype, experts=experts, alpha=2.0 ** -5),
+        **group)
+    want = torch.empty_like(y)
+    mb.moe_combine(out, want, weights=w, row_of_slot=at, problem=route, **kw)
+    assert torch.equal(direct, want) and direct.float().abs().max() > 0
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        block()
+    for _ in range(2):
+        ws.fill_(0x3C)
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    mb.events_status(events, _stream())

@@ -211,6 +211,42 @@ def test_products_refuse_storage():
     assert _status(fn, *[FAKE] * 11, p) == (2, 22)  # SwiGLU tiles are 128 gate + 128 up
 
 
+def _mlp(**kw):
+    base = dict(tokens=5, hidden=64, inter=96, topk=2, experts=4)
+    base.update(kw)
+    return mb.MoeMlp(**base).to_c()
+
+
+@pytest.mark.parametrize("bad,want", [
+    (dict(tokens=-1), (1, 1)), (dict(hidden=40), (1, 21)), (dict(inter=0), (1, 1)),
+    (dict(inter=33), (1, 21)), (dict(topk=0), (1, 1)), (dict(experts=1025), (2, 22)),
+    (dict(dtype=0), (2, 20)), (dict(format=2), (1, 1)), (dict(x_scale=3.0), (1, 1)),
+    (dict(act_scale=-1.0), (1, 1)), (dict(x_scale=0.0), (0, 0)), (dict(), (0, 0)),
+    (dict(tokens=0), (0, 0))])
+def test_routed_mlp_refuses(bad, want):
+    lib = _capi.load()
+    p = ctypes.byref(_mlp(**bad))
+    assert _status(lib.megacu_cuda_moe_mlp_fp4, *[FAKE] * 14, p) == want
+    st = lib.megacu_b200_moe_mlp_workspace_bytes(p, ctypes.byref(ctypes.c_int64()))
+    assert (st.code, st.detail) == want
+
+
+def test_routed_mlp_refuses_storage():
+    lib = _capi.load()
+    p = ctypes.byref(_mlp())
+    names = ("x", "expert_ids", "weights", "gate", "gate_scales", "up", "up_scales", "down",
+             "down_scales", "up_alphas", "down_alphas", "y", "workspace", "events")
+    for i, name in enumerate(names):
+        args = [FAKE] * 14
+        args[i] = None
+        want = (0, 0) if name.endswith("alphas") else (1, 2)
+        assert _status(lib.megacu_cuda_moe_mlp_fp4, *args, p) == want, name
+        args[i] = FAKE + 1
+        assert _status(lib.megacu_cuda_moe_mlp_fp4, *args, p) == (1, 21), name
+    empty = ctypes.byref(_mlp(tokens=0))
+    assert _status(lib.megacu_cuda_moe_mlp_fp4, *[None] * 14, empty) == (0, 0)
+
+
 def test_wrappers_check_tensors():
     """Shapes, types and strides of tensors are checked before the call."""
     p = mb.MoeProblem(4, 2, 3, hidden=8)
@@ -245,7 +281,8 @@ def test_struct_layouts(tmp_path):
         pytest.skip("no C compiler")
     from megacu_b200 import build
     structs = {"megacu_moe_problem": _capi.MoeProblem, "megacu_fp4_matrix": _capi.Fp4Matrix,
-               "megacu_fp4_gemm_problem": _capi.Fp4GemmProblem}
+               "megacu_fp4_gemm_problem": _capi.Fp4GemmProblem,
+               "megacu_moe_mlp_problem": _capi.MoeMlpProblem}
     lines, want = [], []
     for c_name, py in structs.items():
         lines.append(f'  printf("%zu\\n", sizeof({c_name}));')
