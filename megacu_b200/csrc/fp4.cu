@@ -381,6 +381,9 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
   if (m.topk > 0 && slot_of_row == nullptr) {
     return fail(MEGACU_INVALID_ARGUMENT, 2, "gathered rows need slot_of_row");
   }
+  if (m.topk > 0 && m.rows > 0 && m.x_rows == 0) {
+    return fail(MEGACU_INVALID_ARGUMENT, 1, "gathered rows need x_rows");
+  }
   if (m.rows == 0) return ok_status();
   if (x == nullptr || data == nullptr || scales == nullptr) {
     return fail(MEGACU_INVALID_ARGUMENT, 2, "missing storage");

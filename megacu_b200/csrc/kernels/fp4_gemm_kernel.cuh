@@ -384,8 +384,11 @@ __device__ __forceinline__ fp4_rows_out rows_out(fp4_gemm_params const &p, std::
   return {static_cast<std::uint8_t *>(p.out) + row * stride, stride, rows};
 }
 
+// silu(g) * u with exp(-|g|), which neither overflows nor drives the fast
+// division out of its range: g / (1 + e) for g >= 0, g e / (1 + e) below.
 __device__ __forceinline__ float swiglu(float g, float u) {
-  return __fdividef(g, 1.0f + __expf(-g)) * u;
+  float const e = __expf(-fabsf(g));
+  return __fdividef(g < 0.0f ? g * e : g, 1.0f + e) * u;
 }
 
 }  // namespace detail

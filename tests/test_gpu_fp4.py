@@ -358,6 +358,32 @@ def test_swiglu(m, n, k, fmt):
                 _assert_close(out.cpu(), want, err, t, split)
 
 
+@pytest.mark.parametrize("split", [1, 2])
+def test_swiglu_of_large_gates(split):
+    """Gates far from zero, both ways: alpha puts them between -90 and 90, where
+    exp(-g) nears the type's ends; the up products are ones."""
+    k, n = 512, 128
+    gen = torch.Generator().manual_seed(1)
+    gate = torch.randint(-3, 4, (n, k), generator=gen).double()
+    a = torch.zeros(40, k, dtype=torch.float64)
+    a[:, 0] = 1
+    a[:, 1] = torch.arange(40) % 7
+    up = torch.zeros(n, k, dtype=torch.float64)
+    up[:, 0] = 1
+    ops = [ref.pack(*ref.quantize(x, mb.FP4_MX)) for x in (a, gate, up)]
+    va, vg, vu = (ref.values(*x, mb.FP4_MX) for x in ops)
+    alpha = 4.0
+    g, u = alpha * va @ vg.T, alpha * va @ vu.T
+    assert g.min() < -80 and g.max() > 80
+    want = g * torch.where(g < 0, torch.exp(g), torch.ones_like(g)) / (1 + torch.exp(-g.abs())) * u
+    out = torch.empty(40, n, device="cuda")
+    _run(mb.fp4_gemm_swiglu, *(t for x in ops for t in _gpu(x)), out, problem=mb.Fp4Gemm(
+        40, n, k, out_dtype=mb.DTYPE_F32, alpha=alpha, split=split))
+    # the products are whole numbers: exact; then as _swiglu_want's last line
+    err = (g.abs() * 2.0 ** -22 + 2.0 ** -20) * want.abs()
+    _assert_close(out.cpu(), want, err, torch.float32)
+
+
 GROUPS = [  # counts per expert
     [1], [0, 5, 0, 0, 130, 1, 128, 0], [300, 0, 2], [0, 0, 0], [3] * 40,
     [0] * 70 + [129] + [0] * 29 + [1]]

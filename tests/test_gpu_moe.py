@@ -46,7 +46,7 @@ def _ids(kind, tokens, topk, total, seed):
 SORTS = [(1, 1, 1, 0, 1), (1, 8, 8, 0, 128), (64, 8, 128, 0, 128), (37, 3, 5, 2, 8),
          (1024, 1, 1024, 0, 1), (1025, 1, 33, 1, 16), (1023, 8, 64, 0, 128), (1024, 8, 7, 0, 1),
          (4097, 2, 256, 0, 128), (4096, 8, 1000, 100, 128), (5001, 7, 16, 3, 5),
-         (32768, 8, 3, 0, 1), (70001, 4, 300, 0, 1024)]
+         (32768, 8, 3, 0, 1), (70001, 4, 300, 0, 1024), (200003, 4, 1024, 7, 16)]
 
 
 @pytest.mark.parametrize("kind", ["random", "one", "none", "edges"])

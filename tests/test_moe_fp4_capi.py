@@ -157,6 +157,8 @@ def test_quantize_refuses_storage_and_options():
     t = _matrix()
     t.topk = 2
     assert _status(q, FAKE, None, FAKE, FAKE, ctypes.byref(t)) == (1, 2)
+    assert _status(q, FAKE, FAKE, FAKE, FAKE, ctypes.byref(t)) == (1, 1)
+    t.x_rows = 5
     assert _status(q, FAKE, FAKE, FAKE, FAKE, ctypes.byref(t)) == (0, 0)
     assert _status(d, FAKE, FAKE, FAKE, ctypes.byref(t)) == (2, 22)
     # a transposed matrix's stride is between its stored rows
