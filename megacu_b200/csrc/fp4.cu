@@ -255,6 +255,9 @@ megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &
       std::max(p.experts, 1) * p.n > kMaxDim) {
     return fail(MEGACU_UNSUPPORTED, 22, "dimension or number of experts too large");
   }
+  if (p.experts > 0 && p.m / kFp4BlockM > 0xffff) {
+    return fail(MEGACU_UNSUPPORTED, 22, "at most 65535 tiles of 128 rows by expert");
+  }
   if (p.experts > 0 && p.m % kFp4BlockM != 0) {
     return fail(MEGACU_UNSUPPORTED, 22, "rows by expert come in tiles of 128");
   }

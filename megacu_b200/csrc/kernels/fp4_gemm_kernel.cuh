@@ -52,6 +52,10 @@ inline constexpr int kFp4Threads = 64 + 32 * kFp4EpilogueWarps;
 inline constexpr int kFp4BlockM = 128;
 inline constexpr int kFp4BlockK = 256;  // elements per stage: one 128-byte swizzled row
 inline constexpr int kFp4SmallRows = 32;  // rows of the smaller A box
+// Experts whose places are kept in shared memory: each tile's place is looked up
+// before its loads, and four dependent global loads took 1.7 us, as long as
+// the stage ring lasts (3000 rows over 16 experts x 1001 x 1120: 15.0 us).
+inline constexpr int kFp4TableExperts = 256;
 // Bound of the waits that only let copies and MMAs in flight end after an error.
 inline constexpr unsigned long long kFp4DrainNs = 10000000ull;
 
@@ -82,6 +86,12 @@ struct fp4_gemm_params {
   unsigned long long timeout_ns;
 };
 
+// Where each expert's rows are, for at most kFp4TableExperts of them.
+struct fp4_expert_table {
+  std::int32_t end[kFp4TableExperts];            // offsets[e] + counts[e]
+  std::uint16_t first_tile[kFp4TableExperts + 4];  // offsets[e] / 128, experts + 1 entries
+};
+
 // kRows: rows of A that a stage holds, 128, or 32 for products of at most 32
 // rows; the MMA still reads 128, whatever follows, into accumulators that are
 // never stored.
@@ -97,10 +107,12 @@ struct fp4_config {
   // Bytes of a row that an epilogue warp stores at a time. 64 leave faster
   // than 32 (a 2048 x 1792 SwiGLU's last tile 2.7 against 3.2 us) but their
   // staging must not cost the fourth stage.
+  static constexpr int barrier_bytes = (2 * 15 + 2) * 8 + 16;  // of at most 15 stages
+  static constexpr int fixed_bytes = 1024 + barrier_bytes + sizeof(fp4_expert_table);
   static constexpr int segment =
-      BN == 256 && (232448 - 1280 - kFp4EpilogueWarps * 2048) / stage_bytes >= 4 ? 64 : 32;
+      BN == 256 && (232448 - fixed_bytes - kFp4EpilogueWarps * 2048) / stage_bytes >= 4 ? 64 : 32;
   static constexpr int staging_bytes = kFp4EpilogueWarps * 32 * segment;
-  static constexpr int overhead = 1024 + staging_bytes + 256;
+  static constexpr int overhead = fixed_bytes + staging_bytes;
   static constexpr int stages = (232448 - overhead) / stage_bytes;
   static constexpr int ring_bytes = stages * stage_bytes;
   static constexpr int smem_bytes = overhead + ring_bytes;
@@ -246,35 +258,46 @@ __host__ __device__ inline fp4_tile fp4_locate(std::int32_t t, std::int32_t m_ti
 
 namespace detail {
 
-// The expert whose rows hold `row` (whole warp; offsets ascend, the row is
-// below offsets[experts]): how many e have offsets[e + 1] <= row, by two
-// 32-wide counts.
-__device__ __forceinline__ std::int32_t find_expert(std::int32_t const *offsets,
-                                                    std::int32_t experts, std::int32_t row) {
+// The expert whose rows hold tile row `tile` (whole warp; the experts' first
+// tiles ascend, the row is below the last): how many e have first_tile(e + 1)
+// <= tile, by two 32-wide counts.
+template <class F>
+__device__ __forceinline__ std::int32_t find_expert(F const &first_tile, std::int32_t experts,
+                                                    std::int32_t tile) {
   std::int32_t const lane = static_cast<std::int32_t>(ptx::lane_id());
   std::int32_t const step = (experts + 31) / 32;
   std::int32_t const last = (lane + 1) * step;
-  bool const below = last <= experts && offsets[last] <= row;
+  bool const below = last <= experts && first_tile(last) <= tile;
   std::int32_t const base = __popc(__ballot_sync(0xffffffffu, below)) * step;
   std::int32_t const at = base + lane + 1;
-  bool const in = lane < step && at <= experts && offsets[at] <= row;
+  bool const in = lane < step && at <= experts && first_tile(at) <= tile;
   return min(base + __popc(__ballot_sync(0xffffffffu, in)), experts - 1);
 }
 
 // What one tile row needs besides its raster place (whole warp).
 struct fp4_rows {
   std::int32_t expert, valid;  // rows of the tile that exist
-  float alpha;
 };
 
-__device__ __forceinline__ fp4_rows locate_rows(fp4_gemm_params const &p, std::int32_t row) {
-  fp4_rows r{0, p.rows - row, p.alpha};
-  if (p.experts > 0) {
-    r.expert = find_expert(p.offsets, p.experts, row);
+__device__ __forceinline__ fp4_rows locate_rows(fp4_gemm_params const &p,
+                                                fp4_expert_table const &table, std::int32_t tile) {
+  std::int32_t const row = tile * kFp4BlockM;
+  fp4_rows r{0, p.rows - row};
+  if (p.experts > kFp4TableExperts) {
+    r.expert = find_expert([&](std::int32_t e) { return p.offsets[e] / kFp4BlockM; }, p.experts,
+                           tile);
     r.valid = min(r.valid, p.counts[r.expert] - (row - p.offsets[r.expert]));
-    if (p.alphas != nullptr) r.alpha *= p.alphas[r.expert];
+  } else if (p.experts > 0) {
+    r.expert = find_expert(
+        [&](std::int32_t e) { return static_cast<std::int32_t>(table.first_tile[e]); }, p.experts,
+        tile);
+    r.valid = min(r.valid, table.end[r.expert] - row);
   }
   return r;
+}
+
+__device__ __forceinline__ float locate_alpha(fp4_gemm_params const &p, std::int32_t expert) {
+  return p.alphas != nullptr && p.experts > 0 ? p.alpha * p.alphas[expert] : p.alpha;
 }
 
 __device__ __forceinline__ void fp4_error(std::uint32_t *events, std::uint32_t tile,
@@ -414,6 +437,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   std::uint64_t *const acc_full = empty + kStages;
   std::uint64_t *const acc_free = acc_full + 1;
   auto *const tmem_slot = reinterpret_cast<std::uint32_t *>(acc_free + 1);
+  auto &table = *reinterpret_cast<fp4_expert_table *>(staging + cfg::staging_bytes + cfg::barrier_bytes);
   std::uint32_t *const abort_word = &reinterpret_cast<control_block *>(p.events)->error_code;
 
   std::int32_t const warp =
@@ -450,7 +474,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     fp4_tile const c = locate(t);
     load_place l;
     l.row = c.row * kFp4BlockM;
-    detail::fp4_rows const rows = detail::locate_rows(p, l.row);
+    detail::fp4_rows const rows = detail::locate_rows(p, table, c.row);
     l.boxes = min(max((rows.valid + kFp4SmallRows - 1) / kFp4SmallRows, 1), kRows / kFp4SmallRows);
     if constexpr (kPair) l.boxes = 4;  // both CTAs' bytes are counted by the leader
     l.a_tile = min(c.row, m_tiles - 1) * p.scale_tiles;  // a pair's second tile may not exist
@@ -517,6 +541,28 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     ptx::fence_barrier_init();
     ptx::fence_proxy_async_shared();
   };
+  if (warp == 2 && ptx::elect_one()) {
+    ptx::prefetch_tensor_map(&maps.a);
+    ptx::prefetch_tensor_map(&maps.a_small);
+    ptx::prefetch_tensor_map(&maps.b);
+    ptx::prefetch_tensor_map(&maps.a_scales);
+    ptx::prefetch_tensor_map(&maps.b_scales);
+    if constexpr (kSwiglu) {
+      ptx::prefetch_tensor_map(&maps.b2);
+      ptx::prefetch_tensor_map(&maps.b2_scales);
+    }
+  }
+  if (!kPair && p.experts > 0) {
+    if (p.experts <= kFp4TableExperts) {
+      for (std::int32_t e = static_cast<std::int32_t>(threadIdx.x); e <= p.experts;
+           e += kFp4Threads) {
+        std::int32_t const offset = p.offsets[e];
+        table.first_tile[e] = static_cast<std::uint16_t>(offset / kFp4BlockM);
+        if (e < p.experts) table.end[e] = offset + p.counts[e];
+      }
+    }
+    __syncthreads();
+  }
   if (warp == 0) {
     if (ptx::elect_one()) set_up_barriers();
     __syncwarp();
@@ -655,8 +701,8 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     for (std::int32_t t = unit0; t < tiles; t += units, ++tile_index) {
       fp4_tile const c = locate(t);
       std::int32_t const row = c.row * kFp4BlockM;
-      detail::fp4_rows const rows = detail::locate_rows(p, row);
-      float const alpha = rows.alpha;
+      detail::fp4_rows const rows = detail::locate_rows(p, table, c.row);
+      float const alpha = detail::locate_alpha(p, rows.expert);
       detail::fp4_rows_out const out =
           detail::rows_out(p, row + quarter * 32, rows.valid - quarter * 32);
       if (!ptx::mbar_wait_cluster(acc_full, tile_index & 1u, abort_word, p.timeout_ns)) {
@@ -728,9 +774,9 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     float alpha = 1.0f;
     if (warp >= 2 && unit0 < tiles) {
       c = locate(unit0);
-      detail::fp4_rows const rows = detail::locate_rows(p, c.row * kFp4BlockM);
+      detail::fp4_rows const rows = detail::locate_rows(p, table, c.row);
       out = detail::rows_out(p, c.row * kFp4BlockM + quarter * 32, rows.valid - quarter * 32);
-      alpha = rows.alpha;
+      alpha = detail::locate_alpha(p, rows.expert);
     }
     if (out.rows > 0) {
       ptx::tc_fence_after_sync();
