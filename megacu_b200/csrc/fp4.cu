@@ -326,7 +326,10 @@ megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &
   prm.scale_tiles = static_cast<std::int32_t>(scale_tiles(p.k, nv));
   prm.out_dtype = p.out_dtype;
   prm.out_stride = p.out_stride != 0 ? p.out_stride : p.n;
-  prm.vec_store = aligned_to(out, 16) && prm.out_stride * element_size(p.out_dtype) % 16 == 0;
+  std::int64_t const row_bytes = prm.out_stride * element_size(p.out_dtype);
+  prm.row_bytes = aligned_to(out, 32) && row_bytes % 32 == 0   ? 32
+                  : aligned_to(out, 16) && row_bytes % 16 == 0 ? 16
+                                                               : 0;
   prm.alpha = p.alpha;
   prm.alphas = static_cast<float const *>(alphas);
   prm.offsets = static_cast<std::int32_t const *>(offsets);

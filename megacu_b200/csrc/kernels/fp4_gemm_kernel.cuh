@@ -75,7 +75,7 @@ struct fp4_gemm_params {
   std::int32_t split;        // CTAs of a cluster that share a tile's K
   std::int32_t scale_tiles;  // scale tiles per row tile
   std::int32_t out_dtype;    // MEGACU_DTYPE_*
-  std::int32_t vec_store;    // out rows allow 16-byte stores
+  std::int32_t row_bytes;    // 32, 16 or 0: what out's start and rows are multiples of
   std::int64_t out_stride;
   float alpha;
   float const *alphas;            // per expert, or nullptr
@@ -310,12 +310,17 @@ __device__ __forceinline__ void fp4_error(std::uint32_t *events, std::uint32_t t
   }
 }
 
-__device__ __forceinline__ std::uint32_t pack16(std::int32_t dtype, float lo, float hi) {
-  if (dtype == 1) {
-    __half2 const v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<std::uint32_t const *>(&v);
+// Word i of a row's elements in the output type.
+template <class Out, int kCount>
+__device__ __forceinline__ std::uint32_t out_word(float const (&v)[kCount], int i) {
+  if constexpr (std::is_same_v<Out, float>) {
+    return __float_as_uint(v[i]);
+  } else if constexpr (std::is_same_v<Out, __half>) {
+    __half2 const h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    return *reinterpret_cast<std::uint32_t const *>(&h);
+  } else {
+    return ptx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
   }
-  return ptx::pack_bf16x2(lo, hi);
 }
 
 // Where a warp's 32 rows of a tile go.
@@ -325,20 +330,36 @@ struct fp4_rows_out {
   std::int32_t rows;         // rows that exist
 };
 
-// Stores kCount consecutive columns from `col` of a warp's 32 rows (lane = row
-// on entry), kSegment bytes of each row at a time: turned through `stage` (no
-// bank conflicts) so that neighbouring lanes write a row's segment in 16-byte
-// pieces, or, where the rows do not allow 16-byte stores, its elements.
-template <bool kWide, int kSegment, int kCount>
+// Stores kCount consecutive columns from `col` of a warp's 32 rows (lane =
+// row). Rows of 32-byte pieces go straight from the registers, a whole sector
+// per lane (p.row_bytes = 32). Else kSegment bytes of each row at a time are
+// turned through `stage` (no bank conflicts), so that neighbouring lanes write
+// a row's segment in 16-byte pieces (p.row_bytes = 16) or its elements. The
+// turn alone takes as long as the MMAs of 512 of K, since shared memory is
+// busy with those (8192 x 4096 x 1024: 38 us with it, 23 without).
+template <class Out, int kSegment, int kCount>
 __device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uint32_t stage,
                                               float const (&v)[kCount], fp4_rows_out const &out,
                                               std::int32_t col) {
-  using element = std::conditional_t<kWide, std::uint32_t, std::uint16_t>;
-  constexpr int kSize = sizeof(element);
+  constexpr int kSize = sizeof(Out);
+  std::uint32_t const lane = ptx::lane_id();
+  if (p.row_bytes == 32 && col + kCount <= p.n) {
+    if (static_cast<std::int32_t>(lane) < out.rows) {
+      std::uint8_t *const dst =
+          out.base + lane * out.stride + static_cast<std::int64_t>(col) * kSize;
+#pragma unroll
+      for (int i = 0; i < kCount * kSize / 32; ++i) {
+        bytes32 q;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q.w[j] = out_word<Out>(v, i * 8 + j);
+        store32(dst + i * 32, q);
+      }
+    }
+    return;
+  }
   constexpr int kBytes = kCount * kSize < kSegment ? kCount * kSize : kSegment;
   constexpr int kCols = kBytes / kSize;
   constexpr std::uint32_t kPieces = kBytes / 16;
-  std::uint32_t const lane = ptx::lane_id();
   auto slot = [stage](std::uint32_t r, std::uint32_t c) {
     return stage + r * kBytes + ((c ^ (r * kPieces >> 3)) % kPieces) * 16;
   };
@@ -351,15 +372,13 @@ __device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uin
       std::uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        int const e = u * kCols + static_cast<int>(c) * (16 / kSize);
-        w[i] = kWide ? __float_as_uint(v[(e + i) % kCount])
-                     : pack16(p.out_dtype, v[(e + 2 * i) % kCount], v[(e + 2 * i + 1) % kCount]);
+        w[i] = out_word<Out>(v, (u * kBytes + static_cast<int>(c) * 16) / 4 + i);
       }
       ptx::st_shared_v4(slot(lane, c), w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
     std::uint8_t *const dst = out.base + static_cast<std::int64_t>(first) * kSize;
-    if (p.vec_store && first + kCols <= p.n) {
+    if (p.row_bytes >= 16 && first + kCols <= p.n) {
       uint4 q[kPieces];
 #pragma unroll
       for (std::uint32_t h = 0; h < kPieces; ++h) {
@@ -373,16 +392,20 @@ __device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uin
         }
       }
     } else {
-      // kCols lanes per row (16 or 32 of them: one column each; 8: a row's all).
+      // kCols lanes per row, an element each.
       std::uint32_t const e = lane % kCols, step = 32 / kCols;
       if (first + static_cast<std::int32_t>(e) < p.n) {
 #pragma unroll 4
         for (std::uint32_t r = lane / kCols; r < 32; r += step) {
           if (static_cast<std::int32_t>(r) >= out.rows) break;
           std::uint32_t const at = slot(r, e * kSize / 16) + e * kSize % 16;
-          element const x = kWide ? static_cast<element>(ptx::ld_shared_u32(at))
-                                  : static_cast<element>(ptx::ld_shared_u16(at));
-          *reinterpret_cast<element *>(dst + r * out.stride + e * kSize) = x;
+          if constexpr (kSize == 4) {
+            *reinterpret_cast<std::uint32_t *>(dst + r * out.stride + e * 4) =
+                ptx::ld_shared_u32(at);
+          } else {
+            *reinterpret_cast<std::uint16_t *>(dst + r * out.stride + e * 2) =
+                static_cast<std::uint16_t>(ptx::ld_shared_u16(at));
+          }
         }
       }
     }
@@ -395,9 +418,11 @@ __device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uin
                                               float const (&v)[kCount], fp4_rows_out const &out,
                                               std::int32_t col) {
   if (p.out_dtype == 3) {
-    store_columns<true, kSegment, kCount>(p, stage, v, out, col);
+    store_columns<float, kSegment, kCount>(p, stage, v, out, col);
+  } else if (p.out_dtype == 1) {
+    store_columns<__half, kSegment, kCount>(p, stage, v, out, col);
   } else {
-    store_columns<false, kSegment, kCount>(p, stage, v, out, col);
+    store_columns<__nv_bfloat16, kSegment, kCount>(p, stage, v, out, col);
   }
 }
 
