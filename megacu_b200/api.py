@@ -499,6 +499,7 @@ class _CProblem:
         object.__setattr__(self, name, value)
         self.__dict__.pop("_c", None)
         self.__dict__.pop("_sizes", None)
+        self.__dict__.pop("_need", None)
 
     def to_c(self):
         c = self.__dict__.get("_c")
@@ -508,7 +509,8 @@ class _CProblem:
         return c
 
     def _pointer(self):
-        self.to_c()
+        if "_c" not in self.__dict__:
+            self.to_c()
         return self.__dict__["_ref"]
 
 
@@ -782,26 +784,19 @@ def fp4_events_bytes() -> int:
     return out.value
 
 
-def _operand(data, scales, name: str, matrices: int, rows: int, p: Fp4Gemm, where: Optional[int]):
-    """Addresses of a quantised operand of ``matrices`` matrices [rows, k]."""
-    tiles = -(-p.k // (128 if p.format == _capi.FP4_MX else 64))
-    return (_buffer(data, name, matrices * rows * (p.k // 2), "u8", where),
-            _buffer(scales, name, matrices * -(-rows // 128) * tiles * 512, "u8", where))
+def _operand_bytes(matrices: int, rows: int, k: int, fmt: int) -> tuple[int, int]:
+    """Bytes of the data and scales of ``matrices`` quantised matrices [rows, k]."""
+    tiles = -(-k // (128 if fmt == _capi.FP4_MX else 64))
+    return matrices * rows * (k // 2), matrices * -(-rows // 128) * tiles * 512
 
 
-def _product(fn, weights, a, a_scales, out, offsets, counts, alphas, events, p: Fp4Gemm, stream,
-             device: int) -> None:
-    experts, where = max(p.experts, 1), None if stream is None else device
-    args = [*_operand(a, a_scales, "a", 1, p.m, p, where)]
-    for name, data, scales in weights:
-        args += _operand(data, scales, name, experts, p.n, p, where)
-    check(fn(_launch_view(stream, device, None), *args,
-             _buffer(offsets, "offsets", p.experts + 1, "i32", where),
-             _buffer(counts, "counts", p.experts, "i32", where),
-             _buffer(alphas, "alphas", p.experts, _capi.DTYPE_F32, where),
-             _matrix(out, "out", p.m, p.n, p.out_stride, p.out_dtype, where),
-             _buffer(events, "events", 256, "u8", where),
-             p._pointer()))
+def _product_needs(p: Fp4Gemm) -> tuple[int, int, int, int]:
+    """Bytes of A, of its scales, of one B operand and of its scales."""
+    need = p.__dict__.get("_need")
+    if need is None:
+        need = p.__dict__["_need"] = (*_operand_bytes(1, p.m, p.k, p.format),
+                                      *_operand_bytes(max(p.experts, 1), p.n, p.k, p.format))
+    return need
 
 
 def fp4_gemm(a, a_scales, b, b_scales, out, *, events, problem: Fp4Gemm, offsets=None,
@@ -810,8 +805,18 @@ def fp4_gemm(a, a_scales, b, b_scales, out, *, events, problem: Fp4Gemm, offsets
     accumulation and one rounding. By expert: ``offsets`` and ``counts`` of
     :func:`moe_sort` (align 128), ``alphas`` fp32 [experts] factors; rows
     without a slot are left as they were."""
-    _product(lib().megacu_cuda_fp4_gemm, [("b", b, b_scales)], a, a_scales, out, offsets, counts,
-             alphas, events, problem, stream, device)
+    p, where = problem, None if stream is None else device
+    need = _product_needs(p)
+    check(lib().megacu_cuda_fp4_gemm(
+        _launch_view(stream, device, None), _buffer(a, "a", need[0], "u8", where),
+        _buffer(a_scales, "a_scales", need[1], "u8", where),
+        _buffer(b, "b", need[2], "u8", where),
+        _buffer(b_scales, "b_scales", need[3], "u8", where),
+        _buffer(offsets, "offsets", p.experts + 1, "i32", where),
+        _buffer(counts, "counts", p.experts, "i32", where),
+        _buffer(alphas, "alphas", p.experts, _capi.DTYPE_F32, where),
+        _matrix(out, "out", p.m, p.n, p.out_stride, p.out_dtype, where),
+        _buffer(events, "events", 256, "u8", where), p._pointer()))
 
 
 def fp4_gemm_swiglu(a, a_scales, gate, gate_scales, up, up_scales, act, *, events,
@@ -820,8 +825,20 @@ def fp4_gemm_swiglu(a, a_scales, gate, gate_scales, up, up_scales, act, *, event
     """act = silu(alpha * A @ gate^T) * (alpha * A @ up^T) of quantised
     matrices (async); ``problem.n`` = act columns. By expert as
     :func:`fp4_gemm`."""
-    _product(lib().megacu_cuda_fp4_gemm_swiglu, [("gate", gate, gate_scales), ("up", up, up_scales)],
-             a, a_scales, act, offsets, counts, alphas, events, problem, stream, device)
+    p, where = problem, None if stream is None else device
+    need = _product_needs(p)
+    check(lib().megacu_cuda_fp4_gemm_swiglu(
+        _launch_view(stream, device, None), _buffer(a, "a", need[0], "u8", where),
+        _buffer(a_scales, "a_scales", need[1], "u8", where),
+        _buffer(gate, "gate", need[2], "u8", where),
+        _buffer(gate_scales, "gate_scales", need[3], "u8", where),
+        _buffer(up, "up", need[2], "u8", where),
+        _buffer(up_scales, "up_scales", need[3], "u8", where),
+        _buffer(offsets, "offsets", p.experts + 1, "i32", where),
+        _buffer(counts, "counts", p.experts, "i32", where),
+        _buffer(alphas, "alphas", p.experts, _capi.DTYPE_F32, where),
+        _matrix(act, "act", p.m, p.n, p.out_stride, p.out_dtype, where),
+        _buffer(events, "events", 256, "u8", where), p._pointer()))
 
 
 @dataclass
@@ -876,16 +893,19 @@ def moe_mlp_fp4(x, expert_ids, weights, gate, gate_scales, up, up_scales, down, 
     wide = getattr(expert_ids, "dtype", None) is _TYPES["i64"]
     slots = p.tokens * p.topk
     need = moe_mlp_workspace_bytes(p)
-    up_shape = Fp4Gemm(0, p.inter, p.hidden, format=p.format)
-    down_shape = Fp4Gemm(0, p.hidden, p.inter, format=p.format)
+    up_need = _operand_bytes(p.experts, p.inter, p.hidden, p.format)
+    down_need = _operand_bytes(p.experts, p.hidden, p.inter, p.format)
     check(lib().megacu_cuda_moe_mlp_fp4(
         _launch_view(stream, device, None),
         _matrix(x, "x", p.tokens, p.hidden, 0, p.dtype, where),
         _buffer(expert_ids, "expert_ids", slots, "i64" if wide else "i32", where),
         _buffer(weights, "weights", slots, _capi.DTYPE_F32, where),
-        *_operand(gate, gate_scales, "gate", p.experts, p.inter, up_shape, where),
-        *_operand(up, up_scales, "up", p.experts, p.inter, up_shape, where),
-        *_operand(down, down_scales, "down", p.experts, p.hidden, down_shape, where),
+        _buffer(gate, "gate", up_need[0], "u8", where),
+        _buffer(gate_scales, "gate_scales", up_need[1], "u8", where),
+        _buffer(up, "up", up_need[0], "u8", where),
+        _buffer(up_scales, "up_scales", up_need[1], "u8", where),
+        _buffer(down, "down", down_need[0], "u8", where),
+        _buffer(down_scales, "down_scales", down_need[1], "u8", where),
         _buffer(up_alphas, "up_alphas", p.experts, _capi.DTYPE_F32, where),
         _buffer(down_alphas, "down_alphas", p.experts, _capi.DTYPE_F32, where),
         _matrix(y, "y", p.tokens, p.hidden, 0, p.dtype, where),
