@@ -744,7 +744,10 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
         ptx::tc_fence_before_sync();
         if (lane == 0) {
           if constexpr (kPair) {
-            ptx::mbar_arrive_remote(free_bar);
+            // Relaxed: nothing of this thread's memory is published, the TMEM
+            // loads have completed, and a release would wait for the last
+            // tile's stores (1400 cycles of every tile).
+            ptx::mbar_arrive_remote_relaxed(free_bar);
           } else {
             ptx::mbar_arrive(acc_free);
           }

@@ -386,7 +386,9 @@ def test_swiglu_of_large_gates(split):
 
 GROUPS = [  # counts per expert
     [1], [0, 5, 0, 0, 130, 1, 128, 0], [300, 0, 2], [0, 0, 0], [3] * 40,
-    [0] * 70 + [129] + [0] * 29 + [1]]
+    [0] * 70 + [129] + [0] * 29 + [1],
+    [1300, 129, 1700, 0, 2000], [0, 900, 128, 2500],   # pairs of tiles, odd numbers of them
+    [1] * 299 + [130]]                                 # more than are kept on chip
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -415,9 +417,9 @@ def test_by_expert(counts, fmt):
     kw = dict(offsets=torch.tensor(offsets, dtype=torch.int32).cuda(),
               counts=torch.tensor(counts, dtype=torch.int32).cuda())
     for use_alphas in (True, False):
-        for split in (0, 1, 2):
+        for split, tile_n in ((0, 0), (1, 256), (2, 0)):
             p = mb.Fp4Gemm(m, n, k, format=fmt, out_dtype=mb.DTYPE_F32, experts=experts,
-                           alpha=0.5, split=split)
+                           alpha=0.5, split=split, tile_n=tile_n)
             al = dict(alphas=alphas.cuda()) if use_alphas else {}
             out = torch.full((m, n), -3.0, device="cuda")
             act = torch.full((m, n), -3.0, device="cuda")
