@@ -129,6 +129,14 @@ struct fp4_plan {
   std::int64_t m_tiles = 0, n_tiles = 0;
 };
 
+// Clusters of `split` CTAs, one CTA per SM, that run at once: an SM's cluster
+// stays within its GPC, and a B200's GPCs hold 33 clusters of 4 and 15 of 8
+// (the occupancy query's answer; 16 x 2048 x 4096 split in eight, 16 clusters,
+// took 11.6 us against 6.7 for 15).
+std::int64_t clusters_at_once(int split, int sms) {
+  return split == 8 ? 15 : split == 4 ? 33 : sms / split;
+}
+
 // Tile width and K split with the least time on the busiest SM, in us, fitted
 // to measured calls on a B200 (16 to 128 rows, N 8192, K 256 / 3584 / 14336):
 // a call's start-up and end, a k-block of 256 at each width (what an SM can
@@ -147,7 +155,8 @@ megacu_status make_plan(megacu_fp4_gemm_problem const &p, bool swiglu, int sms, 
       if (split > k_blocks || 16 * split > tile_n || (p.split != 0 && p.split != split)) continue;
       std::int64_t const m_tiles = ceil_div(p.m, kFp4BlockM);
       std::int64_t const n_tiles = ceil_div(p.n, swiglu ? tile_n / 2 : tile_n);
-      std::int64_t const waves = std::max<std::int64_t>(ceil_div(m_tiles * n_tiles * split, sms), 1);
+      std::int64_t const waves =
+          std::max<std::int64_t>(ceil_div(m_tiles * n_tiles, clusters_at_once(split, sms)), 1);
       double const rows = static_cast<double>(std::min<std::int64_t>(p.m, kFp4BlockM));
       double const exchange = split > 1 ? 1.5 + 0.035 * rows * tile_n / 256 : 0.0;
       double const cost = start + 0.6 * static_cast<double>(waves - 1) +
