@@ -193,24 +193,22 @@ cudaError_t launch_gemm(int device, int grid, cudaStream_t stream, fp4_maps cons
     if (e != cudaSuccess) return e;
     if (known) configured[device].store(true, std::memory_order_release);
   }
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  static std::atomic<int> max_pairs[kMaxDevices] = {};
-  int const cluster = kPair ? 2 : prm.split;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kFp4Threads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
   if constexpr (kPair) {
     // As many clusters as the device holds at once, each for several tiles.
+    static std::atomic<int> max_pairs[kMaxDevices] = {};
     int pairs = known ? max_pairs[device].load(std::memory_order_acquire) : 0;
     if (pairs == 0) {
+      cudaLaunchConfig_t cfg{};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
       cfg.gridDim = dim3(2);
+      cfg.blockDim = dim3(kFp4Threads);
+      cfg.dynamicSmemBytes = kSmem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
       cudaError_t const e = cudaOccupancyMaxActiveClusters(&pairs, kKernel, &cfg);
       if (e != cudaSuccess) return e;
       if (pairs < 1) return cudaErrorInvalidConfiguration;
@@ -218,8 +216,8 @@ cudaError_t launch_gemm(int device, int grid, cudaStream_t stream, fp4_maps cons
     }
     grid = std::min(grid, 2 * pairs);
   }
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  return cudaLaunchKernelEx(&cfg, kKernel, maps, prm);
+  return launch_chained(kKernel, static_cast<unsigned>(grid), kFp4Threads, kSmem, stream,
+                        static_cast<unsigned>(kPair ? 2 : prm.split), maps, prm);
 }
 
 template <bool kNv>
@@ -418,6 +416,10 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
   auto const grid =
       static_cast<unsigned>(2 * ceil_div(m.rows, kScaleTileRows) * prm.col_tiles);
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
+  cudaError_t e = cudaSuccess;
+  auto launch = [&](auto kernel, auto const *src) {
+    e = launch_chained(kernel, grid, kQuantThreads, 0, stream, 1, prm, src);
+  };
   by_type(m.dtype, m.format, [&](auto value, auto nv) {
     using T = decltype(value);
     auto const *src = static_cast<T const *>(x);
@@ -425,17 +427,16 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
     if (transpose) {
       // Pairs of columns are read together when every row starts on a pair.
       if (m.rows % 2 == 0 && prm.stride % 2 == 0 && aligned_to(x, 2 * size)) {
-        fp4_quantize_t_kernel<T, kNv, true><<<grid, kQuantThreads, 0, stream>>>(prm, src);
+        launch(fp4_quantize_t_kernel<T, kNv, true>, src);
       } else {
-        fp4_quantize_t_kernel<T, kNv, false><<<grid, kQuantThreads, 0, stream>>>(prm, src);
+        launch(fp4_quantize_t_kernel<T, kNv, false>, src);
       }
     } else if (prm.stride * size % 32 == 0 && aligned_to(x, 32)) {
-      fp4_quantize_kernel<T, kNv, true><<<grid, kQuantThreads, 0, stream>>>(prm, src);
+      launch(fp4_quantize_kernel<T, kNv, true>, src);
     } else {
-      fp4_quantize_kernel<T, kNv, false><<<grid, kQuantThreads, 0, stream>>>(prm, src);
+      launch(fp4_quantize_kernel<T, kNv, false>, src);
     }
   });
-  cudaError_t const e = cudaGetLastError();
   return e == cudaSuccess ? ok_status() : cuda_fail(e, 14);
 }
 
@@ -469,18 +470,16 @@ extern "C" megacu_status megacu_cuda_fp4_dequantize(megacu_driver_view driver, v
   auto const grid = static_cast<unsigned>(ceil_div(m.rows, kQuantRows) * prm.col_tiles);
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
   bool const vec = prm.stride * size % 32 == 0 && aligned_to(out, 32);
+  cudaError_t e = cudaSuccess;
   by_type(m.dtype, m.format, [&](auto value, auto nv) {
     using T = decltype(value);
     constexpr bool kNv = decltype(nv)::value;
-    if (vec) {
-      fp4_dequantize_kernel<T, kNv, true><<<grid, kQuantThreads, 0, stream>>>(
-          prm, static_cast<T *>(out));
-    } else {
-      fp4_dequantize_kernel<T, kNv, false><<<grid, kQuantThreads, 0, stream>>>(
-          prm, static_cast<T *>(out));
-    }
+    auto *const dst = static_cast<T *>(out);
+    e = vec ? launch_chained(fp4_dequantize_kernel<T, kNv, true>, grid, kQuantThreads, 0, stream,
+                             1, prm, dst)
+            : launch_chained(fp4_dequantize_kernel<T, kNv, false>, grid, kQuantThreads, 0, stream,
+                             1, prm, dst);
   });
-  cudaError_t const e = cudaGetLastError();
   return e == cudaSuccess ? ok_status() : cuda_fail(e, 14);
 }
 

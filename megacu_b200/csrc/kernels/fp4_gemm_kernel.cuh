@@ -40,6 +40,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "chained.cuh"
 #include "fp4_format.cuh"
 #include "layout.h"
 #include "sm100_ptx.cuh"
@@ -336,7 +337,7 @@ struct fp4_rows_out {
 // turned through `stage` (no bank conflicts), so that neighbouring lanes write
 // a row's segment in 16-byte pieces (p.row_bytes = 16) or its elements. The
 // turn alone takes as long as the MMAs of 512 of K, since shared memory is
-// busy with those (8192 x 4096 x 1024: 38 us with it, 23 without).
+// busy with those (8192 x 4096 x 1024: 38 us with it, 28 without).
 template <class Out, int kSegment, int kCount>
 __device__ __forceinline__ void store_columns(fp4_gemm_params const &p, std::uint32_t stage,
                                               float const (&v)[kCount], fp4_rows_out const &out,
@@ -478,12 +479,48 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   std::int32_t const k_blocks = (p.k + kFp4BlockK - 1) / kFp4BlockK;
   std::int32_t const kb0 = kPair ? 0 : rank * k_blocks / split;
   std::int32_t const kb1 = kPair ? k_blocks : (rank + 1) * k_blocks / split;
+  bool const leader = !kPair || rank == 0;
+
+  // Set-up that reads nothing of earlier kernels.
+  grid_start_next();
+  if (warp == 0) {
+    // Lane s sets up stage s (kStages <= 15).
+    if (lane < kStages) {
+      ptx::mbar_init(&full[lane], 1);
+      ptx::mbar_init(&empty[lane], 1);
+    } else if (lane == 16) {
+      ptx::mbar_init(acc_full, 1);
+      ptx::mbar_init(acc_free, kFp4EpilogueWarps * (kPair ? 2 : 1));
+    }
+    ptx::fence_barrier_init();
+    ptx::fence_proxy_async_shared();
+    __syncwarp();
+  } else if (warp == 1) {
+    if constexpr (kPair) {
+      ptx::tmem_alloc_pair(tmem_slot, cfg::tmem_columns);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, cfg::tmem_columns);
+      ptx::tmem_relinquish();
+    }
+  } else if (warp == 2 && ptx::elect_one()) {
+    ptx::prefetch_tensor_map(&maps.a);
+    ptx::prefetch_tensor_map(&maps.a_small);
+    ptx::prefetch_tensor_map(&maps.b);
+    ptx::prefetch_tensor_map(&maps.a_scales);
+    ptx::prefetch_tensor_map(&maps.b_scales);
+    if constexpr (kSwiglu) {
+      ptx::prefetch_tensor_map(&maps.b2);
+      ptx::prefetch_tensor_map(&maps.b2_scales);
+    }
+  }
+  grid_wait();
+
   std::int32_t const m_tiles =
       p.experts > 0 ? min(p.offsets[p.experts] / kFp4BlockM, p.m_tiles) : p.m_tiles;
   // Rows of tiles as the raster counts them: pairs of 128-row tiles, or tiles.
   std::int32_t const unit_rows = kPair ? (m_tiles + 1) / 2 : m_tiles;
   std::int32_t const tiles = unit_rows * p.n_tiles;
-  bool const leader = !kPair || rank == 0;
   // The 128-row tile of this CTA and the column tile of unit t.
   auto locate = [&](std::int32_t t) {
     fp4_tile c = fp4_locate(t, unit_rows, p.n_tiles, p.group_m);
@@ -556,27 +593,6 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   };
 
   std::uint32_t issued = 0;  // by the producer, in all
-  auto set_up_barriers = [&] {
-    for (std::uint32_t s = 0; s < kStages; ++s) {
-      ptx::mbar_init(&full[s], 1);
-      ptx::mbar_init(&empty[s], 1);
-    }
-    ptx::mbar_init(acc_full, 1);
-    ptx::mbar_init(acc_free, kFp4EpilogueWarps * (kPair ? 2 : 1));
-    ptx::fence_barrier_init();
-    ptx::fence_proxy_async_shared();
-  };
-  if (warp == 2 && ptx::elect_one()) {
-    ptx::prefetch_tensor_map(&maps.a);
-    ptx::prefetch_tensor_map(&maps.a_small);
-    ptx::prefetch_tensor_map(&maps.b);
-    ptx::prefetch_tensor_map(&maps.a_scales);
-    ptx::prefetch_tensor_map(&maps.b_scales);
-    if constexpr (kSwiglu) {
-      ptx::prefetch_tensor_map(&maps.b2);
-      ptx::prefetch_tensor_map(&maps.b2_scales);
-    }
-  }
   if (!kPair && p.experts > 0) {
     if (p.experts <= kFp4TableExperts) {
       for (std::int32_t e = static_cast<std::int32_t>(threadIdx.x); e <= p.experts;
@@ -588,25 +604,13 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     }
     __syncthreads();
   }
-  if (warp == 0) {
-    if (ptx::elect_one()) set_up_barriers();
+  if (!kPair && warp == 0 && unit0 < tiles) {
+    load_place const l = place(unit0);
+    issued = static_cast<std::uint32_t>(min(kb1 - kb0, static_cast<std::int32_t>(kStages)));
+    if (ptx::elect_one()) {
+      for (std::uint32_t s = 0; s < issued; ++s) load(l, kb0 + static_cast<std::int32_t>(s), s);
+    }
     __syncwarp();
-    if (!kPair && unit0 < tiles) {
-      load_place const l = place(unit0);
-      issued = static_cast<std::uint32_t>(min(kb1 - kb0, static_cast<std::int32_t>(kStages)));
-      if (ptx::elect_one()) {
-        for (std::uint32_t s = 0; s < issued; ++s) load(l, kb0 + static_cast<std::int32_t>(s), s);
-      }
-      __syncwarp();
-    }
-  } else if (warp == 1) {
-    if constexpr (kPair) {
-      ptx::tmem_alloc_pair(tmem_slot, cfg::tmem_columns);
-      ptx::tmem_relinquish_pair();
-    } else {
-      ptx::tmem_alloc(tmem_slot, cfg::tmem_columns);
-      ptx::tmem_relinquish();
-    }
   }
   ptx::tc_fence_before_sync();
   __syncthreads();

@@ -19,6 +19,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "chained.cuh"
 #include "fp4_format.cuh"
 #include "vec.cuh"
 
@@ -267,6 +268,8 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_quantize_kernel(fp4_matrix_
   constexpr int kPasses = kQuantRows / 16;
   // [tile][row] of four scale bytes: whole matrices in the scale tile's order
   __shared__ alignas(16) std::uint32_t bytes[kTiles][kQuantRows];
+  grid_start_next();
+  grid_wait();
   constexpr int kSlices = kScaleTileRows / kQuantRows;
   constexpr int kPer = kQuantRows / 4;  // rows of each quarter
   std::uint32_t const rows_cta = blockIdx.x / p.col_tiles;
@@ -361,6 +364,8 @@ __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_ma
   constexpr int kTiles = kQuantCols / kTileCols;
   constexpr int kBlock = fp4_block(kNv);
   constexpr int kWordBlock = kBlock * sizeof(T) / 4;
+  grid_start_next();
+  grid_wait();
   // [tile][row % 32][row / 32] of four scale bytes
   __shared__ std::uint32_t bytes[kTiles][32][2];
   __shared__ uint4 turned[kQuantTRows][8];
@@ -456,6 +461,8 @@ __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_ma
 // The values: element * scale / g, rounded once. A thread decodes 16 elements.
 template <class T, bool kNv, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matrix_params p, T *y) {
+  grid_start_next();
+  grid_wait();
   std::uint32_t const per_row = static_cast<std::uint32_t>(p.cols) / 16;
   std::uint32_t const rows_cta = blockIdx.x / p.col_tiles;
   std::uint32_t const i = (blockIdx.x - rows_cta * p.col_tiles) * 16 + threadIdx.x % 16;

@@ -13,6 +13,7 @@
 
 #include <cstdint>
 
+#include "chained.cuh"
 #include "vec.cuh"
 
 namespace megacu_b200 {
@@ -59,8 +60,9 @@ __device__ __forceinline__ void clear_rows(moe_sort_params const &p) {
 template <class Id>
 __global__ void __launch_bounds__(kMoeSortThreads) moe_count_kernel(moe_sort_params p) {
   extern __shared__ std::int32_t moe_smem[];
-  asm volatile("griddepcontrol.launch_dependents;");
   for (int e = threadIdx.x; e < p.experts; e += blockDim.x) moe_smem[e] = 0;
+  grid_wait();
+  grid_start_next();  // past the wait: the second launch reads the ids before its own
   __syncthreads();
   std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
   std::int64_t const end = min(begin + p.chunk, p.slots);
@@ -120,6 +122,7 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_par
   std::int32_t const w0 = min(warp * part, here), w1 = min(w0 + part, here);
   std::int32_t *const mine = cursor + warp * experts;
   for (int e = lane; e < experts; e += 32) mine[e] = 0;
+  if (!chunked) grid_wait();
   if (chunked) {
     for (int e = tid; e < 2 * experts; e += threads) total[e] = 0;
   } else {
@@ -131,8 +134,8 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_par
     local[s] = static_cast<std::int16_t>(e);
     if (e >= 0) atomicAdd(&mine[e], 1);
   }
-  // The histograms of every chunk are complete past this point.
-  if (chunked) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (chunked) grid_wait();  // every chunk's histogram is complete
+  grid_start_next();
   __syncthreads();
 
   // total[e] = slots of e anywhere, start[e] = slots of e in earlier chunks.
@@ -247,6 +250,8 @@ inline constexpr int kDispatchThreads = 256;
 // per lane (94 us at the sizes above, 6.4 TB/s; 99 with 16).
 template <class T, int N>
 __global__ void moe_dispatch_kernel(moe_rows_params p, T const *x, T *rows) {
+  grid_start_next();
+  grid_wait();
   std::int64_t const t = blockIdx.x;
   std::int32_t const *const at = p.row_of_slot + t * p.topk;
   T const *const src = x + t * p.token_stride;
@@ -263,6 +268,8 @@ __global__ void moe_dispatch_kernel(moe_rows_params p, T const *x, T *rows) {
 // rounding. 95 us at the sizes above, 6.3 TB/s.
 template <class T, int N>
 __global__ void moe_combine_kernel(moe_rows_params p, T const *rows, float const *weights, T *y) {
+  grid_start_next();
+  grid_wait();
   std::int64_t const t = blockIdx.x;
   std::int32_t const *const at = p.row_of_slot + t * p.topk;
   float const *const w = weights == nullptr ? nullptr : weights + t * p.topk;
@@ -298,6 +305,8 @@ template <class T, int N>
 __global__ void moe_combine_grad_kernel(moe_rows_params p, T const *dy, T const *rows,
                                         float const *weights, T *drows, float *dweights) {
   __shared__ float partial[kGradThreads / 32][kGradGroup];
+  grid_start_next();
+  grid_wait();
   std::int64_t const t = blockIdx.x;
   std::int32_t const *const at = p.row_of_slot + t * p.topk;
   float const *const w = weights + t * p.topk;

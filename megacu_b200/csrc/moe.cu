@@ -103,24 +103,16 @@ cudaError_t launch_sort(moe_sort_params const &prm, std::int64_t chunks, int dev
     if (e != cudaSuccess) return e;
     if (known) configured[device].store(true, std::memory_order_release);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(chunks));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  auto const grid = static_cast<unsigned>(chunks);
   if (chunks > 1) {
-    cfg.dynamicSmemBytes = prm.experts * 4;
-    cudaError_t const e = cudaLaunchKernelEx(&cfg, moe_count_kernel<Id>, prm);
+    cudaError_t const e = launch_chained(moe_count_kernel<Id>, grid, threads,
+                                         static_cast<std::size_t>(prm.experts) * 4, stream, 1, prm);
     if (e != cudaSuccess) return e;
-    // The second launch starts while the first counts and waits for it inside.
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
   }
-  cfg.dynamicSmemBytes =
-      static_cast<std::size_t>(moe_place_smem(threads / 32, prm.experts, prm.chunk));
-  return cudaLaunchKernelEx(&cfg, moe_place_kernel<Id>, prm);
+  return launch_chained(moe_place_kernel<Id>, grid, threads,
+                        static_cast<std::size_t>(
+                            moe_place_smem(threads / 32, prm.experts, prm.chunk)),
+                        stream, 1, prm);
 }
 
 enum class rows_op { dispatch, combine, grad };
@@ -134,45 +126,41 @@ struct rows_buffers {
 };
 
 template <class T, int N>
-void launch_rows(rows_op op, moe_rows_params const &prm, rows_buffers const &b,
+cudaError_t launch_rows(rows_op op, moe_rows_params const &prm, rows_buffers const &b,
                  cudaStream_t stream) {
   auto const grid = static_cast<unsigned>(prm.tokens);
   int const most = op == rows_op::dispatch  ? kDispatchThreads
                    : op == rows_op::combine ? kCombineThreads
                                             : kGradThreads;
   int const threads = std::min(most, ((prm.hidden + N - 1) / N + 31) / 32 * 32);
+  auto const *const in = static_cast<T const *>(b.in);
+  auto *const out = static_cast<T *>(b.out);
   switch (op) {
     case rows_op::dispatch:
-      moe_dispatch_kernel<T, N><<<grid, threads, 0, stream>>>(
-          prm, static_cast<T const *>(b.in), static_cast<T *>(b.out));
-      break;
+      return launch_chained(moe_dispatch_kernel<T, N>, grid, threads, 0, stream, 1, prm, in, out);
     case rows_op::combine:
-      moe_combine_kernel<T, N><<<grid, threads, 0, stream>>>(
-          prm, static_cast<T const *>(b.in), b.weights, static_cast<T *>(b.out));
-      break;
-    case rows_op::grad:
-      moe_combine_grad_kernel<T, N><<<grid, threads, 0, stream>>>(
-          prm, static_cast<T const *>(b.in), static_cast<T const *>(b.rows), b.weights,
-          static_cast<T *>(b.out), b.dweights);
-      break;
+      return launch_chained(moe_combine_kernel<T, N>, grid, threads, 0, stream, 1, prm, in,
+                            b.weights, out);
+    default:
+      return launch_chained(moe_combine_grad_kernel<T, N>, grid, threads, 0, stream, 1, prm, in,
+                            static_cast<T const *>(b.rows), b.weights, out, b.dweights);
   }
 }
 
 // The widest access, up to 32 bytes for the dispatch and 16 for the calls
 // that hold several rows, that every row's start and length allow.
 template <class T>
-void launch_rows_typed(rows_op op, moe_rows_params const &prm, rows_buffers const &b, int bytes,
+cudaError_t launch_rows_typed(rows_op op, moe_rows_params const &prm, rows_buffers const &b, int bytes,
                        cudaStream_t stream) {
   if (bytes == 32 && op == rows_op::dispatch) {
-    moe_dispatch_kernel<T, 32 / sizeof(T)>
-        <<<static_cast<unsigned>(prm.tokens),
-           std::min<int>(kDispatchThreads, (prm.hidden * sizeof(T) / 32 + 31) / 32 * 32), 0,
-           stream>>>(prm, static_cast<T const *>(b.in), static_cast<T *>(b.out));
-  } else if (bytes >= 16) {
-    launch_rows<T, 16 / sizeof(T)>(op, prm, b, stream);
-  } else {
-    launch_rows<T, 1>(op, prm, b, stream);
+    int const vectors = static_cast<int>(prm.hidden * sizeof(T) / 32);
+    return launch_chained(moe_dispatch_kernel<T, 32 / sizeof(T)>,
+                          static_cast<unsigned>(prm.tokens),
+                          std::min(kDispatchThreads, (vectors + 31) / 32 * 32), 0, stream, 1, prm,
+                          static_cast<T const *>(b.in), static_cast<T *>(b.out));
   }
+  if (bytes >= 16) return launch_rows<T, 16 / sizeof(T)>(op, prm, b, stream);
+  return launch_rows<T, 1>(op, prm, b, stream);
 }
 
 megacu_status run_rows(rows_op op, megacu_driver_view const &driver, rows_buffers const &b,
@@ -208,12 +196,10 @@ megacu_status run_rows(rows_op op, megacu_driver_view const &driver, rows_buffer
   };
   int const vec = fits(32) ? 32 : fits(16) ? 16 : 0;
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
-  switch (p->dtype) {
-    case MEGACU_DTYPE_F16: launch_rows_typed<__half>(op, prm, b, vec, stream); break;
-    case MEGACU_DTYPE_BF16: launch_rows_typed<__nv_bfloat16>(op, prm, b, vec, stream); break;
-    default: launch_rows_typed<float>(op, prm, b, vec, stream); break;
-  }
-  cudaError_t const e = cudaGetLastError();
+  cudaError_t const e =
+      p->dtype == MEGACU_DTYPE_F16    ? launch_rows_typed<__half>(op, prm, b, vec, stream)
+      : p->dtype == MEGACU_DTYPE_BF16 ? launch_rows_typed<__nv_bfloat16>(op, prm, b, vec, stream)
+                                      : launch_rows_typed<float>(op, prm, b, vec, stream);
   return e == cudaSuccess ? ok_status() : cuda_fail(e, 14);
 }
 

@@ -652,3 +652,52 @@ def test_routed_mlp_block_is_its_calls(tokens, fmt, dtype, ids_type):
         torch.cuda.synchronize()
         assert torch.equal(y, want)
     mb.events_status(events, _stream())
+
+
+def test_calls_in_a_row_wait_for_one_another():
+    """Launches overlap their set-up with the kernel before them; their work
+    must not. Blocks that feed one another in place, with nothing between them,
+    give what they give with a synchronisation after every one."""
+    gen = torch.Generator().manual_seed(12)
+    tokens, topk, experts, hidden, inter, steps = 600, 4, 8, 256, 192, 12
+    ids = torch.rand(steps, tokens, experts, generator=gen).topk(topk, -1).indices.cuda()
+    start = torch.randn(tokens, hidden, generator=gen).to(torch.bfloat16).cuda()
+    w = torch.softmax(torch.randn(tokens, topk, generator=gen), -1).cuda()
+
+    def weights(n, k):
+        parts = [ref.random_operand(gen, n, k, 0) for _ in range(experts)]
+        return tuple(torch.cat([q[i] for q in parts]).cuda() for i in (0, 1))
+
+    gate, up, down = weights(inter, hidden), weights(inter, hidden), weights(hidden, inter)
+    p = mb.MoeMlp(tokens, hidden, inter, topk, experts, up_alpha=2.0 ** -5, down_alpha=2.0 ** -5)
+    dense = mb.Fp4Gemm(tokens, hidden, hidden, alpha=2.0 ** -5)
+    m = mb.Fp4Matrix(tokens, hidden)
+    square = _gpu(ref.random_operand(gen, hidden, hidden, 0))
+
+    def run(sync):
+        x, events = start.clone(), torch.zeros(256, dtype=torch.uint8, device="cuda")
+        ws = torch.empty(mb.moe_mlp_workspace_bytes(p), dtype=torch.uint8, device="cuda")
+        data, scales = _buffers(m)
+        torch.cuda.synchronize()
+        for i in range(steps):
+            mb.moe_mlp_fp4(x, ids[i], w, *gate, *up, *down, x, workspace=ws, events=events,
+                           problem=p, stream=_stream())
+            if sync:
+                torch.cuda.synchronize()
+            mb.fp4_quantize(x, data, scales, problem=m, stream=_stream())
+            if sync:
+                torch.cuda.synchronize()
+            mb.fp4_gemm(data, scales, *square, x, events=events, problem=dense, stream=_stream())
+            # Another library's kernels between them. Without a norm x would
+            # overflow in both runs: the operands' elements are about 10, so a
+            # block multiplies x^2 by about 50.
+            x /= x.abs().amax()
+            if sync:
+                torch.cuda.synchronize()
+        mb.events_status(events, _stream())
+        return x.clone()
+
+    want = run(True)
+    assert torch.isfinite(want.float()).all() and want.float().abs().max() > 0
+    for _ in range(5):
+        assert torch.equal(run(False), want)
