@@ -413,6 +413,8 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
   fp4_matrix_params prm = matrix_params(m, log2_scale, data, scales, transpose);
   prm.slot_of_row = static_cast<std::int32_t const *>(slot_of_row);
   static_assert(kScaleTileRows == 2 * kQuantRows && kQuantRows == kQuantTRows, "two CTAs deep");
+  bool const masked = slot_of_row != nullptr;
+  if (masked) prm.col_tiles = (prm.col_tiles + kMaskedSpan - 1) / kMaskedSpan;
   auto const grid =
       static_cast<unsigned>(2 * ceil_div(m.rows, kScaleTileRows) * prm.col_tiles);
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
@@ -432,9 +434,11 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
         launch(fp4_quantize_t_kernel<T, kNv, false>, src);
       }
     } else if (prm.stride * size % 32 == 0 && aligned_to(x, 32)) {
-      launch(fp4_quantize_kernel<T, kNv, true>, src);
+      masked ? launch(fp4_quantize_kernel<T, kNv, true, true>, src)
+             : launch(fp4_quantize_kernel<T, kNv, true, false>, src);
     } else {
-      launch(fp4_quantize_kernel<T, kNv, false>, src);
+      masked ? launch(fp4_quantize_kernel<T, kNv, false, true>, src)
+             : launch(fp4_quantize_kernel<T, kNv, false, false>, src);
     }
   });
   return e == cudaSuccess ? ok_status() : cuda_fail(e, 14);
