@@ -472,9 +472,50 @@ __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_ma
   }
 }
 
-// The values: element * scale / g, rounded once. A thread decodes 16 elements.
+// 16 elements of the type.
+template <class T>
+struct alignas(32) fp4_plain {
+  T v[16];
+};
+
+// Elements times s1 and, for kTwo, s2: the first product is exact then, the
+// second rounds once.
+template <class T, bool kTwo>
+__device__ __forceinline__ fp4_plain<T> decode16(uint2 d, float s1, float s2) {
+  fp4_plain<T> out;
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    __half2 h[4];
+    from_e2m1x8(b == 0 ? d.x : d.y, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 f = __half22float2(h[i]);
+      f.x *= s1;
+      f.y *= s1;
+      if constexpr (kTwo) {
+        f.x *= s2;
+        f.y *= s2;
+      }
+      out.v[8 * b + 2 * i] = from_f32<T>(f.x);
+      out.v[8 * b + 2 * i + 1] = from_f32<T>(f.y);
+    }
+  }
+  return out;
+}
+
+// MX scales that with 1 / g are no normal power of two, and NaN. A call, so
+// that ordinary blocks do not pay for it.
+template <class T>
+__device__ __noinline__ fp4_plain<T> decode_rare_mx(uint2 d, int e, bool nan) {
+  float const s1 = nan ? __int_as_float(0x7fffffff) : pow2(e < 0 ? -100 : 100);
+  return decode16<T, true>(d, s1, nan ? 1.0f : pow2(e < 0 ? e + 100 : e - 100));
+}
+
+// The values: element * scale / g, rounded once. A thread decodes 16 elements
+// of each of four rows, whose loads are all in flight.
 template <class T, bool kNv, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matrix_params p, T *y) {
+  constexpr int kPasses = kQuantRows / 16;
   grid_start_next();
   grid_wait();
   std::uint32_t const per_row = static_cast<std::uint32_t>(p.cols) / 16;
@@ -483,43 +524,33 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matri
   if (i >= per_row) return;
   int const col = static_cast<int>(i) * 16;
   int const blk = col / fp4_block(kNv);
-  std::int64_t const row0 = static_cast<std::int64_t>(rows_cta) * kQuantRows;
+  std::int64_t const row0 =
+      static_cast<std::int64_t>(rows_cta) * kQuantRows + threadIdx.x / 16;
+  uint2 d[kPasses];
+  std::uint32_t byte[kPasses];
 #pragma unroll
-  for (int pass = 0; pass < kQuantRows / 16; ++pass) {
-    std::int64_t const row = row0 + pass * 16 + threadIdx.x / 16;
-    if (row >= p.rows) break;
-    uint2 const d = *reinterpret_cast<uint2 const *>(p.data + row * (p.cols / 2) + col / 2);
-    std::uint32_t const byte =
-        p.scales[((row / kScaleTileRows) * p.tiles + blk / 4) * kScaleTileBytes +
-                 scale_byte(static_cast<int>(row % kScaleTileRows), blk)];
-    // scale / g: one factor, or two where it is no normal power of two (the
-    // first product is exact, the second rounds once).
-    float s1, s2 = 1.0f;
-    if constexpr (kNv) {
-      s1 = from_e4m3(byte) * pow2(-p.log2_scale);
-    } else {
-      int const e = static_cast<int>(byte) - 127 - p.log2_scale;
-      bool const normal = e >= -126 && e <= 127;
-      s1 = pow2(normal ? e : e < 0 ? -100 : 100);
-      if (!normal) s2 = pow2(e < 0 ? e + 100 : e - 100);
-      if (byte == 0xffu) s1 = __int_as_float(0x7fffffff);
+  for (int pass = 0; pass < kPasses; ++pass) {
+    std::int64_t const row = row0 + pass * 16;
+    if (row < p.rows) {
+      d[pass] = *reinterpret_cast<uint2 const *>(p.data + row * (p.cols / 2) + col / 2);
+      byte[pass] = p.scales[((row / kScaleTileRows) * p.tiles + blk / 4) * kScaleTileBytes +
+                            scale_byte(static_cast<int>(row % kScaleTileRows), blk)];
     }
-    alignas(32) T out[16];
+  }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      __half2 h[4];
-      from_e2m1x8(b == 0 ? d.x : d.y, h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float2 f = __half22float2(h[i]);
-        f.x *= s1;
-        f.y *= s1;
-        if (!kNv && s2 != 1.0f) {
-          f.x *= s2;
-          f.y *= s2;
-        }
-        out[8 * b + 2 * i] = from_f32<T>(f.x);
-        out[8 * b + 2 * i + 1] = from_f32<T>(f.y);
+  for (int pass = 0; pass < kPasses; ++pass) {
+    std::int64_t const row = row0 + pass * 16;
+    if (row >= p.rows) break;
+    fp4_plain<T> out;
+    if constexpr (kNv) {
+      out = decode16<T, false>(d[pass], from_e4m3(byte[pass]) * pow2(-p.log2_scale), 1.0f);
+    } else {
+      int const e = static_cast<int>(byte[pass]) - 127 - p.log2_scale;
+      bool const nan = byte[pass] == 0xffu;
+      if (e >= -126 && e <= 127 && !nan) {
+        out = decode16<T, false>(d[pass], pow2(e), 1.0f);
+      } else {
+        out = decode_rare_mx<T>(d[pass], e, nan);
       }
     }
     T *const dst = y + row * p.stride + col;
@@ -527,11 +558,11 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_dequantize_kernel(fp4_matri
 #pragma unroll
       for (int c = 0; c < static_cast<int>(sizeof(T)) / 2; ++c) {
         store32(reinterpret_cast<char *>(dst) + 32 * c,
-                reinterpret_cast<bytes32 const *>(out)[c]);
+                reinterpret_cast<bytes32 const *>(out.v)[c]);
       }
     } else {
 #pragma unroll
-      for (int c = 0; c < 16; ++c) dst[c] = out[c];
+      for (int c = 0; c < 16; ++c) dst[c] = out.v[c];
     }
   }
 }
