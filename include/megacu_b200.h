@@ -540,6 +540,9 @@ typedef struct megacu_fp4_matrix {
   int32_t transpose; /* 1: the plain matrix is stored [cols, rows] */
   int32_t topk;      /* > 0: row r is the plain matrix's row slot_of_row[r] / topk */
   float scale;       /* g, a power of two from 2^-60 to 2^60; 1 = none */
+  int32_t scatter;   /* 1 (topk > 0): the index is row_of_slot [x_rows, topk] instead:
+                        each row of x is quantised once and written to every
+                        row it names; the same bytes as the gather's */
 } megacu_fp4_matrix;
 
 /* sizes[0] bytes of data, sizes[1] bytes of scales. */
@@ -555,7 +558,8 @@ megacu_status megacu_b200_fp4_sizes(const megacu_fp4_matrix *matrix, int64_t siz
  * the last row or column of a tile are 0. With slot_of_row (int32 [rows], as
  * megacu_cuda_moe_sort writes it) rows whose entry is negative are left as
  * they were, scales included, and x is gathered when topk > 0 (an entry that
- * names no row of x counts as negative); NULL: every row.
+ * names no row of x counts as negative); NULL: every row. With scatter the
+ * index is row_of_slot, and entries outside [0, rows) name no row.
  */
 megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, const void *x,
                                        const void *slot_of_row, void *data, void *scales,
@@ -638,7 +642,7 @@ megacu_status megacu_b200_moe_mlp_workspace_bytes(const megacu_moe_mlp_problem *
 /*
  * A routed MLP block: for every token t and choice j whose expert e is here,
  *   y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t]))
- * as megacu_cuda_moe_sort (align 128), _fp4_quantize (gathered),
+ * as megacu_cuda_moe_sort (align 128), _fp4_quantize (scattered),
  * _fp4_gemm_swiglu, _fp4_quantize, _fp4_gemm and _moe_combine on one
  * workspace; the results are those of the calls. x, y: [tokens, hidden];
  * gate, up: quantised [experts, inter, hidden]; down: [experts, hidden,

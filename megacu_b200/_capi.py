@@ -82,7 +82,7 @@ class MoeProblem(ctypes.Structure):
 class Fp4Matrix(ctypes.Structure):
     _fields_ = [("rows", c_int64), ("cols", c_int64), ("stride", c_int64), ("x_rows", c_int64),
                 ("format", c_int32), ("dtype", c_int32), ("transpose", c_int32), ("topk", c_int32),
-                ("scale", ctypes.c_float)]
+                ("scale", ctypes.c_float), ("scatter", c_int32)]
 
 
 class Fp4GemmProblem(ctypes.Structure):

@@ -695,11 +695,11 @@ class Fp4Matrix(_CProblem):
     scale: float = 1.0
     stride: int = 0
 
-    def _build(self, topk: int = 0, x_rows: int = 0):
+    def _build(self, topk: int = 0, x_rows: int = 0, scatter: int = 0):
         return _capi.Fp4Matrix(rows=self.rows, cols=self.cols, stride=self.stride, x_rows=x_rows,
                                format=self.format, dtype=self.dtype,
                                transpose=1 if self.transpose else 0, topk=topk,
-                               scale=self.scale)
+                               scale=self.scale, scatter=scatter)
 
 
 def fp4_sizes(problem: Fp4Matrix) -> tuple[int, int]:
@@ -712,20 +712,24 @@ def fp4_sizes(problem: Fp4Matrix) -> tuple[int, int]:
     return sizes
 
 
-def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, topk: int = 0,
-                 x_rows: int = 0, stream=None, device: int = 0) -> None:
+def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, row_of_slot=None,
+                 topk: int = 0, x_rows: int = 0, stream=None, device: int = 0) -> None:
     """Quantises ``x`` into ``data`` and ``scales`` (async). With
     ``slot_of_row`` (of :func:`moe_sort`, int32 [rows]) rows whose entry is
     negative are left as they were; with ``topk`` too, row r is taken from
-    x[slot_of_row[r] // topk] (``x_rows``: the rows of ``x``, needed only when
-    ``x`` is a raw address)."""
+    x[slot_of_row[r] // topk]. With ``row_of_slot`` ([x rows, topk]) instead,
+    each row of ``x`` is quantised once and written to the rows of its choices:
+    the same bytes, sooner when topk > 1. ``x_rows``: the rows of ``x``, needed
+    only when ``x`` is a raw address and topk > 0."""
+    if slot_of_row is not None and row_of_slot is not None:
+        raise ValueError("slot_of_row or row_of_slot, not both")
     p, where = problem, None if stream is None else device
     nbytes, sbytes = fp4_sizes(p)
     if topk:
         if x_rows == 0 and x is not None and x.__class__ is not int:
             x_rows = x.shape[0]
         x_ptr = _matrix(x, "x", x_rows, p.cols, p.stride, p.dtype, where)
-        key = (topk, x_rows)
+        key = (topk, x_rows, 0 if row_of_slot is None else 1)
         gathered = p.__dict__.get("_gathered")
         if gathered is None or gathered[0] is not p.to_c() or gathered[1] != key:
             gathered = p.__dict__["_gathered"] = (p.to_c(), key, ctypes.byref(p._build(*key)))
@@ -736,7 +740,8 @@ def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, topk:
         pointer = p._pointer()
     check(lib().megacu_cuda_fp4_quantize(
         _launch_view(stream, device, None), x_ptr,
-        _buffer(slot_of_row, "slot_of_row", p.rows, "i32", where),
+        _buffer(slot_of_row, "slot_of_row", p.rows, "i32", where) if row_of_slot is None else
+        _buffer(row_of_slot, "row_of_slot", x_rows * topk, "i32", where),
         _buffer(data, "data", nbytes, "u8", where),
         _buffer(scales, "scales", sbytes, "u8", where), pointer))
 

@@ -391,6 +391,9 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
   if (transpose && (slot_of_row != nullptr || m.topk > 0)) {
     return fail(MEGACU_UNSUPPORTED, 22, "a transposed matrix is quantised whole");
   }
+  if (m.scatter != 0 && m.topk == 0) {
+    return fail(MEGACU_INVALID_ARGUMENT, 1, "scattered rows need topk");
+  }
   if (m.topk > 0 && slot_of_row == nullptr) {
     return fail(MEGACU_INVALID_ARGUMENT, 2, "gathered rows need slot_of_row");
   }
@@ -413,10 +416,14 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
   fp4_matrix_params prm = matrix_params(m, log2_scale, data, scales, transpose);
   prm.slot_of_row = static_cast<std::int32_t const *>(slot_of_row);
   static_assert(kScaleTileRows == 2 * kQuantRows && kQuantRows == kQuantTRows, "two CTAs deep");
-  bool const masked = slot_of_row != nullptr;
+  bool const masked = slot_of_row != nullptr && m.scatter == 0;
   if (masked) prm.col_tiles = (prm.col_tiles + kMaskedSpan - 1) / kMaskedSpan;
-  auto const grid =
-      static_cast<unsigned>(2 * ceil_div(m.rows, kScaleTileRows) * prm.col_tiles);
+  std::int64_t const row_ctas = m.scatter != 0 ? ceil_div(m.x_rows, kScatterRows)
+                                               : 2 * ceil_div(m.rows, kScaleTileRows);
+  if (row_ctas * prm.col_tiles > 0x7fffffffll) {
+    return fail(MEGACU_UNSUPPORTED, 22, "dimension too large");
+  }
+  auto const grid = static_cast<unsigned>(row_ctas * prm.col_tiles);
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
   cudaError_t e = cudaSuccess;
   auto launch = [&](auto kernel, auto const *src) {
@@ -433,6 +440,10 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
       } else {
         launch(fp4_quantize_t_kernel<T, kNv, false>, src);
       }
+    } else if (m.scatter != 0) {
+      prm.stride * size % 32 == 0 && aligned_to(x, 32)
+          ? launch(fp4_quantize_scatter_kernel<T, kNv, true>, src)
+          : launch(fp4_quantize_scatter_kernel<T, kNv, false>, src);
     } else if (prm.stride * size % 32 == 0 && aligned_to(x, 32)) {
       masked ? launch(fp4_quantize_kernel<T, kNv, true, true>, src)
              : launch(fp4_quantize_kernel<T, kNv, true, false>, src);
@@ -451,7 +462,7 @@ extern "C" megacu_status megacu_cuda_fp4_dequantize(megacu_driver_view driver, v
   megacu_status const st = check_matrix(matrix, log2_scale);
   if (st.code != MEGACU_OK) return st;
   megacu_fp4_matrix const &m = *matrix;
-  if (m.transpose != 0 || m.topk != 0) {
+  if (m.transpose != 0 || m.topk != 0 || m.scatter != 0) {
     return fail(MEGACU_UNSUPPORTED, 22, "values come back row by row as quantised");
   }
   if (m.stride != 0 && m.stride < m.cols) {

@@ -1,7 +1,7 @@
 // A routed (mixture of experts) MLP block with 4-bit weights (no counterpart
 // in megacu): the routing and 4-bit entry points called in a row on one
 // workspace.
-//   sort -> quantise the tokens' rows by expert -> act = silu(gate) * up by
+//   sort -> quantise the tokens' rows, to their experts -> act = silu(gate) * up by
 //   expert -> quantise act -> down by expert -> weighted sum back
 #include <cuda_runtime.h>
 
@@ -134,6 +134,7 @@ extern "C" megacu_status megacu_cuda_moe_mlp_fp4(
   megacu_fp4_matrix x_matrix = matrix(p, l.capacity, p.hidden, p.x_scale);
   x_matrix.topk = p.topk;
   x_matrix.x_rows = p.tokens;
+  x_matrix.scatter = 1;
   megacu_fp4_matrix const act_matrix = matrix(p, l.capacity, p.inter, p.act_scale);
   megacu_fp4_gemm_problem const gate_up =
       product(p, l.capacity, p.inter, p.hidden, p.up_alpha / x_matrix.scale);
@@ -147,7 +148,7 @@ extern "C" megacu_status megacu_cuda_moe_mlp_fp4(
     st = megacu_cuda_moe_sort(d, expert_ids, part(l.counts), part(l.offsets), part(l.row_of_slot),
                               part(l.slot_of_row), part(l.sort), &route);
     if (st.code != MEGACU_OK) return st;
-    st = megacu_cuda_fp4_quantize(d, x, part(l.slot_of_row), part(l.x_data), part(l.x_scales),
+    st = megacu_cuda_fp4_quantize(d, x, part(l.row_of_slot), part(l.x_data), part(l.x_scales),
                                   &x_matrix);
     if (st.code != MEGACU_OK) return st;
     st = megacu_cuda_fp4_gemm_swiglu(d, part(l.x_data), part(l.x_scales), gate, gate_scales, up,

@@ -188,7 +188,7 @@ def test_quantize_gathered(align, fmt):
     tokens, topk, experts, cols = 50, 3, 6, 288
     p = mb.MoeProblem(tokens, topk, experts, align=align)
     ids = torch.randint(0, experts + 1, (tokens, topk), generator=gen)
-    _, _, _, slots = ref.sort(ids, experts, 0, align, mb.moe_rows(p))
+    _, _, row_of_slot, slots = ref.sort(ids, experts, 0, align, mb.moe_rows(p))
     x = _matrix(tokens, cols, torch.bfloat16, gen)
     m = mb.Fp4Matrix(mb.moe_rows(p), cols, format=fmt)
     used = slots >= 0
@@ -197,10 +197,12 @@ def test_quantize_gathered(align, fmt):
     r, b = torch.meshgrid(torch.arange(m.rows), torch.arange(-(-cols // ref.BLOCK[fmt] // 4) * 4),
                           indexing="ij")
     at = ref.scale_index(r, b, -(-cols // ref.BLOCK[fmt] // 4))
-    for gather in (True, False):
+    for way in ("gather", "mask", "scatter"):
         data, scales = _buffers(m)
-        mb.fp4_quantize((x if gather else rows).cuda(), data, scales, problem=m,
-                        slot_of_row=slots.cuda(), topk=topk if gather else 0, stream=_stream())
+        index = dict(row_of_slot=row_of_slot.cuda()) if way == "scatter" else \
+            dict(slot_of_row=slots.cuda())
+        mb.fp4_quantize((rows if way == "mask" else x).cuda(), data, scales, problem=m,
+                        topk=0 if way == "mask" else topk, stream=_stream(), **index)
         data, scales = data.cpu().view(m.rows, -1), scales.cpu()
         assert torch.equal(data[used] & 0x77, want_data[used] & 0x77)
         assert (data[~used] == 0xEE).all()
@@ -218,6 +220,34 @@ def test_gathered_entries_that_name_no_row_are_skipped():
         got.append(_buffers(m))
         mb.fp4_quantize(x.cuda(), *got[-1], problem=m, slot_of_row=slots.cuda(), topk=2,
                         stream=_stream())
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    for rows in ([[0, -1], [4, 2], [-1, -1], [5, 3], [1, -1], [-1, -1]],
+                 [[0, 6], [4, 2], [-7, 2 ** 31 - 1], [5, 3], [1, 600], [-1, -2 ** 31]]):
+        got.append(_buffers(m))
+        mb.fp4_quantize(x.cuda(), *got[-1], problem=m, topk=2, stream=_stream(),
+                        row_of_slot=torch.tensor(rows, dtype=torch.int32).cuda())
+    assert torch.equal(got[2][0], got[3][0]) and torch.equal(got[2][1], got[3][1])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("tokens,topk,cols,pad", [(1, 1, 32, 0), (33, 8, 96, 0), (70, 5, 544, 3),
+                                                  (300, 2, 4096, 16)])
+def test_scattered_rows_are_the_gathered_ones(tokens, topk, cols, pad, dtype, fmt):
+    gen = torch.Generator().manual_seed(cols)
+    p = mb.MoeProblem(tokens, topk, 9, first_expert=1, align=128)
+    ids = torch.randint(0, 11, (tokens, topk), generator=gen)
+    _, _, row_of_slot, slots = ref.sort(ids, 9, 1, 128, mb.moe_rows(p))
+    x = torch.zeros(tokens, cols + pad, dtype=DTYPES[dtype])
+    x[:, :cols] = _matrix(tokens, cols, DTYPES[dtype], gen)
+    x[tokens // 2, 7] = math.inf
+    x = x.cuda()[:, :cols]
+    m = mb.Fp4Matrix(mb.moe_rows(p), cols, format=fmt, dtype=dtype, scale=4.0,
+                     stride=cols + pad if pad else 0)
+    got = [_buffers(m) for _ in range(2)]
+    mb.fp4_quantize(x, *got[0], problem=m, slot_of_row=slots.cuda(), topk=topk, stream=_stream())
+    mb.fp4_quantize(x, *got[1], problem=m, row_of_slot=row_of_slot.cuda(), topk=topk,
+                    stream=_stream())
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
 
 

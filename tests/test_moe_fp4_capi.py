@@ -160,6 +160,12 @@ def test_quantize_refuses_storage_and_options():
     assert _status(q, FAKE, FAKE, FAKE, FAKE, ctypes.byref(t)) == (1, 1)
     t.x_rows = 5
     assert _status(q, FAKE, FAKE, FAKE, FAKE, ctypes.byref(t)) == (0, 0)
+    t.scatter = 1
+    assert _status(q, FAKE, FAKE, FAKE, FAKE, ctypes.byref(t)) == (0, 0)
+    assert _status(q, FAKE, None, FAKE, FAKE, ctypes.byref(t)) == (1, 2)
+    t.topk = 0
+    assert _status(q, FAKE, FAKE, FAKE, FAKE, ctypes.byref(t)) == (1, 1)
+    t.topk = 2
     assert _status(d, FAKE, FAKE, FAKE, ctypes.byref(t)) == (2, 22)
     # a transposed matrix's stride is between its stored rows
     t = _matrix(transpose=True, rows=10, cols=64, stride=12)
