@@ -142,8 +142,8 @@ std::int64_t clusters_at_once(int split, int sms) {
 // a call's start-up and end, a k-block of 256 at each width (what an SM can
 // load in a time that its MMAs do not exceed), a further tile on the same SM,
 // and the exchange of a split, which grows with the tile's accumulators.
-// 16 x 8192 x 3584: tile_n 64 takes 7.3 us, 128 7.2, 256 9.4, 128 split in two
-// 7.7, 256 split in four 8.7.
+// 16 x 8192 x 3584: tile_n 64 takes 6.4 us, 128 6.5, 256 8.7, 128 split in two
+// 8.0, 256 split in four 9.2.
 megacu_status make_plan(megacu_fp4_gemm_problem const &p, bool swiglu, int sms, fp4_plan &out) {
   std::int64_t const k_blocks = ceil_div(p.k, kFp4BlockK);
   double best = -1.0;
