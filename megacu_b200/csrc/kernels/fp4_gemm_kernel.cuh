@@ -54,8 +54,8 @@ inline constexpr int kFp4BlockM = 128;
 inline constexpr int kFp4BlockK = 256;  // elements per stage: one 128-byte swizzled row
 inline constexpr int kFp4SmallRows = 32;  // rows of the smaller A box
 // Experts whose places are kept in shared memory: each tile's place is looked up
-// before its loads, and four dependent global loads took 1.7 us, as long as
-// the stage ring lasts (3000 rows over 16 experts x 1001 x 1120: 15.0 us).
+// before its loads, and four dependent global loads took 1.7 us, as long as the
+// stage ring lasts.
 inline constexpr int kFp4TableExperts = 256;
 // Bound of the waits that only let copies and MMAs in flight end after an error.
 inline constexpr unsigned long long kFp4DrainNs = 10000000ull;
