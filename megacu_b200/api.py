@@ -717,12 +717,15 @@ def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, row_o
     """Quantises ``x`` into ``data`` and ``scales`` (async). With
     ``slot_of_row`` (of :func:`moe_sort`, int32 [rows]) rows whose entry is
     negative are left as they were; with ``topk`` too, row r is taken from
-    x[slot_of_row[r] // topk]. With ``row_of_slot`` ([x rows, topk]) instead,
-    each row of ``x`` is quantised once and written to the rows of its choices:
-    the same bytes, sooner when topk > 1. ``x_rows``: the rows of ``x``, needed
-    only when ``x`` is a raw address and topk > 0."""
+    x[slot_of_row[r] // topk]. With ``row_of_slot`` ([x rows, topk]) and its
+    ``topk`` instead, each row of ``x`` is quantised once and written to the
+    rows of its choices: the same bytes, sooner when topk > 1. ``x_rows``: the
+    rows of ``x``, needed only when ``x`` is a raw address and topk > 0."""
     if slot_of_row is not None and row_of_slot is not None:
         raise ValueError("slot_of_row or row_of_slot, not both")
+    if row_of_slot is not None and (topk < 1 or (getattr(row_of_slot, "ndim", 1) == 2
+                                                 and row_of_slot.shape[1] != topk)):
+        raise ValueError(f"row_of_slot holds topk entries per row of x, topk is {topk}")
     p, where = problem, None if stream is None else device
     nbytes, sbytes = fp4_sizes(p)
     if topk:

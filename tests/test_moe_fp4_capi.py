@@ -328,3 +328,25 @@ def test_reference_quantiser_against_every_element(fmt):
     assert (mag[tie] % 2 == 0).all() and tie.any()
     data, tiled = ref.pack(code, byte)
     assert torch.equal(ref.values(data, tiled, fmt), ref.ELEMENTS[code] * s)
+
+
+def test_scattered_quantisation_needs_its_choices():
+    """row_of_slot is a map of `topk` entries per row of x, never a mask of the
+    matrix's rows: without topk, or with another one than the map's, the call
+    is refused, whatever the map's length."""
+    m = mb.Fp4Matrix(4, 32)
+    data, scales = (torch.zeros(n, dtype=torch.uint8) for n in mb.fp4_sizes(m))
+    x = torch.zeros(4, 32, dtype=torch.bfloat16)
+    for at in (torch.tensor([2, 0, 3, 1], dtype=torch.int32), torch.zeros(1, dtype=torch.int32),
+               torch.zeros(4, 1, dtype=torch.int32), FAKE):
+        with pytest.raises(ValueError, match="topk"):
+            mb.fp4_quantize(x, data, scales, problem=m, row_of_slot=at)
+        with pytest.raises(ValueError, match="topk"):
+            mb.fp4_quantize(x, data, scales, problem=m, row_of_slot=at, topk=-1)
+    with pytest.raises(ValueError, match="topk"):
+        mb.fp4_quantize(x[:2], data, scales, problem=m, topk=1,
+                        row_of_slot=torch.zeros(2, 2, dtype=torch.int32))
+    mb.fp4_quantize(x, data, scales, problem=m, topk=1,
+                    row_of_slot=torch.zeros(4, 1, dtype=torch.int32))
+    mb.fp4_quantize(x, data, scales, problem=m, topk=1,
+                    row_of_slot=torch.zeros(4, dtype=torch.int32))
