@@ -30,7 +30,9 @@
 // sums one slice of the tile's columns over the cluster, in rank order,
 // through distributed shared memory (the drained stage ring).
 //
-// Every wait is bounded; one that gives up sets the error word in `events`.
+// Every wait is bounded; one that gives up sets the error word in `events`. A
+// CTA leaves only when its loads have landed and its MMAs have ended, whichever
+// wait gave up (stage_ring.h); on the normal path they have long since.
 #pragma once
 
 #include <cuda.h>
@@ -44,6 +46,7 @@
 #include "fp4_format.cuh"
 #include "layout.h"
 #include "sm100_ptx.cuh"
+#include "stage_ring.h"
 #include "vec.cuh"
 
 namespace megacu_b200 {
@@ -57,8 +60,9 @@ inline constexpr int kFp4SmallRows = 32;  // rows of the smaller A box
 // before its loads, and four dependent global loads took 1.7 us, as long as the
 // stage ring lasts.
 inline constexpr int kFp4TableExperts = 256;
-// Bound of the waits that only let copies and MMAs in flight end after an error.
-inline constexpr unsigned long long kFp4DrainNs = 10000000ull;
+// Bound of the waits that only let copies and MMAs in flight end: they take
+// microseconds, and nothing that an earlier error stopped is among them.
+inline constexpr unsigned long long kFp4DrainNs = 1000000000ull;
 
 // b2, b2_scales: SwiGLU's up; a_small: A in boxes of kFp4SmallRows rows.
 struct fp4_maps {
@@ -222,6 +226,12 @@ __device__ __forceinline__ std::uint32_t ld_shared_u16(std::uint32_t at) {
   return v;
 }
 
+// Counts `bytes` of a barrier's announced ones as arrived.
+__device__ __forceinline__ void mbar_complete_tx(std::uint64_t *bar, std::uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;"
+               :: "r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+
 // Descriptor of a scale tile: no swizzle, 8-row groups 128 bytes apart.
 __device__ __forceinline__ std::uint64_t scale_desc(std::uint32_t start) {
   return static_cast<std::uint64_t>((start >> 4) & 0x3fffu) |
@@ -296,6 +306,21 @@ __device__ __forceinline__ fp4_rows locate_rows(fp4_gemm_params const &p,
   }
   return r;
 }
+
+// The waits of stage_ring.h on the `full` barriers.
+struct fp4_drain {
+  std::uint64_t *full;
+  std::uint32_t follower_bytes;  // of one stage
+  __device__ __forceinline__ void wait(std::uint32_t stage, std::uint32_t parity) const {
+    ptx::mbar_wait(&full[stage], parity, nullptr, kFp4DrainNs);
+  }
+  __device__ __forceinline__ void announce(std::uint32_t stage) const {
+    ptx::mbar_arrive_expect_tx(&full[stage], follower_bytes);
+  }
+  __device__ __forceinline__ void complete(std::uint32_t stage) const {
+    ptx::mbar_complete_tx(&full[stage], follower_bytes);
+  }
+};
 
 __device__ __forceinline__ float locate_alpha(fp4_gemm_params const &p, std::int32_t expert) {
   return p.alphas != nullptr && p.experts > 0 ? p.alpha * p.alphas[expert] : p.alpha;
@@ -463,6 +488,10 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   std::uint64_t *const acc_full = empty + kStages;
   std::uint64_t *const acc_free = acc_full + 1;
   auto *const tmem_slot = reinterpret_cast<std::uint32_t *>(acc_free + 1);
+  // A pair's, written at the end: the tiles that the leader's MMA warp committed
+  // and whether it gave up (2 * tiles + 1, in both CTAs), and the loads of each
+  // producer (in the leader).
+  std::uint32_t *const mma_end = tmem_slot + 1, *const loads = tmem_slot + 2;
   auto &table = *reinterpret_cast<fp4_expert_table *>(staging + cfg::staging_bytes + cfg::barrier_bytes);
   std::uint32_t *const abort_word = &reinterpret_cast<control_block *>(p.events)->error_code;
 
@@ -642,19 +671,17 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       }
       skip = 0;
     }
-    if (!ok && leader) {
-      // Copies still in flight land before the CTA may exit (a pair's are all
-      // counted by the leader).
-      std::uint32_t const pending = issued < kStages ? issued : kStages;
-      for (std::uint32_t i = 0; i < pending; ++i) {
-        if (stage == 0) phase ^= 1u;
-        stage = stage == 0 ? kStages - 1 : stage - 1;
-        ptx::mbar_wait(&full[stage], phase, nullptr, kFp4DrainNs);
+    if constexpr (kPair) {
+      if (lane == 0) {
+        ptx::st_shared_remote(ptx::map_to_rank(&loads[rank], 0),
+                              static_cast<std::int32_t>(issued));
       }
+    } else {
+      drain_ring(issued, kStages, detail::fp4_drain{full, 0});
     }
   } else if (warp == 1 && leader) {
     // ---------------- scale copies and MMA issue ----------------
-    std::uint32_t stage = 0, phase = 0, tile_index = 0;
+    std::uint32_t stage = 0, phase = 0, tile_index = 0, committed = 0;
     std::uint32_t const sf = tmem + cfg::sf_column;
     // Descriptors of stage 0; a stage is a multiple of 16 bytes further.
     std::uint64_t const a_desc0 = ptx::smem_desc_sw128(ptx::smem_addr(smem), 16, 1024);
@@ -665,6 +692,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       if (tile_index > 0 &&
           !ptx::mbar_wait_cluster(acc_free, (tile_index - 1) & 1u, abort_word, p.timeout_ns)) {
         if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 52);
+        ok = false;
         break;
       }
       ptx::tc_fence_after_sync();
@@ -714,9 +742,19 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
         }
       }
       if (ptx::elect_one()) ptx::commit_fp4<kPair>(acc_full);
+      ++committed;
       __syncwarp();
-      // MMAs in flight end before the CTA may free its TMEM.
-      if (!ok) ptx::mbar_wait_cluster(acc_full, tile_index & 1u, nullptr, kFp4DrainNs);
+    }
+    // MMAs in flight end before the CTA may free its TMEM. (A tile starts when
+    // the commit of the one before has arrived: one phase is open at most.)
+    if (committed > 0) {
+      ptx::mbar_wait_cluster(acc_full, (committed - 1) & 1u, nullptr, kFp4DrainNs);
+    }
+    if constexpr (kPair) {
+      if (lane < 2) {
+        ptx::st_shared_remote(ptx::map_to_rank(mma_end, lane),
+                              static_cast<std::int32_t>(2 * committed + (ok ? 0 : 1)));
+      }
     }
     __syncwarp();
   } else if (warp >= 2) {
@@ -870,7 +908,24 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
 
   ptx::tc_fence_before_sync();
   __syncthreads();
-  if constexpr (kPair) ptx::cluster_sync();  // no more accesses to the other CTA
+  if constexpr (kPair) {
+    ptx::cluster_sync();  // no more accesses to the other CTA
+    // An MMA warp that did not give up has seen every load of both CTAs land.
+    std::uint32_t const end = *reinterpret_cast<std::uint32_t volatile *>(mma_end);
+    if (warp == 1 && end >= 2) {  // its last commit has arrived here too
+      ptx::mbar_wait_cluster(acc_full, (end / 2 - 1) & 1u, nullptr, kFp4DrainNs);
+    }
+    __syncwarp();
+    if (end & 1u) {  // in both CTAs or in neither
+      if (leader && threadIdx.x == 0) {
+        drain_pair_ring(loads[0], loads[1], kStages,
+                        detail::fp4_drain{full, kFp4BlockM * 128 + cfg::b_bytes + cfg::sfa_bytes +
+                                                    cfg::sfb_bytes});
+      }
+      __syncwarp();
+      ptx::cluster_sync();
+    }
+  }
   if (warp == 1) {
     ptx::tc_fence_after_sync();
     if constexpr (kPair) {
