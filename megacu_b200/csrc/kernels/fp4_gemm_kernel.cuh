@@ -307,6 +307,25 @@ __device__ __forceinline__ fp4_rows locate_rows(fp4_gemm_params const &p,
   return r;
 }
 
+// ptx::mbar_wait_cluster for a whole converged warp, with one answer: what
+// follows are warp-wide instructions, and lanes that decided for themselves
+// could give up apart.
+__device__ __forceinline__ bool warp_wait(std::uint64_t *bar, std::uint32_t parity,
+                                          std::uint32_t const *abort_word,
+                                          unsigned long long timeout_ns) {
+  std::uint32_t const a = ptx::smem_addr(bar);
+  if (__all_sync(0xffffffffu, ptx::mbar_test_cluster(a, parity))) return true;
+  std::uint64_t const start = ptx::now_ns();
+  for (std::uint32_t spin = 1;; ++spin) {
+    if (__all_sync(0xffffffffu, ptx::mbar_test_cluster(a, parity))) return true;
+    if ((spin & 127u) == 0) {
+      bool const over =
+          ptx::ld_relaxed_gpu(abort_word) != 0 || ptx::now_ns() - start > timeout_ns;
+      if (__any_sync(0xffffffffu, over)) return false;
+    }
+  }
+}
+
 // The waits of stage_ring.h on the `full` barriers.
 struct fp4_drain {
   std::uint64_t *full;
@@ -655,7 +674,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     for (std::int32_t t = unit0; ok && t < tiles; t += units) {
       load_place const l = place(t);
       for (std::int32_t kb = kb0 + skip; kb < kb1; ++kb) {
-        if (!ptx::mbar_wait_cluster(&empty[stage], phase ^ 1u, abort_word, p.timeout_ns)) {
+        if (!detail::warp_wait(&empty[stage], phase ^ 1u, abort_word, p.timeout_ns)) {
           if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 51);
           ok = false;
           break;
@@ -690,7 +709,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     bool ok = true;
     for (std::int32_t t = unit0; ok && t < tiles; t += units, ++tile_index) {
       if (tile_index > 0 &&
-          !ptx::mbar_wait_cluster(acc_free, (tile_index - 1) & 1u, abort_word, p.timeout_ns)) {
+          !detail::warp_wait(acc_free, (tile_index - 1) & 1u, abort_word, p.timeout_ns)) {
         if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 52);
         ok = false;
         break;
@@ -700,7 +719,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       // A tile of 64 columns uses half of a scale tile's four TMEM columns.
       std::uint32_t const b_half = BN == 64 ? (locate(t).col & 1) * 2u : 0u;
       for (std::int32_t kb = kb0; kb < kb1; ++kb) {
-        if (!ptx::mbar_wait_cluster(&full[stage], phase, abort_word, p.timeout_ns)) {
+        if (!detail::warp_wait(&full[stage], phase, abort_word, p.timeout_ns)) {
           if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 53);
           ok = false;
           break;
@@ -772,7 +791,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       float const alpha = detail::locate_alpha(p, rows.expert);
       detail::fp4_rows_out const out =
           detail::rows_out(p, row + quarter * 32, rows.valid - quarter * 32);
-      if (!ptx::mbar_wait_cluster(acc_full, tile_index & 1u, abort_word, p.timeout_ns)) {
+      if (!detail::warp_wait(acc_full, tile_index & 1u, abort_word, p.timeout_ns)) {
         if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 54);
         break;
       }

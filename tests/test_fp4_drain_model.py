@@ -30,6 +30,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import re
 import shutil
 import subprocess
 import tempfile
@@ -250,3 +251,12 @@ def test_drain_waits_for_the_last_load_of_every_stage(stages):
             want[i % stages] = i // stages & 1
         ops = drain_ops(False, issued, 0, stages)
         assert {s: parity for _, s, parity in ops} == want and len(ops) == len(want)
+
+
+def test_whole_warps_give_up():
+    """A wait that may give up decides once for all lanes of its warp: lanes
+    that disagree would meet different warp-wide instructions."""
+    path = os.path.join(ROOT, "megacu_b200", "csrc", "kernels", "fp4_gemm_kernel.cuh")
+    body = open(path).read().split("fp4_gemm_kernel(__grid_constant__", 1)[1]
+    calls = re.findall(r"(\w+)\([^;{]*abort_word, p\.timeout_ns\)", body)
+    assert len(calls) == 4 and set(calls) == {"warp_wait"}

@@ -731,3 +731,53 @@ def test_calls_in_a_row_wait_for_one_another():
     assert torch.isfinite(want.float()).all() and want.float().abs().max() > 0
     for _ in range(5):
         assert torch.equal(run(False), want)
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("m,n,k,experts,tile_n,split", [
+    (16, 2048, 8192, 0, 64, 1), (100, 1000, 4096, 0, 256, 8), (100, 2000, 8192, 0, 256, 4),
+    (1000, 4000, 8192, 0, 256, 1), (300, 9000, 2048, 0, 128, 1), (1024, 512, 4096, 8, 256, 1),
+    (1024, 512, 4096, 8, 256, 2)])
+def test_given_up_waits_end_the_call_and_spare_the_next(m, n, k, experts, tile_n, split, swiglu):
+    """A call on events that still hold an error, and one whose waits may last
+    no time at all, return (which of their waits give up is a matter of
+    timing), report it, and the next calls compute what they always do."""
+    if swiglu and tile_n != 256:
+        tile_n, split = 256, 1
+    gen = torch.Generator().manual_seed(n)
+    a = _gpu(ref.random_operand(gen, m, k, 0))
+    parts = [_gpu(ref.random_operand(gen, max(experts, 1) * n, k, 0)) for _ in range(1 + swiglu)]
+    kw = {}
+    if experts:
+        rows = torch.full((experts,), m // experts, dtype=torch.int32)
+        kw = dict(offsets=torch.arange(experts + 1, dtype=torch.int32).mul(m // experts).cuda(),
+                  counts=rows.cuda())
+    operands = [t for part in parts for t in part]
+    fn = mb.fp4_gemm_swiglu if swiglu else mb.fp4_gemm
+    events = torch.zeros(mb.fp4_events_bytes(), dtype=torch.uint8, device="cuda")
+
+    def run(timeout_ns=0):
+        p = mb.Fp4Gemm(m, n, k, alpha=2.0 ** -8, experts=experts, tile_n=tile_n, split=split,
+                       timeout_ns=timeout_ns)
+        out = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+        fn(*a, *operands, out, events=events, problem=p, stream=_stream(), **kw)
+        return out
+
+    want = run()
+    mb.events_status(events, _stream())
+    for _ in range(3):
+        events.view(torch.int32)[4] = 41  # the error word
+        run()
+        run(1)
+        with pytest.raises(mb.MegacuError):
+            mb.events_status(events, _stream())
+        assert torch.equal(run(), want)
+        mb.events_status(events, _stream())
+        out = run(1)
+        try:
+            mb.events_status(events, _stream())
+            assert torch.equal(out, want)
+        except mb.MegacuError:
+            pass
+        assert torch.equal(run(), want)
+        mb.events_status(events, _stream())
