@@ -63,6 +63,8 @@ inline constexpr int kFp4TableExperts = 256;
 // Bound of the waits that only let copies and MMAs in flight end: they take
 // microseconds, and nothing that an earlier error stopped is among them.
 inline constexpr unsigned long long kFp4DrainNs = 1000000000ull;
+// Bound of a follower's wait for a commit that may have been issued or not.
+inline constexpr unsigned long long kFp4CommitNs = 10000000ull;
 
 // b2, b2_scales: SwiGLU's up; a_small: A in boxes of kFp4SmallRows rows.
 struct fp4_maps {
@@ -207,6 +209,17 @@ __device__ __forceinline__ void st_shared_v4(std::uint32_t at, std::uint32_t a, 
                :: "r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// map_to_rank of a shared::cta address.
+__device__ __forceinline__ std::uint32_t map_to_rank(std::uint32_t local, std::uint32_t rank) {
+  std::uint32_t out;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(local), "r"(rank));
+  return out;
+}
+
+__device__ __forceinline__ void st_shared_u32(std::uint32_t at, std::uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" :: "r"(at), "r"(v) : "memory");
+}
+
 __device__ __forceinline__ uint4 ld_shared_v4(std::uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -224,6 +237,12 @@ __device__ __forceinline__ std::uint32_t ld_shared_u16(std::uint32_t at) {
   std::uint16_t v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
   return v;
+}
+
+// Warps 0 and 1 wait for one another.
+__device__ __forceinline__ void two_warps_sync() {
+  __syncwarp();
+  asm volatile("bar.sync 1, 64;" ::: "memory");
 }
 
 // Counts `bytes` of a barrier's announced ones as arrived.
@@ -340,6 +359,51 @@ struct fp4_drain {
     ptx::mbar_complete_tx(&full[stage], follower_bytes);
   }
 };
+
+// A follower's epilogue warp gave up: the commit that it waited for may yet
+// arrive here (the leader's MMA warp waits for its own arrival of the last). A
+// call, since inlined it slows the epilogue.
+__device__ __noinline__ void wait_commit(std::uint64_t *acc_full, std::uint32_t parity) {
+  ptx::mbar_wait_cluster(acc_full, parity, nullptr, kFp4CommitNs);
+}
+
+// One thread of a pair's leader waits for both CTAs' loads after the MMA warp
+// gave up.
+template <class cfg>
+__device__ __forceinline__ void drain_pair(std::uint32_t at, std::uint32_t loads,
+                                           unsigned long long timeout_ns) {
+  auto const volatile *const follower_loads =
+      static_cast<std::uint32_t const volatile *>(__cvta_shared_to_generic(at + 4));
+  auto *const full = static_cast<std::uint64_t *>(
+      __cvta_shared_to_generic(at - 4 - (2 * cfg::stages + 2) * 8));
+  // The follower's producer ends as soon as its wait does.
+  std::uint64_t const start = ptx::now_ns();
+  std::uint32_t theirs = 0;
+  while ((theirs = *follower_loads) == 0) {
+    std::uint64_t const waited = ptx::now_ns() - start;
+    if (waited > timeout_ns && waited - timeout_ns > kFp4DrainNs) return;
+  }
+  drain_pair_ring(loads, theirs - 1, cfg::stages,
+                  fp4_drain{full, kFp4BlockM * 128 + cfg::b_bytes + cfg::sfa_bytes +
+                                      cfg::sfb_bytes});
+}
+
+// The end of a pair's producers (whole warps). Both CTAs' loads count on the
+// leader's barriers, and an MMA warp that did not give up has seen them all
+// land; else the leader's producer waits for them, knowing how many there are.
+// `at`: the pair's two words.
+template <class cfg>
+__device__ __forceinline__ void end_pair_producer(std::uint32_t at, std::uint32_t loads,
+                                                  bool leader, unsigned long long timeout_ns) {
+  if (!leader) {
+    if (ptx::lane_id() == 0) {
+      ptx::st_shared_remote(ptx::map_to_rank(at + 4, 0), static_cast<std::int32_t>(loads + 1));
+    }
+    return;
+  }
+  ptx::two_warps_sync();  // the MMA warp has ended
+  if (ptx::lane_id() == 0 && ptx::ld_shared_u32(at) != 0) drain_pair<cfg>(at, loads, timeout_ns);
+}
 
 __device__ __forceinline__ float locate_alpha(fp4_gemm_params const &p, std::int32_t expert) {
   return p.alphas != nullptr && p.experts > 0 ? p.alpha * p.alphas[expert] : p.alpha;
@@ -507,10 +571,17 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   std::uint64_t *const acc_full = empty + kStages;
   std::uint64_t *const acc_free = acc_full + 1;
   auto *const tmem_slot = reinterpret_cast<std::uint32_t *>(acc_free + 1);
-  // A pair's, written at the end: the tiles that the leader's MMA warp committed
-  // and whether it gave up (2 * tiles + 1, in both CTAs), and the loads of each
-  // producer (in the leader).
-  std::uint32_t *const mma_end = tmem_slot + 1, *const loads = tmem_slot + 2;
+  // In a pair's leader: whether its MMA warp gave up, and 1 + the follower's
+  // loads once its producer has ended.
+  // Two words of a pair's leader: whether its MMA warp gave up, and 1 + the
+  // follower's loads once its producer has ended. Their address is computed
+  // anew at each use, so that the epilogue holds no register for it.
+  auto pair_words = [] {
+    std::uint32_t raw;
+    asm volatile("mov.u32 %0, %1;" : "=r"(raw) : "r"(ptx::smem_addr(raw_smem)));
+    return ((raw + 1023u) & ~1023u) + cfg::ring_bytes + cfg::staging_bytes +
+           (2 * kStages + 2) * 8 + 4;
+  };
   auto &table = *reinterpret_cast<fp4_expert_table *>(staging + cfg::staging_bytes + cfg::barrier_bytes);
   std::uint32_t *const abort_word = &reinterpret_cast<control_block *>(p.events)->error_code;
 
@@ -539,6 +610,10 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     } else if (lane == 16) {
       ptx::mbar_init(acc_full, 1);
       ptx::mbar_init(acc_free, kFp4EpilogueWarps * (kPair ? 2 : 1));
+      if constexpr (kPair) {
+        ptx::st_shared_u32(pair_words(), 0);
+        ptx::st_shared_u32(pair_words() + 4, 0);
+      }
     }
     ptx::fence_barrier_init();
     ptx::fence_proxy_async_shared();
@@ -691,10 +766,8 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       skip = 0;
     }
     if constexpr (kPair) {
-      if (lane == 0) {
-        ptx::st_shared_remote(ptx::map_to_rank(&loads[rank], 0),
-                              static_cast<std::int32_t>(issued));
-      }
+      detail::end_pair_producer<cfg>(pair_words(), issued, leader, p.timeout_ns);
+      __syncwarp();
     } else {
       drain_ring(issued, kStages, detail::fp4_drain{full, 0});
     }
@@ -770,10 +843,8 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       ptx::mbar_wait_cluster(acc_full, (committed - 1) & 1u, nullptr, kFp4DrainNs);
     }
     if constexpr (kPair) {
-      if (lane < 2) {
-        ptx::st_shared_remote(ptx::map_to_rank(mma_end, lane),
-                              static_cast<std::int32_t>(2 * committed + (ok ? 0 : 1)));
-      }
+      if (!ok && lane == 0) ptx::st_shared_u32(pair_words(), 1);
+      ptx::two_warps_sync();  // with the producer's end
     }
     __syncwarp();
   } else if (warp >= 2) {
@@ -793,6 +864,10 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
           detail::rows_out(p, row + quarter * 32, rows.valid - quarter * 32);
       if (!detail::warp_wait(acc_full, tile_index & 1u, abort_word, p.timeout_ns)) {
         if (lane == 0) detail::fp4_error(p.events, static_cast<std::uint32_t>(t), 54);
+        if constexpr (kPair) {
+          if (!leader) detail::wait_commit(acc_full, tile_index & 1u);
+        }
+        // The leader's MMA warp waits for its own arrival of a last commit.
         break;
       }
       __syncwarp();
@@ -927,24 +1002,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
 
   ptx::tc_fence_before_sync();
   __syncthreads();
-  if constexpr (kPair) {
-    ptx::cluster_sync();  // no more accesses to the other CTA
-    // An MMA warp that did not give up has seen every load of both CTAs land.
-    std::uint32_t const end = *reinterpret_cast<std::uint32_t volatile *>(mma_end);
-    if (warp == 1 && end >= 2) {  // its last commit has arrived here too
-      ptx::mbar_wait_cluster(acc_full, (end / 2 - 1) & 1u, nullptr, kFp4DrainNs);
-    }
-    __syncwarp();
-    if (end & 1u) {  // in both CTAs or in neither
-      if (leader && threadIdx.x == 0) {
-        drain_pair_ring(loads[0], loads[1], kStages,
-                        detail::fp4_drain{full, kFp4BlockM * 128 + cfg::b_bytes + cfg::sfa_bytes +
-                                                    cfg::sfb_bytes});
-      }
-      __syncwarp();
-      ptx::cluster_sync();
-    }
-  }
+  if constexpr (kPair) ptx::cluster_sync();  // no more accesses to the other CTA
   if (warp == 1) {
     ptx::tc_fence_after_sync();
     if constexpr (kPair) {

@@ -16,9 +16,10 @@ The model follows megacu_b200/csrc/kernels/fp4_gemm_kernel.cuh:
   * every one of these waits may give up whenever it does not pass, and its
     thread then goes to its end;
   * at their ends the MMA warp waits for its last commit; a single CTA's
-    producer waits for the last load of every stage; a pair meets, the follower
-    waits for the last commit too, and if the MMA warp gave up the leader runs
-    the drain over both producers' counts before the CTAs leave.
+    producer waits for the last load of every stage; the producer of a pair's
+    leader waits for the MMA warp's end and, if that gave up, for the
+    follower's producer's, and runs the drain over both counts;
+  * the CTAs of a pair leave together.
 The drains' operations come from the kernel's own header (stage_ring.h).
 
 Planted: no wait at the producer's end unless its own wait gave up, none for
@@ -183,13 +184,13 @@ def explore(stages, tiles, kbs, ctas, mistake=None, limit=3_000_000):
             drained = pos == len(drain_ops(False, issued, 0, stages)) or (
                 mistake == "drain_if_gave_up" and status == ENDED)
             leaving = leaving and drained
-        elif leaving:
-            leaving = mma[1] == 0 or passes(acc_full[1], last)
-            if leaving and mma[2] == GAVE_UP:
+        elif mma[2] == GAVE_UP:
+            # Once both producers and the MMA warp have ended, whatever the epilogues do.
+            leaving = False
+            if committed_done and all(q[1] != RUN for q in prod):
                 follower = prod[0][0] if mistake == "leaders_loads_only" else prod[1][0]
                 ops = drain_ops(True, prod[0][0], follower, stages)
-                leaving = at == len(ops)
-                if not leaving:
+                if at < len(ops):
                     kind, s, parity = ops[at]
                     phase, missing, units = full[s]
                     if kind == ANNOUNCE:
@@ -200,6 +201,8 @@ def explore(stages, tiles, kbs, ctas, mistake=None, limit=3_000_000):
                         to(at=at + 1, full=_set(full, s, _settle((phase, missing, units - 1))))
                     elif passes(phase, parity):
                         to(at=at + 1)
+                else:
+                    leaving = at_end
         if leaving:
             if loads:
                 raise Violation(f"left with loads in flight: {sorted(loads)}")
