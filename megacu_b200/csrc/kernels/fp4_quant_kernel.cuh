@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kQuantThreads, 2) fp4_quantize_t_kernel(fp4_ma
   grid_start_next();
   grid_wait();
   // [tile][row % 32][row / 32] of four scale bytes
-  __shared__ std::uint32_t bytes[kTiles][32][2];
+  __shared__ alignas(8) std::uint32_t bytes[kTiles][32][2];
   __shared__ uint4 turned[kQuantTRows][8];
   std::uint32_t const rows_cta = blockIdx.x / p.col_tiles;
   std::int64_t const row_tile = rows_cta / 2;
