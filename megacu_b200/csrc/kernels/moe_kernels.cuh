@@ -60,9 +60,9 @@ __device__ __forceinline__ void clear_rows(moe_sort_params const &p) {
 template <class Id>
 __global__ void __launch_bounds__(kMoeSortThreads) moe_count_kernel(moe_sort_params p) {
   extern __shared__ std::int32_t moe_smem[];
+  grid_start_next();
   for (int e = threadIdx.x; e < p.experts; e += blockDim.x) moe_smem[e] = 0;
   grid_wait();
-  grid_start_next();  // past the wait: the second launch reads the ids before its own
   __syncthreads();
   std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
   std::int64_t const end = min(begin + p.chunk, p.slots);
@@ -116,26 +116,26 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_par
   int const tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   bool const chunked = gridDim.x > 1;
 
+  grid_start_next();
   std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
   std::int32_t const here = static_cast<std::int32_t>(min(p.chunk + begin, p.slots) - begin);
   std::int32_t const part = (p.chunk + threads - 1) / threads * 32;
   std::int32_t const w0 = min(warp * part, here), w1 = min(w0 + part, here);
   std::int32_t *const mine = cursor + warp * experts;
   for (int e = lane; e < experts; e += 32) mine[e] = 0;
-  if (!chunked) grid_wait();
   if (chunked) {
     for (int e = tid; e < 2 * experts; e += threads) total[e] = 0;
-  } else {
-    clear_rows(p);  // the first launch did it for several chunks
   }
+  // Also for the ids, which the first launch has read: that it has started
+  // this one does not make them visible here, its end does.
+  grid_wait();
+  if (!chunked) clear_rows(p);  // the first launch did it for several chunks
   __syncwarp();
   for (std::int32_t s = w0 + lane; s < w1; s += 32) {
     std::int32_t const e = local_expert<Id>(p, begin + s);
     local[s] = static_cast<std::int16_t>(e);
     if (e >= 0) atomicAdd(&mine[e], 1);
   }
-  if (chunked) grid_wait();  // every chunk's histogram is complete
-  grid_start_next();
   __syncthreads();
 
   // total[e] = slots of e anywhere, start[e] = slots of e in earlier chunks.

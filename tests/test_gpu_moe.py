@@ -260,3 +260,42 @@ def test_entries_that_name_no_row_are_skipped():
         got.append((rows, y, drows, dw))
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+def test_long_sorts_in_a_row_wait_for_their_ids():
+    """Sorts of two launches whose ids the kernel before them has just written,
+    with nothing between them, give what they give with a synchronisation
+    before each: no launch reads the ids before its own wait."""
+    tokens, topk, experts, steps = 20000, 4, 64, 16
+    p = mb.MoeProblem(tokens, topk, experts)
+    gen = torch.Generator().manual_seed(4)
+    order = torch.randperm(tokens, generator=gen).to(torch.int32).view(-1, 1).cuda()
+    move = mb.MoeProblem(tokens, 1, 1, hidden=topk, dtype=mb.DTYPE_F32)
+    first = torch.randint(0, experts, (tokens, topk), generator=gen, dtype=torch.int32).cuda()
+
+    def run(sync):
+        ids = [first.clone(), torch.empty_like(first)]
+        got = []
+        for i in range(steps):
+            # permutes the ids' rows: their 32 bits as a row's elements
+            mb.moe_dispatch(ids[0].view(torch.float32), ids[1].view(torch.float32),
+                            row_of_slot=order, problem=move, stream=torch.cuda.current_stream())
+            if sync:
+                torch.cuda.synchronize()
+            got.append(outs[i])
+            mb.moe_sort(ids[1], counts=outs[i][0], offsets=outs[i][1], row_of_slot=outs[i][2],
+                        slot_of_row=outs[i][3], workspace=ws, problem=p,
+                        stream=torch.cuda.current_stream())
+            ids.reverse()
+        return [t.clone() for out in got for t in out]
+
+    ws = _new(mb.moe_workspace_bytes(p), dtype=torch.uint8)
+    assert ws.numel() > 0
+    outs = [(_new(experts), _new(experts + 1), _new(tokens, topk), _new(mb.moe_rows(p)))
+            for _ in range(steps)]
+    want = run(True)
+    ids = first.cpu()[torch.argsort(order.view(-1).long().cpu())]
+    for g, w in zip(want[:4], ref.sort(ids, experts, 0, 1, mb.moe_rows(p))):
+        assert torch.equal(g.cpu(), w)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(run(False), want))
