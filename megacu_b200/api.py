@@ -493,7 +493,8 @@ def mlp_chain(x, w_gate, w_up, w_down, out, *, act, workspace, x_work, events_sw
 class _CProblem:
     """Base of the problem dataclasses passed by pointer: the C struct, the
     pointer to it and what follows from it are built once and reused until a
-    field changes."""
+    field changes. Struct and pointer are one entry, so that threads that meet
+    on a new problem see both or neither."""
 
     def __setattr__(self, name, value):
         object.__setattr__(self, name, value)
@@ -501,17 +502,18 @@ class _CProblem:
         self.__dict__.pop("_sizes", None)
         self.__dict__.pop("_need", None)
 
+    def _built(self):
+        built = self.__dict__.get("_c")
+        if built is None:
+            c = self._build()
+            built = self.__dict__["_c"] = (c, ctypes.byref(c))
+        return built
+
     def to_c(self):
-        c = self.__dict__.get("_c")
-        if c is None:
-            c = self.__dict__["_c"] = self._build()
-            self.__dict__["_ref"] = ctypes.byref(c)
-        return c
+        return self._built()[0]
 
     def _pointer(self):
-        if "_c" not in self.__dict__:
-            self.to_c()
-        return self.__dict__["_ref"]
+        return self._built()[1]
 
 
 class _Types(dict):
@@ -584,10 +586,10 @@ class MoeProblem(_CProblem):
 
     def _wide_ids(self):
         """The pointer for 64-bit ids."""
-        self.to_c()
+        c = self.to_c()
         wide = self.__dict__.get("_wide")
-        if wide is None or wide[0] is not self._c:
-            wide = self.__dict__["_wide"] = (self._c, ctypes.byref(self._build(8)))
+        if wide is None or wide[0] is not c:
+            wide = self.__dict__["_wide"] = (c, ctypes.byref(self._build(8)))
         return wide[1]
 
 

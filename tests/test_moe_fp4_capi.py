@@ -350,3 +350,41 @@ def test_scattered_quantisation_needs_its_choices():
                     row_of_slot=torch.zeros(4, 1, dtype=torch.int32))
     mb.fp4_quantize(x, data, scales, problem=m, topk=1,
                     row_of_slot=torch.zeros(4, dtype=torch.int32))
+
+
+def test_problems_are_used_by_several_threads_at_once(monkeypatch):
+    """Threads that meet on a new problem all get its C struct, whichever of
+    them builds it, and a changed field's struct after the change."""
+    import threading
+    import time
+
+    byref = ctypes.byref
+
+    def slow_byref(c):  # holds the window open between a struct and its pointer
+        time.sleep(0.002)
+        return byref(c)
+
+    monkeypatch.setattr(mb.api.ctypes, "byref", slow_byref)
+    for i in range(10):
+        p = mb.MoeProblem(i, 2, 4)
+        gate = threading.Barrier(4)
+        seen, errors = [], []
+
+        def use(late):
+            try:
+                gate.wait()
+                time.sleep(late * 0.001)
+                seen.append(p._pointer()._obj.tokens)
+                seen.append(p._wide_ids()._obj.tokens)
+                mb.moe_rows(p)
+            except Exception as e:  # a thread's error must reach the test
+                errors.append(repr(e))
+
+        threads = [threading.Thread(target=use, args=(n,)) for n in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert errors == [] and set(seen) == {i}
+        p.tokens = i + 1
+        assert p._pointer()._obj.tokens == p._wide_ids()._obj.tokens == i + 1
