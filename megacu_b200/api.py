@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import weakref
-from dataclasses import dataclass
+from dataclasses import dataclass, fields
 from typing import Callable, Optional, Sequence
 
 from . import _capi
@@ -501,6 +501,11 @@ class _CProblem:
         self.__dict__.pop("_c", None)
         self.__dict__.pop("_sizes", None)
         self.__dict__.pop("_need", None)
+
+    def __getstate__(self):
+        """Copies and pickles hold the fields alone: structs and pointers to them
+        belong to one object."""
+        return {f.name: getattr(self, f.name) for f in fields(self)}
 
     def _built(self):
         built = self.__dict__.get("_c")

@@ -388,3 +388,24 @@ def test_problems_are_used_by_several_threads_at_once(monkeypatch):
         assert errors == [] and set(seen) == {i}
         p.tokens = i + 1
         assert p._pointer()._obj.tokens == p._wide_ids()._obj.tokens == i + 1
+
+
+def test_used_problems_can_be_copied_and_pickled():
+    """A problem's struct and pointers are its own: a copy of one that calls
+    have used has the fields, builds its own and follows its own changes."""
+    import copy
+    import dataclasses
+    import pickle
+
+    problems = (mb.MoeProblem(5, 2, 4, hidden=64), mb.Fp4Matrix(10, 64), mb.Fp4Gemm(256, 96, 64),
+                mb.MoeMlp(5, 64, 96, 2, 4))
+    for p in problems:
+        p._pointer()
+        if hasattr(p, "_wide_ids"):
+            p._wide_ids()
+        for q in (copy.copy(p), copy.deepcopy(p), pickle.loads(pickle.dumps(p)),
+                  dataclasses.replace(p)):
+            assert q == p and q.to_c() is not p.to_c()
+            first = dataclasses.fields(q)[0].name
+            setattr(q, first, 7)
+            assert getattr(q.to_c(), first) == 7 and getattr(p.to_c(), first) != 7
