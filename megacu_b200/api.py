@@ -582,11 +582,13 @@ class MoeProblem(_CProblem):
     dtype: int = _capi.DTYPE_BF16
     token_stride: int = 0
     row_stride: int = 0
+    id_bytes: int = 0    # of ids given as an address: 4 (or 0) or 8; a tensor has its type
 
     def _build(self, id_bytes: int = 0):
         return _capi.MoeProblem(tokens=self.tokens, hidden=self.hidden, topk=self.topk,
                                 experts=self.experts, first_expert=self.first_expert,
-                                align=self.align, dtype=self.dtype, id_bytes=id_bytes,
+                                align=self.align, dtype=self.dtype,
+                                id_bytes=id_bytes or self.id_bytes,
                                 token_stride=self.token_stride, row_stride=self.row_stride)
 
     def _wide_ids(self):
@@ -596,6 +598,17 @@ class MoeProblem(_CProblem):
         if wide is None or wide[0] is not c:
             wide = self.__dict__["_wide"] = (c, ctypes.byref(self._build(8)))
         return wide[1]
+
+
+def _expert_ids(ids, slots: int, problem, device: Optional[int]):
+    """The address of ``ids`` and the problem's pointer for their width: a
+    tensor's type, or problem.id_bytes for an address."""
+    wide = getattr(ids, "dtype", None) is _TYPES["i64"]
+    if problem.id_bytes and ids is not None and ids.__class__ is not int and (
+            wide != (problem.id_bytes == 8)):
+        raise ValueError(f"expert_ids has dtype {ids.dtype}, id_bytes is {problem.id_bytes}")
+    return (_buffer(ids, "expert_ids", slots, "i64" if wide else "i32", device),
+            problem._wide_ids() if wide else problem._pointer())
 
 
 def _moe_sizes(problem: MoeProblem) -> tuple[int, int]:
@@ -619,23 +632,22 @@ def moe_workspace_bytes(problem: MoeProblem) -> int:
 def moe_sort(expert_ids, *, counts, offsets, row_of_slot, slot_of_row, problem: MoeProblem,
              workspace=None, stream=None, device: int = 0) -> None:
     """Sorts the (token, choice) slots by expert, stably (async).
-    ``expert_ids`` [tokens, topk] int32 or int64; writes int32 ``counts``
+    ``expert_ids`` [tokens, topk] int32 or int64 (an address: problem.id_bytes
+    each); writes int32 ``counts``
     [experts], ``offsets`` [experts + 1], ``row_of_slot`` [tokens, topk] and
     ``slot_of_row`` [moe_rows(problem)]; -1 marks slots whose expert is
     elsewhere and rows without a slot. ``workspace``: moe_workspace_bytes()."""
     where = None if stream is None else device
     rows, need = _moe_sizes(problem)
     slots, experts = problem.tokens * problem.topk, problem.experts
-    wide = getattr(expert_ids, "dtype", None) is _TYPES["i64"]
+    ids, pointer = _expert_ids(expert_ids, slots, problem, where)
     check(lib().megacu_cuda_moe_sort(
-        _launch_view(stream, device, None),
-        _buffer(expert_ids, "expert_ids", slots, "i64" if wide else "i32", where),
+        _launch_view(stream, device, None), ids,
         _buffer(counts, "counts", experts, "i32", where),
         _buffer(offsets, "offsets", experts + 1, "i32", where),
         _buffer(row_of_slot, "row_of_slot", slots, "i32", where),
         _buffer(slot_of_row, "slot_of_row", rows, "i32", where),
-        _buffer(workspace, "workspace", need, "u8", where) if need else None,
-        problem._wide_ids() if wide else problem._pointer()))
+        _buffer(workspace, "workspace", need, "u8", where) if need else None, pointer))
 
 
 def _token_rows(x, name: str, p: MoeProblem, where: Optional[int]) -> Optional[int]:
@@ -873,12 +885,13 @@ class MoeMlp(_CProblem):
     up_alpha: float = 1.0
     down_alpha: float = 1.0
     timeout_ns: int = 0
+    id_bytes: int = 0   # as MoeProblem's
 
     def _build(self, id_bytes: int = 0):
         return _capi.MoeMlpProblem(
             tokens=self.tokens, hidden=self.hidden, inter=self.inter, topk=self.topk,
             experts=self.experts, first_expert=self.first_expert, dtype=self.dtype,
-            id_bytes=id_bytes, format=self.format, x_scale=self.x_scale,
+            id_bytes=id_bytes or self.id_bytes, format=self.format, x_scale=self.x_scale,
             act_scale=self.act_scale, up_alpha=self.up_alpha, down_alpha=self.down_alpha,
             timeout_ns=self.timeout_ns)
 
@@ -905,15 +918,14 @@ def moe_mlp_fp4(x, expert_ids, weights, gate, gate_scales, up, up_scales, down, 
     aligned); with experts or inter spread over PEs, y is this PE's part of
     the sum."""
     p, where = problem, None if stream is None else device
-    wide = getattr(expert_ids, "dtype", None) is _TYPES["i64"]
     slots = p.tokens * p.topk
+    ids, pointer = _expert_ids(expert_ids, slots, p, where)
     need = moe_mlp_workspace_bytes(p)
     up_need = _operand_bytes(p.experts, p.inter, p.hidden, p.format)
     down_need = _operand_bytes(p.experts, p.hidden, p.inter, p.format)
     check(lib().megacu_cuda_moe_mlp_fp4(
         _launch_view(stream, device, None),
-        _matrix(x, "x", p.tokens, p.hidden, 0, p.dtype, where),
-        _buffer(expert_ids, "expert_ids", slots, "i64" if wide else "i32", where),
+        _matrix(x, "x", p.tokens, p.hidden, 0, p.dtype, where), ids,
         _buffer(weights, "weights", slots, _capi.DTYPE_F32, where),
         _buffer(gate, "gate", up_need[0], "u8", where),
         _buffer(gate_scales, "gate_scales", up_need[1], "u8", where),
@@ -925,8 +937,7 @@ def moe_mlp_fp4(x, expert_ids, weights, gate, gate_scales, up, up_scales, down, 
         _buffer(down_alphas, "down_alphas", p.experts, _capi.DTYPE_F32, where),
         _matrix(y, "y", p.tokens, p.hidden, 0, p.dtype, where),
         _buffer(workspace, "workspace", need, "u8", where),
-        _buffer(events, "events", 256, "u8", where),
-        p._wide_ids() if wide else p._pointer()))
+        _buffer(events, "events", 256, "u8", where), pointer))
 
 
 def events_status(events, stream=None) -> list[int]:

@@ -409,3 +409,47 @@ def test_used_problems_can_be_copied_and_pickled():
             first = dataclasses.fields(q)[0].name
             setattr(q, first, 7)
             assert getattr(q.to_c(), first) == 7 and getattr(p.to_c(), first) != 7
+
+
+@pytest.mark.parametrize("block", [False, True])
+def test_width_of_expert_ids(monkeypatch, block):
+    """A tensor's type is its ids' width; an address has the problem's id_bytes
+    (0: 32 bits), and a tensor of the other type than a given id_bytes is
+    refused."""
+    lib = _capi.load()
+    seen = []
+
+    class Spy:
+        def __getattr__(self, name):
+            fn = getattr(lib, name)
+            if name not in ("megacu_cuda_moe_sort", "megacu_cuda_moe_mlp_fp4"):
+                return fn
+
+            def call(*args):
+                seen.append(args[-1]._obj.id_bytes)
+                return fn(*args)
+
+            return call
+
+    monkeypatch.setattr(mb.api, "lib", lambda: Spy())
+
+    def call(ids, **kw):
+        seen.clear()
+        if block:
+            p = mb.MoeMlp(5, 64, 96, 2, 4, **kw)
+            mb.moe_mlp_fp4(FAKE, ids, *[FAKE] * 8, workspace=FAKE, events=FAKE, problem=p)
+        else:
+            p = mb.MoeProblem(5, 2, 4, **kw)
+            mb.moe_sort(ids, counts=FAKE, offsets=FAKE, row_of_slot=FAKE, slot_of_row=FAKE,
+                        problem=p)
+        return seen[0]
+
+    narrow, wide = (torch.zeros(5, 2, dtype=t) for t in (torch.int32, torch.int64))
+    assert call(narrow) in (0, 4) and call(wide) == 8
+    assert call(FAKE) in (0, 4) and call(FAKE, id_bytes=8) == 8 and call(FAKE, id_bytes=4) == 4
+    assert call(wide, id_bytes=8) == 8 and call(narrow, id_bytes=4) == 4
+    for ids, width in ((narrow, 8), (wide, 4)):
+        with pytest.raises(ValueError, match="expert_ids"):
+            call(ids, id_bytes=width)
+    with pytest.raises(mb.MegacuError):
+        call(FAKE, id_bytes=2)
