@@ -44,7 +44,7 @@ megacu_status check_matrix(megacu_fp4_matrix const *m, int &log2_scale) {
   if (m->cols % 32 != 0) {
     return fail(MEGACU_INVALID_ARGUMENT, 21, "cols must be a multiple of 32 (16-byte rows)");
   }
-  if (m->rows > kMaxDim || m->cols > kMaxDim ||
+  if (m->rows > kMaxDim || m->cols > kMaxDim || m->x_rows > kMaxDim ||
       2 * ceil_div(m->rows, kScaleTileRows) * ceil_div(m->cols, kQuantCols) > 0x7fffffffll) {
     return fail(MEGACU_UNSUPPORTED, 22, "dimension too large");
   }
@@ -271,6 +271,14 @@ megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &
   fp4_plan plan;
   megacu_status const st = make_plan(p, swiglu, 148, plan);
   if (st.code != MEGACU_OK) return st;
+  bool const nv = p.format == MEGACU_FP4_NV;
+  std::int64_t const tiles_k = scale_tiles(p.k, nv);
+  std::int64_t const a_tiles = plan.m_tiles * tiles_k;
+  std::int64_t const b_tiles =
+      std::max(p.experts, 1) * ceil_div(p.n, kScaleTileRows) * tiles_k;
+  if (a_tiles > 0x7fffffffll || b_tiles > 0x7fffffffll) {
+    return fail(MEGACU_UNSUPPORTED, 22, "operand too large");
+  }
   if (p.m == 0) return ok_status();
   void const *const needed[] = {op.a, op.a_scales, op.b, op.b_scales, out, events};
   for (void const *ptr : needed) {
@@ -298,16 +306,8 @@ megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &
   cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (e != cudaSuccess) return cuda_fail(e, 10);
 
-  bool const nv = p.format == MEGACU_FP4_NV;
   std::int64_t const b_rows = std::max(p.experts, 1) * p.n;
   std::uint32_t const b_box = swiglu || plan.pair ? 128 : static_cast<std::uint32_t>(plan.tile_n);
-  std::int64_t const tiles_k = scale_tiles(p.k, nv);
-  std::int64_t const a_tiles = plan.m_tiles * tiles_k;
-  std::int64_t const b_tiles =
-      std::max(p.experts, 1) * ceil_div(p.n, kScaleTileRows) * tiles_k;
-  if (a_tiles > 0x7fffffffll || b_tiles > 0x7fffffffll) {
-    return fail(MEGACU_UNSUPPORTED, 22, "operand too large");
-  }
   std::uint32_t const scale_box = kFp4BlockK / fp4_tile_cols(nv);
   fp4_maps maps;
   if (!encode_fp4_map(&maps.a, op.a, p.m, p.k, kFp4BlockM) ||
@@ -410,9 +410,6 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
     return fail(MEGACU_INVALID_ARGUMENT, 21,
                 "data and scales must be 16-byte aligned, x to its element");
   }
-  if (driver.launch.stream == nullptr) return ok_status();
-  device_guard const guard(driver.launch.device_ordinal);
-  if (guard.status() != cudaSuccess) return cuda_fail(guard.status(), 10);
   fp4_matrix_params prm = matrix_params(m, log2_scale, data, scales, transpose);
   prm.slot_of_row = static_cast<std::int32_t const *>(slot_of_row);
   static_assert(kScaleTileRows == 2 * kQuantRows && kQuantRows == kQuantTRows, "two CTAs deep");
@@ -423,6 +420,9 @@ extern "C" megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, voi
   if (row_ctas * prm.col_tiles > 0x7fffffffll) {
     return fail(MEGACU_UNSUPPORTED, 22, "dimension too large");
   }
+  if (driver.launch.stream == nullptr) return ok_status();
+  device_guard const guard(driver.launch.device_ordinal);
+  if (guard.status() != cudaSuccess) return cuda_fail(guard.status(), 10);
   auto const grid = static_cast<unsigned>(row_ctas * prm.col_tiles);
   auto const stream = static_cast<cudaStream_t>(driver.launch.stream);
   cudaError_t e = cudaSuccess;

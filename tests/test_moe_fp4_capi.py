@@ -453,3 +453,22 @@ def test_width_of_expert_ids(monkeypatch, block):
             call(ids, id_bytes=width)
     with pytest.raises(mb.MegacuError):
         call(FAKE, id_bytes=2)
+
+
+def test_sizes_are_refused_without_a_stream():
+    """A call that only validates refuses what a launch would: the composed
+    block launches nothing before all its parts have passed."""
+    lib = _capi.load()
+    # B's scale tiles past 2^31: 1024 experts x 2^13 row tiles x 2^23 tiles of K
+    huge = ctypes.byref(_gemm(m=128, n=1 << 20, k=1 << 30, experts=1024))
+    assert _status(lib.megacu_cuda_fp4_gemm, *[FAKE] * 9, huge) == (2, 22)
+    # A's: 2^16 row tiles x 2^23
+    huge = ctypes.byref(_gemm(m=1 << 23, n=64, k=1 << 30))
+    assert _status(lib.megacu_cuda_fp4_gemm, *[FAKE] * 9, huge) == (2, 22)
+    # a scatter's CTAs, 32 rows of x x 256 columns each: 2^31 - 2^10, 2^31, and
+    # more rows than a matrix may have
+    for x_rows, want in (((1 << 26) - 32, (0, 0)), (1 << 26, (2, 22)), ((1 << 30) + 1, (2, 22)),
+                         (1 << 62, (2, 22)), ((1 << 63) - 1, (2, 22))):
+        m = _matrix(rows=128, cols=1 << 18)
+        m.topk, m.x_rows, m.scatter = 1, x_rows, 1
+        assert _status(lib.megacu_cuda_fp4_quantize, *[FAKE] * 4, ctypes.byref(m)) == want
