@@ -749,7 +749,8 @@ def fp4_quantize(x, data, scales, *, problem: Fp4Matrix, slot_of_row=None, row_o
     nbytes, sbytes = fp4_sizes(p)
     if topk:
         if x_rows == 0 and x is not None and x.__class__ is not int:
-            x_rows = x.shape[0]
+            dense = p.stride == 0 or p.stride == p.cols
+            x_rows = x.numel() // p.cols if dense else x.shape[0]
         x_ptr = _matrix(x, "x", x_rows, p.cols, p.stride, p.dtype, where)
         key = (topk, x_rows, 0 if row_of_slot is None else 1)
         gathered = p.__dict__.get("_gathered")

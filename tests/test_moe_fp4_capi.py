@@ -472,3 +472,41 @@ def test_sizes_are_refused_without_a_stream():
         m = _matrix(rows=128, cols=1 << 18)
         m.topk, m.x_rows, m.scatter = 1, x_rows, 1
         assert _status(lib.megacu_cuda_fp4_quantize, *[FAKE] * 4, ctypes.byref(m)) == want
+
+
+def test_gathered_rows_of_a_batch_of_sequences(monkeypatch):
+    """x of any dense shape is its rows of `cols` elements, as for the other
+    calls: all of them are there to be gathered or scattered."""
+    lib = _capi.load()
+    seen = []
+
+    class Spy:
+        def __getattr__(self, name):
+            fn = getattr(lib, name)
+            if name != "megacu_cuda_fp4_quantize":
+                return fn
+
+            def call(*args):
+                seen.append(args[-1]._obj.x_rows)
+                return fn(*args)
+
+            return call
+
+    monkeypatch.setattr(mb.api, "lib", lambda: Spy())
+    m = mb.Fp4Matrix(128, 32)
+    data, scales = (torch.zeros(n, dtype=torch.uint8) for n in mb.fp4_sizes(m))
+    for shape in ((2, 3, 32), (6, 32), (192,)):
+        x = torch.zeros(shape, dtype=torch.bfloat16)
+        mb.fp4_quantize(x, data, scales, problem=m, topk=2,
+                        slot_of_row=torch.zeros(128, dtype=torch.int32))
+        mb.fp4_quantize(x, data, scales, problem=m, topk=2,
+                        row_of_slot=torch.zeros(6, 2, dtype=torch.int32))
+        with pytest.raises(ValueError):
+            mb.fp4_quantize(x, data, scales, problem=m, topk=2,
+                            row_of_slot=torch.zeros(5, 2, dtype=torch.int32))
+    assert seen == [6] * 6
+    strided = mb.Fp4Matrix(128, 32, stride=40)
+    wide = torch.zeros(6, 40, dtype=torch.bfloat16)
+    mb.fp4_quantize(wide[:, :32], data, scales, problem=strided, topk=2,
+                    slot_of_row=torch.zeros(128, dtype=torch.int32))
+    assert seen[-1] == 6
