@@ -459,7 +459,7 @@ megacu_status megacu_b200_events_counters(void *events, void *stream,
  * row (-1). Two choices of one token may name the same expert.
  */
 typedef struct megacu_moe_problem {
-  int64_t tokens;       /* 0 is an empty batch; tokens * topk <= 2^30 */
+  int64_t tokens;       /* 0 is an empty batch; tokens * topk <= 2^30, sorted: 2^26 */
   int64_t hidden;       /* elements of a row; not read by the sort */
   int32_t topk;         /* 1..32 */
   int32_t experts;      /* experts held here, 1..1024 */

@@ -636,7 +636,7 @@ def moe_sort(expert_ids, *, counts, offsets, row_of_slot, slot_of_row, problem: 
     each); writes int32 ``counts``
     [experts], ``offsets`` [experts + 1], ``row_of_slot`` [tokens, topk] and
     ``slot_of_row`` [moe_rows(problem)]; -1 marks slots whose expert is
-    elsewhere and rows without a slot. ``workspace``: moe_workspace_bytes()."""
+    elsewhere and rows without a slot. At most 2^26 slots. ``workspace``: moe_workspace_bytes()."""
     where = None if stream is None else device
     rows, need = _moe_sizes(problem)
     slots, experts = problem.tokens * problem.topk, problem.experts

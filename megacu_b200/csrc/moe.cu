@@ -16,6 +16,10 @@ namespace {
 using namespace megacu_b200;
 
 constexpr std::int64_t kMaxSlots = 1ll << 30;
+// Of the sort, whose second launch reads every chunk's histogram in each CTA.
+// With 256 experts 2^24 slots take 0.55 ms and 2^26 6.8, with 1024 experts 2.1
+// and 31; 2^30 would hold the GPU for seconds.
+constexpr std::int64_t kMaxSortSlots = 1ll << 26;
 constexpr std::int32_t kMaxAlign = 1024;
 constexpr int kMaxDevices = 64;
 
@@ -227,6 +231,7 @@ extern "C" megacu_status megacu_cuda_moe_sort(megacu_driver_view driver, void co
     return fail(MEGACU_UNSUPPORTED, 20, "expert ids are 32 or 64 bits");
   }
   std::int64_t const slots = p.tokens * p.topk;
+  if (slots > kMaxSortSlots) return fail(MEGACU_UNSUPPORTED, 22, "a sort of at most 2^26 slots");
   std::int64_t const chunks = chunks_of(slots);
   if (counts == nullptr || offsets == nullptr ||
       (slots > 0 && (expert_ids == nullptr || row_of_slot == nullptr || slot_of_row == nullptr)) ||

@@ -510,3 +510,15 @@ def test_gathered_rows_of_a_batch_of_sequences(monkeypatch):
     mb.fp4_quantize(wide[:, :32], data, scales, problem=strided, topk=2,
                     slot_of_row=torch.zeros(128, dtype=torch.int32))
     assert seen[-1] == 6
+
+
+def test_sort_refuses_more_slots_than_it_is_made_for():
+    """Up to 2^26 slots: its second launch's work grows with the square. Calls
+    on an order that another sort made have no such bound."""
+    lib = _capi.load()
+    for tokens, want in ((1 << 23, (0, 0)), ((1 << 23) + 1, (2, 22)), (1 << 27, (2, 22))):
+        p = ctypes.byref(_moe(tokens=tokens, topk=8))
+        assert _status(lib.megacu_cuda_moe_sort, *[FAKE] * 6, p) == want
+        assert _status(lib.megacu_cuda_moe_dispatch, *[FAKE] * 3, p) == (0, 0)
+        st = lib.megacu_b200_moe_sizes(p, (ctypes.c_int64 * 2)())
+        assert (st.code, st.detail) == (0, 0)
