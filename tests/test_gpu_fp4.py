@@ -781,3 +781,15 @@ def test_given_up_waits_end_the_call_and_spare_the_next(m, n, k, experts, tile_n
             pass
         assert torch.equal(run(), want)
         mb.events_status(events, _stream())
+
+
+@pytest.mark.parametrize("tokens,fmt,dtype", [(3000, mb.FP4_MX, mb.DTYPE_F32),
+                                              (4097, mb.FP4_NV, mb.DTYPE_BF16),
+                                              (40, mb.FP4_NV, mb.DTYPE_F32)])
+def test_routed_mlp_block_of_long_batches_and_in_f32(tokens, fmt, dtype):
+    """The same where the block's sort takes two launches and a workspace (more
+    than 8192 slots), and in 32 bits."""
+    p = mb.MoeMlp(tokens, 320, 160, 3, 6)
+    assert (mb.moe_workspace_bytes(mb.MoeProblem(tokens, p.topk, p.experts, align=128)) > 0) == (
+        tokens * p.topk > 8192)
+    test_routed_mlp_block_is_its_calls(tokens, fmt, dtype, torch.int64)
