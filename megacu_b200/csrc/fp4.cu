@@ -129,12 +129,16 @@ struct fp4_plan {
   std::int64_t m_tiles = 0, n_tiles = 0;
 };
 
+// The plan is made for a B200's SMs, whatever the device: it decides what is
+// refused too, also by calls without a stream. The grid goes by the device.
+constexpr int kPlanSms = 148;
+
 // Clusters of `split` CTAs, one CTA per SM, that run at once: an SM's cluster
 // stays within its GPC, and a B200's GPCs hold 33 clusters of 4 and 15 of 8
 // (the occupancy query's answer; 16 x 2048 x 4096 split in eight, 16 clusters,
 // took 11.6 us against 6.7 for 15).
-std::int64_t clusters_at_once(int split, int sms) {
-  return split == 8 ? 15 : split == 4 ? 33 : sms / split;
+std::int64_t clusters_at_once(int split) {
+  return split == 8 ? 15 : split == 4 ? 33 : kPlanSms / split;
 }
 
 // Tile width and K split with the least time on the busiest SM, in us, fitted
@@ -144,7 +148,13 @@ std::int64_t clusters_at_once(int split, int sms) {
 // and the exchange of a split, which grows with the tile's accumulators.
 // 16 x 8192 x 3584: tile_n 64 takes 6.4 us, 128 6.5, 256 8.7, 128 split in two
 // 8.0, 256 split in four 9.2.
-megacu_status make_plan(megacu_fp4_gemm_problem const &p, bool swiglu, int sms, fp4_plan &out) {
+// The costs are a single CTA's; whether tiles run as pairs is decided after the
+// choice. It holds past the fit all the same: with 129 to 2000 rows the choice
+// was within 1 % of the best of 256, 128 and 64 columns, whole or split, at
+// N x K 8192 x 3584, 4096 x 4096 and 1792 x 8192 (1000 rows 15.5, 11.0 and
+// 11.4 us), and at 14336 x 1024 but for 129 to 256 rows (7.0 us, 128 columns
+// 6.0).
+megacu_status make_plan(megacu_fp4_gemm_problem const &p, bool swiglu, fp4_plan &out) {
   std::int64_t const k_blocks = ceil_div(p.k, kFp4BlockK);
   double best = -1.0;
   for (int tile_n : {256, 128, 64}) {
@@ -156,7 +166,7 @@ megacu_status make_plan(megacu_fp4_gemm_problem const &p, bool swiglu, int sms, 
       std::int64_t const m_tiles = ceil_div(p.m, kFp4BlockM);
       std::int64_t const n_tiles = ceil_div(p.n, swiglu ? tile_n / 2 : tile_n);
       std::int64_t const waves =
-          std::max<std::int64_t>(ceil_div(m_tiles * n_tiles, clusters_at_once(split, sms)), 1);
+          std::max<std::int64_t>(ceil_div(m_tiles * n_tiles, clusters_at_once(split)), 1);
       double const rows = static_cast<double>(std::min<std::int64_t>(p.m, kFp4BlockM));
       double const exchange = split > 1 ? 1.5 + 0.035 * rows * tile_n / 256 : 0.0;
       double const cost = start + 0.6 * static_cast<double>(waves - 1) +
@@ -269,7 +279,7 @@ megacu_status run_product(megacu_driver_view const &driver, fp4_operands const &
     return fail(MEGACU_UNSUPPORTED, 22, "rows by expert come in tiles of 128");
   }
   fp4_plan plan;
-  megacu_status const st = make_plan(p, swiglu, 148, plan);
+  megacu_status const st = make_plan(p, swiglu, plan);
   if (st.code != MEGACU_OK) return st;
   bool const nv = p.format == MEGACU_FP4_NV;
   std::int64_t const tiles_k = scale_tiles(p.k, nv);
