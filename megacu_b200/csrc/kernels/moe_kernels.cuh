@@ -60,9 +60,9 @@ __device__ __forceinline__ void clear_rows(moe_sort_params const &p) {
 template <class Id>
 __global__ void __launch_bounds__(kMoeSortThreads) moe_count_kernel(moe_sort_params p) {
   extern __shared__ std::int32_t moe_smem[];
-  grid_start_next();
   for (int e = threadIdx.x; e < p.experts; e += blockDim.x) moe_smem[e] = 0;
   grid_wait();
+  grid_start_next();
   __syncthreads();
   std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
   std::int64_t const end = min(begin + p.chunk, p.slots);
@@ -116,7 +116,6 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_par
   int const tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   bool const chunked = gridDim.x > 1;
 
-  grid_start_next();
   std::int64_t const begin = static_cast<std::int64_t>(blockIdx.x) * p.chunk;
   std::int32_t const here = static_cast<std::int32_t>(min(p.chunk + begin, p.slots) - begin);
   std::int32_t const part = (p.chunk + threads - 1) / threads * 32;
@@ -136,6 +135,10 @@ __global__ void __launch_bounds__(kMoeSortThreads) moe_place_kernel(moe_sort_par
     local[s] = static_cast<std::int16_t>(e);
     if (e >= 0) atomicAdd(&mine[e], 1);
   }
+  // Not earlier: a product two launches on would start its CTAs while this one
+  // still holds its SM, and its last CTA would wait for it (a routed block of 64
+  // tokens 97 -> 102 us).
+  grid_start_next();
   __syncthreads();
 
   // total[e] = slots of e anywhere, start[e] = slots of e in earlier chunks.
