@@ -559,7 +559,8 @@ megacu_status megacu_b200_fp4_sizes(const megacu_fp4_matrix *matrix, int64_t siz
  * megacu_cuda_moe_sort writes it) rows whose entry is negative are left as
  * they were, scales included, and x is gathered when topk > 0 (an entry that
  * names no row of x counts as negative); NULL: every row. With scatter the
- * index is row_of_slot, and entries outside [0, rows) name no row.
+ * index is row_of_slot, entries outside [0, rows) name no row, and two entries
+ * must not name the same one.
  */
 megacu_status megacu_cuda_fp4_quantize(megacu_driver_view driver, const void *x,
                                        const void *slot_of_row, void *data, void *scales,
@@ -587,7 +588,8 @@ typedef struct megacu_fp4_gemm_problem {
 } megacu_fp4_gemm_problem;
 
 /* Bytes of `events` of the products: zero-filled once, then reused; it holds
- * only the error word that megacu_b200_events_status reads and clears
+ * only the error word that megacu_b200_events_status reads and clears; until
+ * then waits of later calls on it may give up as well
  * (detail 41; info[0] = tile, info[2] = which wait: 51 producer's free stage,
  * 52 MMA's free accumulator, 53 MMA's full stage, 54 epilogue's accumulator). */
 megacu_status megacu_b200_fp4_events_bytes(int64_t *bytes);
@@ -631,8 +633,8 @@ typedef struct megacu_moe_mlp_problem {
   int32_t format;       /* enum megacu_fp4_format, of weights and activations */
   float x_scale;        /* powers of two that multiply x and act before they are */
   float act_scale;      /* quantised (undone in the products); 0 = 1 */
-  float up_alpha;       /* factor of gate and up, 1 / the weights' scale */
-  float down_alpha;     /* factor of down */
+  float up_alpha;       /* factor of gate and up, 1 / the weights' scale; 0 gives zeros */
+  float down_alpha;     /* factor of down, likewise */
   uint64_t timeout_ns;  /* bound of every wait inside the products; 0 = 4 s */
 } megacu_moe_mlp_problem;
 
