@@ -571,8 +571,6 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   std::uint64_t *const acc_full = empty + kStages;
   std::uint64_t *const acc_free = acc_full + 1;
   auto *const tmem_slot = reinterpret_cast<std::uint32_t *>(acc_free + 1);
-  // In a pair's leader: whether its MMA warp gave up, and 1 + the follower's
-  // loads once its producer has ended.
   // Two words of a pair's leader: whether its MMA warp gave up, and 1 + the
   // follower's loads once its producer has ended. Their address is computed
   // anew at each use, so that the epilogue holds no register for it.
@@ -867,7 +865,6 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
         if constexpr (kPair) {
           if (!leader) detail::wait_commit(acc_full, tile_index & 1u);
         }
-        // The leader's MMA warp waits for its own arrival of a last commit.
         break;
       }
       __syncwarp();
